@@ -1,0 +1,200 @@
+"""The draw with temperature, top-k, top-p and min-p from given numbers, against its definition in 64 bits (numpy): tokens are
+equal, log-probabilities within 2^-24 of their value (the rounding) and 2^-20 (exponentials and differences in 32 bits: 2^-23 each of
+what they stand for, a logarithm's error is the relative error of the sum, and a sum of positive terms keeps theirs)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tlie_amd import ops
+from tlie_amd.errors import EngineError
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def oracle(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
+    tokens, logprobs = [], []
+    for row in range(logits.shape[0]):
+        values = logits[row].double().numpy()
+        if np.isnan(values).any() or (values == np.inf).any() or (values == -np.inf).all():
+            tokens.append(-1), logprobs.append(math.nan)
+            continue
+        order = np.lexsort((np.arange(values.size), -values))
+        with np.errstate(all="ignore"):
+            gap = values[order] - values[order[0]]
+            t = float(temperature[row]) if temperature is not None else 0.0
+            pick = 0
+            if t > 0:
+                weights = np.where(gap == -np.inf, 0.0, np.exp(np.maximum(gap / t, -800.0)))
+                kept = int((weights > 2.0 ** -45).sum())           # (lighter ones are never drawn, as documented)
+                if top_k is not None and int(top_k[row]) > 0:
+                    kept = min(kept, int(top_k[row]))
+                if top_p is not None and float(top_p[row]) < 1.0:
+                    sums = np.cumsum(weights[:kept])
+                    kept = min(kept, int((sums < float(top_p[row]) * sums[-1]).sum()) + 1)
+                if min_p is not None and float(min_p[row]) > 0.0:
+                    kept = max(1, int((weights[:kept] >= float(min_p[row])).sum()))
+                sums = np.cumsum(weights[:kept])
+                u = float(uniform[row])
+                pick = min(kept - 1, int((sums <= max(u, 0.0) * sums[-1]).sum())) if u == u else 0
+            tokens.append(int(order[pick]))
+            logprobs.append(gap[pick] - math.log(np.exp(gap).sum()))
+    return np.array(tokens), np.array(logprobs)
+
+
+def check(logits, uniform, **filters):
+    on = lambda value: value.to(DEV) if value is not None else None
+    got, logprob = ops.sample_filtered(on(logits), on(uniform), **{name: on(value) for name, value in filters.items()}, logprobs=True)
+    want, want_logprob = oracle(logits, uniform, **filters)
+    np.testing.assert_array_equal(got.cpu().numpy(), want)
+    logprob = logprob.double().cpu().numpy()
+    assert (np.isnan(logprob) == np.isnan(want_logprob)).all()
+    live = ~np.isnan(want_logprob)
+    assert (np.abs(logprob - want_logprob)[live] <= 2.0 ** -24 * np.abs(want_logprob[live]) + 2.0 ** -20).all()
+    return got
+
+
+def rows_of(seed, rows, vocab, spread=2.5):
+    gen = torch.Generator().manual_seed(seed)
+    logits = spread * torch.randn((rows, vocab), generator=gen)
+    logits += (torch.rand((rows, vocab), generator=gen) < 20.0 / vocab) * 8.0 * torch.rand((rows, vocab), generator=gen)
+    return logits, torch.rand((rows,), generator=gen), gen
+
+
+def filters_of(gen, rows):
+    choose = lambda values: torch.tensor(values)[torch.randint(0, len(values), (rows,), generator=gen)]
+    return dict(temperature=choose([0.0, 0.3, 0.7, 1.0, 1.0, 1.7]), top_k=choose([0, 0, 1, 5, 50, 700, 1 << 30, -1]).int(),
+                top_p=choose([1.0, 1.0, 0.99, 0.9, 0.5, 0.01]), min_p=choose([0.0, 0.0, 0.001, 0.05, 0.6]))
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (40, 5), (64, 255), (64, 1000), (33, 2049), (64, 4097), (200, 8191), (64, 32000), (3, 50261),
+                                        (24, 128256), (2, 300001)])
+def test_all_filters(rows, vocab):
+    logits, uniform, gen = rows_of(vocab, rows, vocab)
+    check(logits, uniform, **filters_of(gen, rows))
+
+
+@pytest.mark.parametrize("name", ["temperature", "top_k", "top_p", "min_p"])
+def test_one_filter_at_a_time(name):
+    logits, uniform, gen = rows_of(3, 48, 3001)
+    filters = filters_of(gen, 48)
+    check(logits, uniform, **{"temperature": torch.full((48,), 0.9), name: filters[name]})
+
+
+def test_without_a_temperature_the_first_maximum():
+    logits, uniform, _ = rows_of(4, 9, 700)
+    logits[3, 600] = logits[3, 20] = 50.0
+    logits[4, 1:4] = 0.0
+    logits[4] = -logits[4].abs()
+    logits[4, 1], logits[4, 3] = -0.0, 0.0
+    got = check(logits, uniform)
+    assert got[3] == 20 and got[4] in (1, 2)
+    check(logits, uniform, temperature=torch.full((9,), -1.0))
+
+
+@pytest.mark.parametrize("rounding", ["bfloat16", "halves"])
+def test_equal_logits(rounding):
+    """Ties go to the lower index, also where top_k and the draw cut through them."""
+    logits, uniform, gen = rows_of(5, 64, 9000)
+    logits = logits.bfloat16().float() if rounding == "bfloat16" else (logits * 2).round() / 2
+    check(logits, uniform, **filters_of(gen, 64))
+
+
+@pytest.mark.parametrize("vocab", [7, 1000, 20000])
+def test_rows_of_one_value(vocab):
+    """More tokens of one class than are sorted: the way without a list."""
+    logits = torch.zeros(12, vocab)
+    logits[4:8, vocab // 2] = -1.0
+    uniform = torch.tensor([0.0, 0.25, 0.5, 1 - 2.0 ** -24] * 3)
+    k = torch.tensor([0, 3, vocab - 1, 0, 0, 3, vocab - 1, 0, 2500, 2500, 0, 0]).int()
+    p = torch.tensor([1.0] * 4 + [0.75] * 4 + [1.0, 0.625, 0.25, 0.4375])
+    check(logits, uniform, temperature=torch.ones(12), top_k=k, top_p=p, min_p=torch.tensor([0.0, 0.5] * 6))
+
+
+@pytest.mark.parametrize("t", [1e-30, 1e-4, 0.05, 5.0, 300.0, 1e20, math.inf])
+def test_far_temperatures(t):
+    logits, uniform, gen = rows_of(6, 16, 5000)
+    filters = filters_of(gen, 16)
+    filters["temperature"] = torch.full((16,), t)
+    check(logits, uniform, **filters)
+
+
+def test_numbers_at_the_ends():
+    logits, _, _ = rows_of(7, 24, 2500)
+    uniform = torch.tensor([0.0, 2.0 ** -24, 0.5, 1 - 2.0 ** -24, 1.0, 1.5, -1.0, math.nan] * 3)
+    ones = torch.ones(24)
+    check(logits, uniform, temperature=ones, top_p=torch.tensor([1.0, 0.9, 0.0] * 8))
+    check(logits, uniform, temperature=ones, top_p=torch.tensor([math.nan, 2.0, -1.0] * 8), min_p=torch.tensor([1.0, 2.0, math.nan, 0.0] * 6))
+
+
+def test_tokens_that_cannot_be_drawn():
+    logits, uniform, gen = rows_of(8, 32, 6000)
+    masked = torch.rand((32, 6000), generator=gen) < 0.9
+    logits[masked] = -math.inf
+    logits[5] = -math.inf
+    logits[5, 77] = 3.0
+    logits[6] = -math.inf                                           # nothing is left
+    logits[7, 9] = math.nan
+    logits[8, 9] = math.inf
+    logits[9, 10:] = torch.finfo(torch.float32).min
+    logits[10] = torch.finfo(torch.float32).min
+    logits[10, 5] = torch.finfo(torch.float32).max
+    filters = filters_of(gen, 32)
+    got = check(logits, uniform, **filters)
+    assert got[5] == 77 and got[6] == -1 and got[7] == -1 and got[8] == -1 and got[10] == 5
+
+
+def test_the_same_row_in_any_batch_and_from_call_to_call():
+    logits, uniform, gen = rows_of(9, 300, 7001)
+    filters = filters_of(gen, 300)
+    got = check(logits, uniform, **filters)
+    pick = torch.tensor([7, 299, 0, 31])
+    few = ops.sample_filtered(logits[pick].to(DEV), uniform[pick].to(DEV), **{name: value[pick].to(DEV) for name, value in filters.items()})
+    assert torch.equal(few.cpu(), got.cpu()[pick])
+
+
+def test_draws_follow_the_probabilities():
+    """A thousand evenly spaced numbers give each token as often as its share says, within one at each end."""
+    logits = torch.tensor([0.1, 2.0, -1.0, 1.0, 0.7])
+    numbers = (torch.arange(1000) + 0.5) / 1000
+    got = ops.sample_filtered(logits.repeat(1000, 1).to(DEV), numbers.to(DEV), torch.ones(1000, device=DEV)).cpu()
+    share = torch.softmax(logits.double(), 0)
+    for token in range(5):
+        assert abs(int((got == token).sum()) - 1000 * float(share[token])) <= 1
+
+
+def test_outputs_streams_and_replays():
+    logits, uniform, gen = rows_of(10, 20, 3000)
+    filters = {name: value.to(DEV) for name, value in filters_of(gen, 20).items()}
+    logits, uniform = logits.to(DEV), uniform.to(DEV)
+    want, want_logprob = ops.sample_filtered(logits, uniform, **filters, logprobs=True)
+    out, out_logprob = torch.empty_like(want), torch.empty_like(want_logprob)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.sample_filtered(logits, uniform, **filters, logprobs=True, out=out, out_logprobs=out_logprob)
+    torch.cuda.current_stream().wait_stream(side)
+    assert got[0] is out and got[1] is out_logprob and torch.equal(out, want) and torch.equal(out_logprob, want_logprob)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded, recorded_logprob = ops.sample_filtered(logits, uniform, **filters, logprobs=True)
+    for round in range(3):
+        uniform.copy_(torch.rand((20,), generator=gen).to(DEV))
+        graph.replay()
+        replayed, replayed_logprob = recorded.clone(), recorded_logprob.clone()
+        want, want_logprob = ops.sample_filtered(logits, uniform, **filters, logprobs=True)
+        assert torch.equal(replayed, want) and torch.equal(replayed_logprob, want_logprob)
+
+
+def test_refusals_and_no_rows():
+    logits, uniform = torch.zeros(4, 10, device=DEV), torch.zeros(4, device=DEV)
+    assert ops.sample_filtered(logits[:0], uniform[:0]).shape == (0,)
+    bad = [dict(logits=logits.bfloat16()), dict(logits=logits[0]), dict(logits=logits[:, :0]), dict(logits=torch.zeros(10, 4, device=DEV).t()), dict(uniform=None),
+           dict(uniform=uniform.double()), dict(uniform=uniform[:3]), dict(uniform=uniform.cpu()), dict(top_k=torch.zeros(4, device=DEV)),
+           dict(top_p=torch.zeros(5, device=DEV)), dict(min_p=torch.zeros(4, 1, device=DEV)), dict(temperature=torch.ones(4, dtype=torch.float64, device=DEV)),
+           dict(out=torch.zeros(4, device=DEV)), dict(out_logprobs=uniform)]
+    for change in bad:
+        with pytest.raises(EngineError):
+            ops.sample_filtered(**{"logits": logits, "uniform": uniform, **change})

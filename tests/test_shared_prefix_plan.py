@@ -1,0 +1,92 @@
+"""The work list of attention over shared prefixes: every (token, head, key) in exactly one item, every part written once; and
+what the plan refuses."""
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from tlie_amd import ops
+from tlie_amd.errors import EngineError
+
+
+def drawn_step(rng):
+    """Cumulative token counts, lengths, groups and every sequence's prefix."""
+    sequences = rng.randint(0, 12)
+    counts = [rng.choice([0, 1, 1, 1, rng.randint(1, 40)]) for _ in range(sequences)]
+    groups, prefix, at = [], [0] * sequences, 0
+    while at < sequences:
+        count = rng.randint(1, 4)
+        if rng.random() < 0.6 and at + count <= sequences:
+            groups.append((at, count, rng.choice([0, 1, 16, 100, 1000, 5000])))
+            prefix[at:at + count] = [groups[-1][2]] * count
+            at += count
+        else:
+            at += 1
+    lengths = [prefix[s] + counts[s] + rng.choice([0, 1, 50, 1000]) if counts[s] else rng.randint(0, 100) for s in range(sequences)]
+    rng.shuffle(groups)
+    return np.concatenate([[0], np.cumsum(counts)]).astype(np.int64), np.array(lengths, dtype=np.int64), groups, prefix
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 4, 64), (32, 8, 128), (8, 8, 256), (40, 1, 64), (12, 4, 48)])
+def test_every_key_of_every_column_is_in_one_item(heads, kv_heads, dim):
+    rng, group = random.Random(heads), heads // kv_heads
+    for _ in range(40):
+        start, lengths, groups, prefix = drawn_step(rng)
+        items, part_first, wide = ops.shared_prefix_items(start, lengths, groups, heads, kv_heads, dim)
+        covered, written = {}, set()
+        for sequence, tok0, tokens, col0, low, high, own, part in items.tolist():
+            assert low < high
+            for column in range(col0, min(col0 + (16 * wide if tokens * group - col0 > 16 else 16), tokens * group)):
+                token, head = tok0 + column // group, column % group
+                seq = int(np.searchsorted(start, token, side="right") - 1)
+                position = lengths[seq] - start[seq + 1] + token
+                assert (seq == sequence and low >= prefix[seq]) if own else high <= prefix[seq]
+                end = min(high, position + 1) if own else high
+                if part < part_first[token + 1] - part_first[token]:
+                    assert (part_first[token] + part, head) not in written
+                    written.add((part_first[token] + part, head))
+                    covered.setdefault((token, head), []).append((low, max(low, end)))
+                else:
+                    assert end <= low                          # nothing the token sees
+        for token in range(int(start[-1])):
+            seq = int(np.searchsorted(start, token, side="right") - 1)
+            for head in range(group):
+                end = 0
+                for low, high in sorted(covered[token, head]):
+                    assert low == end or high == low
+                    end = max(end, high)
+                assert end == lengths[seq] - start[seq + 1] + token + 1
+                assert all((part, head) in written for part in range(part_first[token], part_first[token + 1]))
+
+
+@pytest.mark.parametrize("start,lengths,groups,heads", [
+    ([0, 1], [1, 1], [], 8),                       # lengths of another count
+    ([1, 2], [4], [], 8),                          # not from 0
+    ([0, 2, 1], [4, 4], [], 8),                    # counting down
+    ([0, 3], [2], [], 8),                          # shorter than what it brings
+    ([0, 1, 2], [9, 9], [(0, 2, 9)], 8),           # a token inside its prefix
+    ([0, 1, 2], [9, 9], [(0, 2, 4), (1, 1, 4)], 8),     # a sequence in two groups
+    ([0, 1, 2], [9, 9], [(1, 2, 4)], 8),           # a group past the step
+    ([0, 1, 2], [9, 9], [(0, 0, 4)], 8),           # a group of none
+    ([0, 1, 2], [9, 9], [(0, 2, -1)], 8),          # a negative prefix
+    ([0, 1, 2], [9, 9], [], 9),                    # heads that do not share kv heads evenly
+])
+def test_plans_that_are_refused(start, lengths, groups, heads):
+    with pytest.raises(EngineError):
+        ops.shared_prefix_plan(start, lengths, groups, heads, 4, 64, torch.bfloat16, "cpu")
+
+
+def test_other_types_are_refused():
+    with pytest.raises(EngineError):
+        ops.shared_prefix_plan([0, 1], [4], [], 8, 4, 64, torch.float16, "cpu")
+
+
+def test_arguments_on_the_host_are_refused():
+    logits, number = torch.zeros(2, 8), torch.zeros(2)
+    with pytest.raises(EngineError):
+        ops.sample_filtered(logits, number)
+    plan = ops.SharedPrefixPlan(torch.zeros(1, 8, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 1, 1, 1, 1, 1, (2, 1, 16, torch.float32))
+    with pytest.raises(EngineError):
+        ops.attention_shared_prefix(torch.zeros(1, 32), torch.zeros(1, 2, 1, 256), torch.zeros(1, 1, dtype=torch.int32),
+                                    torch.zeros(1, dtype=torch.int32), plan, 2, 1, 16, 1.0)

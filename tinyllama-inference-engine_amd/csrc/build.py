@@ -19,7 +19,7 @@ SOURCES = ["elementwise.hip", "rope_cache.hip", "attention_generic.hip", "attent
            "gemm_skinny.hip", "gemm_rows.hip", "gemm_tiles.hip", "sampling.hip", "library_gemm.hip", "probes.hip",
            "block_linear.hip", "latent.hip", "recurrence.hip", "heads.hip", "mlstm.hip", "routing.hip", "side.hip",
            "decay_scan.hip", "canon.hip", "streams.hip", "short_conv.hip",
-           "gated_scan.hip", "post_norm.hip"]
+           "gated_scan.hip", "post_norm.hip", "attention_prefix.hip", "draw.hip"]
 HEADERS = ["common.h", "no_alloc.h"]
 LIBRARY = "libtlie_hip.so"
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-shared",

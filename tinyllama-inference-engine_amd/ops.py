@@ -2089,6 +2089,69 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor | None = None, top_p:
     return out
 
 
+def _one_device(what: str, *tensors) -> None:
+    """All tensors (None: absent) lie on the current device, whose current stream the kernels go to."""
+    current = torch._C._cuda_getDevice()
+    for tensor in tensors:
+        if tensor is not None and tensor.device.index != current:
+            raise invalid_argument(f"{what}: a tensor lies on {tensor.device}, the current device is cuda:{current}")
+
+
+DRAW_MAX_VOCAB = (1 << 24) - 1
+
+
+def draw_parts(rows: int, vocab: int) -> int:
+    """Into how many parts `sample_filtered` cuts each row: a thousand workgroups in all, of 2048 tokens at least each."""
+    return max(1, min(1024 // max(rows, 1), 16, (vocab + 2047) // 2048))
+
+
+def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+                    top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None, logprobs: bool = False,
+                    out: torch.Tensor | None = None, out_logprobs: torch.Tensor | None = None):
+    """One token per row of float32 logits [rows, vocab], from given random numbers `uniform` (float32 [rows], in [0, 1)).
+
+    Tokens stand in descending order of their logits, equal ones by index, with weights exp((logit - max) / temperature).  Kept are
+    the first top_k (int32; 0 or less: all); of those the shortest beginning that holds at least top_p of their weight (float32;
+    1 or more: all); of those the ones whose weight is at least min_p of the largest (float32; 0: all); the first token always.
+    The token is the first in this order at which the running sum of the kept weights passes uniform times their sum.
+    A row whose temperature is not positive (and every row when none is given) takes the first token.  Each of temperature,
+    top_k, top_p and min_p holds one entry a row.  A logit of -inf is a token that cannot be drawn; a row with a NaN or +inf, or
+    of -inf alone, gives -1 (and a NaN).  Weights are summed as whole numbers of 2^-44 of the largest (fewer bits beyond a vocabulary of
+    262144): what is lighter than half of that is never drawn, and the same inputs give the same token in any batch.
+    logprobs: also returns float32 [rows], log softmax(logits)[token] of the logits as they are, without temperature and filters.
+    out (int32 [rows]), out_logprobs (float32 [rows]): to write into, else new tensors."""
+    _device_tensor(logits, "logits", torch.float32)
+    if logits.dim() != 2:
+        raise invalid_shape("sample_filtered takes logits [rows, vocab]")
+    rows, vocab = logits.shape
+    if not 0 < vocab <= DRAW_MAX_VOCAB or rows > 65535:
+        raise invalid_shape(f"sample_filtered takes 1 to {DRAW_MAX_VOCAB} tokens and up to 65535 rows, not {list(logits.shape)}")
+    if uniform is None:
+        raise invalid_argument("sample_filtered needs a random number per row")
+    for name, tensor, dtype in (("uniform", uniform, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                                ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("out", out, torch.int32),
+                                ("out_logprobs", out_logprobs, torch.float32)):
+        if tensor is not None:
+            _device_tensor(tensor, name, dtype)
+            if tensor.shape != (rows,):
+                raise invalid_shape(f"sample_filtered: {name} needs one entry per row")
+    if out_logprobs is not None and not logprobs:
+        raise invalid_argument("sample_filtered: out_logprobs goes with logprobs")
+    _one_device("sample_filtered", logits, uniform, temperature, top_k, top_p, min_p, out, out_logprobs)
+    if out is None:
+        out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    if logprobs and out_logprobs is None:
+        out_logprobs = torch.empty((rows,), dtype=torch.float32, device=logits.device)
+    if rows > 0:
+        parts = draw_parts(rows, vocab)
+        size = library().tlie_draw_scratch_bytes
+        size.restype = ctypes.c_longlong
+        scratch = torch.empty((size(rows, parts),), dtype=torch.uint8, device=logits.device)
+        _check(library().tlie_draw(_ptr(logits), rows, vocab, _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), parts,
+                                   _ptr(scratch), _ptr(out), _ptr(out_logprobs), _stream()), "sample_filtered")
+    return (out, out_logprobs) if logprobs else out
+
+
 def feed_tokens(tokens: torch.Tensor, source: torch.Tensor, sampled: torch.Tensor, vocab: int) -> None:
     """tokens[i] = sampled[source[i]] wherever source[i] >= 0, on the device, brought into the
     vocabulary's range 0 .. vocab - 1 (a sample of -1 marks a row of logits that held a NaN or an
@@ -2656,6 +2719,171 @@ def attention_mfma(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tens
                                          int(window) if window else 0, int(chunk) if chunk else 0, _ptr(sink),
                                          ctypes.c_float(scale), waves, int(bool(shared)), _ptr(order), _stream()),
            "attention_mfma")
+    return out
+
+
+# ---- attention for sequences that share their first positions -----------------------------------------
+
+
+@dataclass
+class SharedPrefixPlan:
+    """The work of `attention_shared_prefix` for one step, made by `shared_prefix_plan` on the host and read by every layer."""
+    items: torch.Tensor            # int32 [n, 8] (sequence, first token, tokens, first column, first key, end of the keys, own, part)
+    part_first: torch.Tensor       # int32 [tokens + 1]: the first part of each token
+    tokens: int
+    parts: int
+    wide: int                      # column groups of 16 that a tile has
+    sequences: int
+    longest: int
+    sizes: tuple                   # (num_heads, num_kv_heads, head_dim, dtype)
+
+
+PREFIX_ALIGN = 128         # keys that the four waves of a workgroup take in one turn (bfloat16)
+
+
+def prefix_wide(head_dim: int) -> int:
+    return 2 if head_dim <= 128 else 1
+
+
+def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, compute_units: int = 256):
+    """The host's half of `shared_prefix_plan`: (items [n, 8], part_first [tokens + 1], wide), int32 arrays of numpy."""
+    import numpy as np
+    seq_start, seq_len = np.asarray(seq_start, dtype=np.int64), np.asarray(seq_len, dtype=np.int64)
+    if seq_start.ndim != 1 or seq_len.ndim != 1 or seq_start.shape[0] != seq_len.shape[0] + 1:
+        raise invalid_shape("shared_prefix_plan takes seq_start [sequences + 1] and seq_len [sequences]")
+    counts = seq_start[1:] - seq_start[:-1]
+    if seq_start[0] != 0 or (counts < 0).any() or (seq_len < counts).any():
+        raise invalid_argument("shared_prefix_plan: seq_start must count up from 0, and a sequence be as long as the tokens it brings")
+    if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads != 0:
+        raise invalid_shape("shared_prefix_plan: the number of heads must be a multiple of the number of kv heads")
+    group, sequences = num_heads // num_kv_heads, seq_len.shape[0]
+    prefix_of = np.zeros(sequences, dtype=np.int64)
+    seen, shared = 0, []
+    for first, count, prefix in sorted((int(a), int(b), int(c)) for a, b, c in groups):
+        if count < 1 or prefix < 0 or first < seen or first + count > sequences:
+            raise invalid_argument("shared_prefix_plan: groups are runs of sequences of the step, apart from one another, with prefixes of 0 positions or more")
+        seen = first + count
+        members = slice(first, first + count)
+        if ((seq_len[members] - counts[members] < prefix) & (counts[members] > 0)).any():
+            raise invalid_argument("shared_prefix_plan: a group's tokens stand behind its prefix")
+        if prefix > 0 and seq_start[first + count] > seq_start[first]:
+            shared.append((first, count, prefix))
+            prefix_of[members] = prefix
+    wide = prefix_wide(head_dim)
+
+    def tiles(tokens: int):
+        columns = tokens * group
+        return np.arange(0, columns, 16 if columns <= 16 else 16 * wide, dtype=np.int64), (16 if columns <= 16 else 16 * wide)
+
+    # (sequence, first token, tokens, first column, first key, end of the keys, own)
+    rows = []
+    for first, count, prefix in shared:
+        begin, total = int(seq_start[first]), int(seq_start[first + count] - seq_start[first])
+        col0, _ = tiles(total)
+        block = np.zeros((col0.shape[0], 7), dtype=np.int64)
+        block[:, 0], block[:, 1], block[:, 2], block[:, 3], block[:, 5] = first, begin, total, col0, prefix
+        rows.append(block)
+    for seq in np.nonzero(counts > 0)[0]:
+        total = int(counts[seq])
+        col0, width = tiles(total)
+        block = np.zeros((col0.shape[0], 7), dtype=np.int64)
+        block[:, 0], block[:, 1], block[:, 2], block[:, 3], block[:, 4], block[:, 6] = seq, seq_start[seq], total, col0, prefix_of[seq], 1
+        block[:, 5] = seq_len[seq] - total + np.minimum(total - 1, (col0 + width - 1) // group) + 1
+        rows.append(block)
+    tokens = int(seq_start[-1])
+    if not rows:
+        return np.zeros((0, 8), dtype=np.int32), np.zeros(tokens + 1, dtype=np.int32), wide
+    rows = np.concatenate(rows)
+    # parts of equal length, so many that the step makes about two workgroups a compute unit
+    work = int((rows[:, 5] - rows[:, 4]).sum()) * num_kv_heads
+    part = max(1, -(-work // (2 * compute_units * PREFIX_ALIGN))) * PREFIX_ALIGN
+    # a group's prefix in even parts (they are all there is to cut of it); a sequence's own keys every `part` positions
+    lengths = rows[:, 5] - rows[:, 4]
+    cuts = -(-lengths // part)
+    even = np.where(rows[:, 6] == 0, -(-(-(-lengths // cuts)) // 32) * 32, part)
+    cuts = -(-lengths // even)
+    index = np.repeat(np.arange(rows.shape[0]), cuts)
+    place = np.arange(index.shape[0]) - np.repeat(np.cumsum(cuts) - cuts, cuts)
+    items = np.empty((index.shape[0], 8), dtype=np.int32)
+    items[:, :7] = rows[index]
+    items[:, 4] = rows[index, 4] + place * even[index]
+    items[:, 5] = np.minimum(rows[index, 5], items[:, 4] + even[index])
+    # parts of a token: its group's, then its own
+    ahead = np.zeros(sequences, dtype=np.int64)
+    for first, count, prefix in shared:
+        ahead[first:first + count] = cuts[np.nonzero((rows[:, 6] == 0) & (rows[:, 0] == first))[0][0]]
+    items[:, 7] = place + np.where(items[:, 6] == 1, ahead[items[:, 0]], 0)
+    owner = np.repeat(np.arange(sequences), counts)
+    position = seq_len[owner] - counts[owner] + np.arange(tokens) - seq_start[owner]
+    parts = ahead[owner] + -(-(position + 1 - prefix_of[owner]) // part)
+    part_first = np.zeros(tokens + 1, dtype=np.int32)
+    part_first[1:] = np.cumsum(parts)
+    return items, part_first, wide
+
+
+def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device) -> SharedPrefixPlan:
+    """What `attention_shared_prefix` does in a step, for all of its layers.
+
+    seq_start: the step's cumulative token counts [sequences + 1]; seq_len: the sequences' lengths after the step [sequences]
+    (arrays on the host).  groups: (first sequence, sequences, prefix) each, runs of sequences that hold the same keys and values at the
+    positions 0 .. prefix - 1; all their tokens stand behind it.  Sequences in no group share nothing."""
+    dtype_code(dtype)
+    device = torch.device(device)
+    items, part_first, wide = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim,
+                                                  _compute_units(device) if device.type == "cuda" else 256)
+    if int(part_first[-1]) * num_heads >= 1 << 31 or items.shape[0] * num_kv_heads >= 1 << 31:
+        raise invalid_shape("shared_prefix_plan: the step is beyond what one launch takes")
+    longest = max((int(length) for length in seq_len), default=0)
+    return SharedPrefixPlan(torch.from_numpy(items).to(device), torch.from_numpy(part_first).to(device), part_first.shape[0] - 1, int(part_first[-1]),
+                            wide, len(seq_len), longest, (num_heads, num_kv_heads, head_dim, dtype))
+
+
+def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, plan: SharedPrefixPlan,
+                            num_heads: int, num_kv_heads: int, head_dim: int, scale: float, softcap: float | None = None,
+                            sink: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of every token of a step over its sequence's cache, bfloat16 or float32, in which groups of sequences share
+    the keys and values of their first positions: those are read once for all tokens of the group.
+
+    q [tokens, nq * d], cache [pages, 2, nkv, page_size * d] and block_table [sequences, max_blocks] as for `attention_mfma`, which gives
+    the same result (up to rounding) from the same arguments.  plan: from `shared_prefix_plan` for this step and these sizes; a group's shared
+    positions are read through its first sequence's row of the table, all others through their own sequence's.  The pages of whole blocks
+    are usually the same ones in all rows of the group, but need not be.  positions: int32 [tokens], the tokens' positions, as the plan has them.
+    softcap: a scaled score s enters the softmax as softcap * tanh(s / softcap).  sink: float32 [nq], a number per head whose exponential
+    joins the softmax's denominator.  Rows of q that no sequence brings give zeros."""
+    if (num_heads, num_kv_heads, head_dim, q.dtype) != plan.sizes:
+        raise invalid_argument(f"attention_shared_prefix: the plan is for {plan.sizes}, not for {(num_heads, num_kv_heads, head_dim, q.dtype)}")
+    _device_tensor(q, "q", (torch.float32, torch.bfloat16))
+    _device_tensor(cache, "cache", q.dtype)
+    _device_tensor(block_table, "block_table", torch.int32)
+    _device_tensor(positions, "positions", torch.int32)
+    if softcap is not None and not float(softcap) > 0.0:
+        raise invalid_argument("attention_shared_prefix: a cap of the scores must be positive")
+    if sink is not None:
+        _device_tensor(sink, "sink", torch.float32)
+        if sink.shape != (num_heads,):
+            raise invalid_shape("attention_shared_prefix: the sink needs one entry per query head")
+    if not scale > 0:
+        raise invalid_argument(f"attention_shared_prefix: the scale {scale} of the scores is not positive")
+    tokens = q.shape[0]
+    if q.dim() != 2 or q.shape[1] != num_heads * head_dim or tokens != plan.tokens or positions.shape != (tokens,):
+        raise invalid_shape(f"attention_shared_prefix: q {list(q.shape)} and positions {list(positions.shape)} are not [{plan.tokens}, nq * d] and [{plan.tokens}]")
+    page_size = _check_cache(cache, num_kv_heads, head_dim, "attention_shared_prefix")
+    if head_dim % 16 != 0 or not 0 < head_dim <= ATTENTION_MAX_HEAD_DIM or page_size < 16 or page_size & (page_size - 1):
+        raise invalid_argument("attention_shared_prefix takes head sizes in steps of 16 up to 256, pages of a power of two of rows (at least 16)")
+    if block_table.dim() != 2 or block_table.shape[0] < plan.sequences or block_table.shape[1] * page_size < plan.longest:
+        raise invalid_shape(f"attention_shared_prefix: block_table {list(block_table.shape)} does not hold {plan.sequences} sequences of up to {plan.longest} positions")
+    _one_device("attention_shared_prefix", q, cache, block_table, positions, plan.items, plan.part_first, sink)
+    out = torch.empty_like(q)
+    if tokens == 0:
+        return out
+    if plan.items.shape[0] == 0:
+        return out.zero_()
+    part_o = torch.empty((plan.parts * num_heads, head_dim), dtype=torch.float32, device=q.device)
+    part_ml = torch.empty((plan.parts * num_heads, 2), dtype=torch.float32, device=q.device)
+    _check(library().tlie_attention_prefix(_ptr(q), _ptr(cache), dtype_code(q.dtype), _ptr(block_table), block_table.shape[1], _ptr(plan.items),
+                                           plan.items.shape[0], plan.wide, _ptr(positions), _ptr(plan.part_first), _ptr(part_o), _ptr(part_ml),
+                                           _ptr(sink), _ptr(out), tokens, num_heads, num_kv_heads, head_dim, page_size, ctypes.c_float(scale),
+                                           ctypes.c_float(softcap or 0.0), _stream()), "attention_shared_prefix")
     return out
 
 
