@@ -13,12 +13,50 @@
 // of them are exact in any order, so atomics leave the result the same from call to call, class sums and token sums agree to the
 // unit, and a crossing is found in exactly one place.
 //
-// Three launches: the row's maximum from its parts; weights into the parts' histograms; one workgroup a row for the rest.
+// Four launches.  The first three take every row in parts: its maximum; weights into the parts' histograms; the classes in question (each
+// part's workgroup finds them again, which costs less than another launch) and their tokens into the row's list.  The fourth, a workgroup
+// a row, finds the crossings.
 #include "common.h"
 
 namespace tlie {
 
-constexpr int kClasses = 1024, kPickThreads = 1024, kListMost = 2048, kPartThreads = 512;
+constexpr int kClasses = 1024, kPartThreads = 512, kGatherThreads = 256, kPickThreads = 512, kListMost = 2048, kPartsMost = 16;
+
+// 2^(j / 128)
+constexpr int kPowers = 128;
+__constant__ double powers_of_two[kPowers] = {
+    1.0, 1.0054299011128027, 1.0108892860517005, 1.016378314910953,
+    1.0218971486541166, 1.0274459491187637, 1.0330248790212284, 1.0386341019613787,
+    1.0442737824274138, 1.0499440858006872, 1.0556451783605572, 1.061377227289262,
+    1.0671404006768237, 1.0729348675259756, 1.0787607977571199, 1.0846183622133092,
+    1.0905077326652577, 1.0964290818163769, 1.102382583307841, 1.1083684117236787,
+    1.1143867425958924, 1.1204377524096067, 1.1265216186082418, 1.1326385195987192,
+    1.1387886347566916, 1.1449721444318042, 1.1511892299529827, 1.1574400736337511,
+    1.1637248587775775, 1.1700437696832502, 1.1763969916502812, 1.182784710984341,
+    1.189207115002721, 1.1956643920398273, 1.202156731452703, 1.2086843236265816,
+    1.215247359980469, 1.2218460329727576, 1.22848053610687, 1.2351510639369334,
+    1.241857812073484, 1.2486009771892048, 1.255380757024691, 1.2621973503942507,
+    1.2690509571917332, 1.275941778396392, 1.2828700160787783, 1.2898358734066657,
+    1.2968395546510096, 1.3038812651919358, 1.3109612115247644, 1.318079601266064,
+    1.3252366431597413, 1.3324325470831615, 1.339667524053303, 1.3469417862329458,
+    1.3542555469368927, 1.3616090206382248, 1.3690024229745905, 1.3764359707545302,
+    1.383909881963832, 1.3914243757719262, 1.3989796725383112, 1.4065759938190154,
+    1.4142135623730951, 1.4218926021691656, 1.42961333839197, 1.4373759974489824,
+    1.4451808069770467, 1.4530279958490526, 1.460917794180647, 1.4688504333369818,
+    1.4768261459394993, 1.4848451658727524, 1.4929077282912648, 1.5010140696264256,
+    1.5091644275934228, 1.5173590411982147, 1.5255981507445384, 1.533881997840956,
+    1.5422108254079407, 1.550584877685, 1.559004400237837, 1.567469639965553,
+    1.5759808451078865, 1.5845382652524937, 1.593142151342267, 1.6017927556826934,
+    1.6104903319492543, 1.6192351351948637, 1.6280274218573478, 1.6368674497669644,
+    1.645755478153965, 1.6546917676561943, 1.6636765803267364, 1.6727101796415966,
+    1.681792830507429, 1.6909247992693053, 1.7001063537185235, 1.709337763100463,
+    1.718619298122478, 1.7279512309618377, 1.7373338352737062, 1.746767386199169,
+    1.7562521603732995, 1.7657884359332727, 1.7753764925265212, 1.785016611318935,
+    1.7947090750031072, 1.804454167806624, 1.8142521755003989, 1.8241033854070534,
+    1.8340080864093424, 1.843966568958626, 1.8539791250833855, 1.864046048397789,
+    1.8741676341103, 1.8843441790323345, 1.8945759815869656, 1.9048633418176741,
+    1.9152065613971474, 1.925605943636125, 1.9360617934922943, 1.9465744175792332,
+    1.9571441241754002, 1.9677712232331759, 1.978456026387951, 1.9891988469672663};
 
 // larger for what stands earlier: the float's order, then the lower index (-0 and +0 are equal)
 __device__ __forceinline__ uint64_t place_key(float v, int index) {
@@ -35,42 +73,49 @@ __device__ __forceinline__ int place_index(uint64_t key) { return static_cast<in
 // What is the same for all tokens of a row.
 struct RowScale {
   float max, class_scale;
-  double max_wide, inv_t, one;       // one: the weight 1
+  double max_wide, steps, one;       // one: the weight 1
+  const double* powers;              // in LDS: 2^(j / 128) times the weight 1
 };
 
+// Every thread of the workgroup: the powers into LDS (to be read after the next barrier).
+template <int THREADS>
+__device__ __forceinline__ void bring_powers(double* powers, int shift) {
+  const double one = __longlong_as_double((1023ll + shift) << 52);
+  for (int j = threadIdx.x; j < kPowers; j += THREADS) powers[j] = powers_of_two[j] * one;
+}
+
 // The classes share the gaps from 0 to 32 T (what is lighter than e^-32 rounds to no weight), or to the smallest logit if that is nearer.
-__device__ __forceinline__ RowScale row_scale(float max, float min, float temperature, int shift) {
+__device__ __forceinline__ RowScale row_scale(float max, float min, float temperature, int shift, const double* powers) {
   const float span = fminf(32.f * temperature, max - min);
   RowScale row;
   row.max = max, row.class_scale = span > 0.f ? kClasses / span : 0.f;
-  row.max_wide = max, row.inv_t = 1.0 / static_cast<double>(temperature), row.one = __longlong_as_double((1023ll + shift) << 52);
+  row.max_wide = max, row.steps = 184.6649652337873 / static_cast<double>(temperature), row.one = __longlong_as_double((1023ll + shift) << 52);
+  row.powers = powers;
   return row;
 }
 __device__ __forceinline__ int gap_class(const RowScale& row, float v) {
   return static_cast<int>(fminf((row.max - v) * row.class_scale, static_cast<float>(kClasses - 1)));
 }
 
-// exp((v - max) / T) in units of 2^-shift, rounded; one function, each operation written out, for every kernel that forms it.
-// exp(x) = 2^n exp(r), n the whole number nearest to x / ln 2, and exp(r) by its series to r^11 (|r| <= 0.347: 6e-15 of it is left).
+// exp((v - max) / T) in units of 2^-shift; one function, each operation written out, for every kernel that forms it.  The exponent in steps
+// of ln 2 / 128 is a whole number n and a rest f of half a step at most: 2^(n / 128) from the table and its exponent, exp of the rest by its
+// series to the fourth power (1.3e-15 of it is left).  12 operations on 64-bit floats; by the series alone, to the eleventh power
+// of |r| <= 0.347, 23: the weights of 256 rows of 128256 tokens took 57 us that way.
 __device__ __forceinline__ double weight_wide(const RowScale& row, float v) {
 #pragma clang fp contract(off)
-  const double x = fmax((static_cast<double>(v) - row.max_wide) * row.inv_t, -64.0);
-  const double n = rint(x * 1.4426950408889634);
-  double r = fma(n, -0.6931471805599453, x);
-  r = fma(n, -2.3190468138462996e-17, r);
-  double e = 1.0 / 39916800.0;
-  e = fma(e, r, 1.0 / 3628800.0);
-  e = fma(e, r, 1.0 / 362880.0);
-  e = fma(e, r, 1.0 / 40320.0);
-  e = fma(e, r, 1.0 / 5040.0);
-  e = fma(e, r, 1.0 / 720.0);
-  e = fma(e, r, 1.0 / 120.0);
-  e = fma(e, r, 1.0 / 24.0);
-  e = fma(e, r, 1.0 / 6.0);
-  e = fma(e, r, 0.5);
-  e = fma(e, r, 1.0);
-  e = fma(e, r, 1.0);
-  return ldexp(e * row.one, static_cast<int>(n));
+  const double y = fmax((static_cast<double>(v) - row.max_wide) * row.steps, -8192.0);
+  const double shifted = y + 6755399441055744.0;                        // 1.5 * 2^52: the nearest whole number in the low bits
+  const int n = static_cast<int>(__double_as_longlong(shifted));
+  const double f = y - (shifted - 6755399441055744.0);
+  constexpr double step = 0.6931471805599453 / kPowers;
+  double p = step * step * step * step / 24.0;
+  p = fma(p, f, step * step * step / 6.0);
+  p = fma(p, f, step * step / 2.0);
+  p = fma(p, f, step);
+  p = p * f;
+  const double power = row.powers[n & (kPowers - 1)];
+  const double scaled = __hiloint2double(__double2hiint(power) + ((n >> 7) << 20), __double2loint(power));
+  return fma(scaled, p, scaled);
 }
 // a weight below 2^52 to the nearest whole number: adding 2^52 leaves it in the low bits
 __device__ __forceinline__ uint64_t weight_units(double wide) {
@@ -78,30 +123,62 @@ __device__ __forceinline__ uint64_t weight_units(double wide) {
   return static_cast<uint64_t>(__double_as_longlong(wide + 4503599627370496.0)) & 0xfffffffffffffull;
 }
 
-// ceil(share * total) and floor(share * total), exact, for a float share in [0, 1] and total < 2^63.
+// ceil(share * total) or floor(share * total), exact, for a float share in [0, 1) and total < 2^63.
 __device__ __forceinline__ uint64_t share_of(float share, uint64_t total, bool up) {
-  const uint32_t bits = __float_as_uint(share), exponent = (bits >> 23) & 255;
-  const uint64_t mantissa = exponent ? (bits & 0x7fffffu) | 0x800000u : bits & 0x7fffffu;
-  const int down = 150 - static_cast<int>(exponent ? exponent : 1);          // share = mantissa * 2^-down, down >= 23
-  const unsigned __int128 product = static_cast<unsigned __int128>(mantissa) * total;
-  if (down >= 128) return up && product != 0 ? 1 : 0;
-  const unsigned __int128 whole = product >> down;
-  return static_cast<uint64_t>(whole) + (up && (whole << down) != product ? 1 : 0);
+  const uint32_t bits = __float_as_uint(share), exponent = bits >> 23;
+  const uint64_t mantissa = exponent ? (bits & 0x7fffffu) | 0x800000u : bits;
+  const int down = 150 - static_cast<int>(exponent ? exponent : 1);          // share = mantissa * 2^-down, down >= 24
+  const uint64_t low = mantissa * total, high = __umul64hi(mantissa, total);
+  uint64_t whole, rest;
+  if (down < 64) whole = (high << (64 - down)) | (low >> down), rest = low << (64 - down);
+  else if (down < 128) whole = high >> (down - 64), rest = low | (down > 64 ? high << (128 - down) : 0);
+  else whole = 0, rest = low | high;
+  return whole + (up && rest != 0 ? 1 : 0);
 }
 
-// f(index, value) over the part's tokens
-template <int THREADS, typename F>
+// f(index, values) over the tokens begin .. end - 1 in groups of four that start at multiples of 16 bytes, the THREADS threads side
+// by side; what lies outside the range is -inf, a token that nothing counts.  TOGETHER groups a thread are worked on while as many
+// more are on their way: a row of 128256 tokens reaches a workgroup from beyond its L2, some 1 us for each batch that it waits for.
+template <int THREADS, int TOGETHER, typename F>
 __device__ __forceinline__ void scan_tokens(const float* __restrict__ row, int begin, int end, F f) {
-  constexpr int kTogether = 8;
-  int i = begin + threadIdx.x;
-  for (; i + (kTogether - 1) * THREADS < end; i += kTogether * THREADS) {
-    float v[kTogether];
-#pragma unroll
-    for (int u = 0; u < kTogether; ++u) v[u] = row[i + u * THREADS];
-#pragma unroll
-    for (int u = 0; u < kTogether; ++u) f(i + u * THREADS, v[u]);
+  const int ahead = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 2) & 3;      // tokens by which the row starts past such a place
+  const int whole = (begin + ahead + 3) >> 2, past = (end + ahead) >> 2;              // the groups that lie inside
+  if (begin >= end) return;
+  // a group that the range's ends cut: at most one at each, by a thread each (which lie in one wave)
+  if (threadIdx.x < 2) {
+    const int g = threadIdx.x == 0 ? whole - 1 : past, first = 4 * g - ahead;
+    const bool cut = threadIdx.x == 0 ? first + 4 > begin && first < begin : first < end && (first >= begin || whole > past);
+    if (cut && !(threadIdx.x == 1 && first < begin)) {
+      float4 v;
+      v.x = first >= begin && first < end ? row[first] : -INFINITY;
+      v.y = first + 1 >= begin && first + 1 < end ? row[first + 1] : -INFINITY;
+      v.z = first + 2 >= begin && first + 2 < end ? row[first + 2] : -INFINITY;
+      v.w = first + 3 >= begin && first + 3 < end ? row[first + 3] : -INFINITY;
+      f(first, v);
+    }
   }
-  for (; i < end; i += THREADS) f(i, row[i]);
+  if (whole >= past) return;
+  const float4* groups = reinterpret_cast<const float4*>(row - ahead);
+  // (every load is made, past the end the last group's again: under a condition each would be waited for by itself)
+  auto bring = [&](int g, float4 (&v)[TOGETHER]) {
+#pragma unroll
+    for (int u = 0; u < TOGETHER; ++u) v[u] = groups[min(g + u * THREADS, past - 1)];
+  };
+  float4 now[TOGETHER], next[TOGETHER];
+  int g = whole + threadIdx.x;
+  bring(g, now);
+  for (; g < past; g += TOGETHER * THREADS) {
+    bring(g + TOGETHER * THREADS, next);
+#pragma unroll
+    for (int u = 0; u < TOGETHER; ++u) {
+      if (g + u * THREADS < past) f(4 * (g + u * THREADS) - ahead, now[u]);
+      now[u] = next[u];
+    }
+  }
+}
+template <typename F>
+__device__ __forceinline__ void each_of(int index, const float4& v, F f) {
+  f(index, v.x), f(index + 1, v.y), f(index + 2, v.z), f(index + 3, v.w);
 }
 
 struct PartStat {
@@ -110,23 +187,24 @@ struct PartStat {
   uint32_t unused;
 };
 constexpr uint64_t kBadPart = ~0ull;
+constexpr uint32_t kNotListed = ~0u;
 
 __global__ void __launch_bounds__(kPartThreads)
 draw_best_kernel(const float* __restrict__ logits, int vocab, int part_len, int parts, PartStat* __restrict__ stats) {
   __shared__ uint64_t best_of[kPartThreads / kWave];
   __shared__ float min_of[kPartThreads / kWave];
   const int row = blockIdx.y, part = blockIdx.x, begin = part * part_len, end = min(vocab, begin + part_len);
-  uint64_t best = 0;
-  float least = INFINITY;
+  float most = -INFINITY, least = INFINITY;
+  int at = 0;
   bool bad = false;
-  scan_tokens<kPartThreads>(logits + static_cast<size_t>(row) * vocab, begin, end, [&](int i, float v) {
-    bad = bad || !(v < INFINITY);
-    if (v > -INFINITY) {
-      const uint64_t key = place_key(v, i);
-      best = key > best ? key : best;
-      least = fminf(least, v);
-    }
+  scan_tokens<kPartThreads, 4>(logits + static_cast<size_t>(row) * vocab, begin, end, [&](int first, const float4& four) {
+    each_of(first, four, [&](int i, float v) {
+      bad = bad || !(v < INFINITY);
+      if (v > most) most = v, at = i;                             // (a thread meets its tokens in the order of their index)
+      least = v > -INFINITY ? fminf(least, v) : least;
+    });
   });
+  uint64_t best = most > -INFINITY ? place_key(most, at) : 0;
   if (bad) best = kBadPart;
   for (int offset = 32; offset > 0; offset >>= 1) {
     const uint64_t other = __shfl_xor(best, offset, 64);
@@ -136,6 +214,7 @@ draw_best_kernel(const float* __restrict__ logits, int vocab, int part_len, int 
   if ((threadIdx.x & 63) == 0) best_of[threadIdx.x >> 6] = best, min_of[threadIdx.x >> 6] = least;
   __syncthreads();
   if (threadIdx.x == 0) {
+#pragma unroll
     for (int w = 1; w < kPartThreads / kWave; ++w) {
       best = best_of[w] > best ? best_of[w] : best;
       least = fminf(least, min_of[w]);
@@ -144,19 +223,17 @@ draw_best_kernel(const float* __restrict__ logits, int vocab, int part_len, int 
   }
 }
 
+// (all parts are asked for together: one after the other each waits for the one before)
 __device__ __forceinline__ void join_stats(const PartStat* __restrict__ stats, int parts, uint64_t& best, float& least) {
+  PartStat part[kPartsMost];
+#pragma unroll
+  for (int p = 0; p < kPartsMost; ++p) part[p] = stats[min(p, parts - 1)];
   best = 0, least = INFINITY;
-  for (int p = 0; p < parts; ++p) {
-    best = stats[p].best > best ? stats[p].best : best;
-    least = fminf(least, stats[p].min);
+#pragma unroll
+  for (int p = 0; p < kPartsMost; ++p) {
+    best = part[p].best > best ? part[p].best : best;
+    least = fminf(least, part[p].min);
   }
-}
-
-// exp(v - max) for the log-probability: the rounding of (v - max) log2(e) is made good, the exponential's own is left
-__device__ __forceinline__ float plain_weight(float max, float v) {
-  const float x = v - max, high = x * 1.44269502f, low = fmaf(x, 1.44269502f, -high) + x * 1.92596303e-8f;
-  const float e = __builtin_amdgcn_exp2f(high);
-  return x < -100.f ? 0.f : fmaf(e, low * 0.693147182f, e);
 }
 
 __global__ void __launch_bounds__(kPartThreads)
@@ -166,6 +243,7 @@ draw_weigh_kernel(const float* __restrict__ logits, int vocab, int part_len, int
   __shared__ unsigned long long mass[kClasses];
   __shared__ uint32_t count[kClasses];
   __shared__ double sum_of[kPartThreads / kWave];
+  __shared__ double powers[kPowers];
   const int row = blockIdx.y, part = blockIdx.x, begin = part * part_len, end = min(vocab, begin + part_len);
   uint64_t best;
   float least;
@@ -174,22 +252,24 @@ draw_weigh_kernel(const float* __restrict__ logits, int vocab, int part_len, int
   const float t = temperature ? temperature[row] : 0.f;
   const bool drawn = t > 0.f;
   if (!drawn && !want_sum) return;
-  const RowScale scale = row_scale(place_value(best), least, t, shift);
-  if (drawn) {
-    for (int c = threadIdx.x; c < kClasses; c += kPartThreads) mass[c] = 0, count[c] = 0;
-    __syncthreads();
-  }
+  bring_powers<kPartThreads>(powers, shift);
+  for (int c = threadIdx.x; c < kClasses; c += kPartThreads) mass[c] = 0, count[c] = 0;
+  __syncthreads();
+  const RowScale scale = row_scale(place_value(best), least, t, shift, powers);
   double sum = 0.0;
-  scan_tokens<kPartThreads>(logits + static_cast<size_t>(row) * vocab, begin, end, [&](int, float v) {
-    if (drawn) {
-      const uint64_t units = weight_units(weight_wide(scale, v));
-      if (units != 0) {
-        const int c = gap_class(scale, v);
-        atomicAdd(&mass[c], static_cast<unsigned long long>(units));
-        atomicAdd(&count[c], 1u);
-      }
-    }
-    if (want_sum) sum += static_cast<double>(plain_weight(scale.max, v));
+  scan_tokens<kPartThreads, 4>(logits + static_cast<size_t>(row) * vocab, begin, end, [&](int first, const float4& four) {
+    if (drawn)
+      each_of(first, four, [&](int, float v) {
+        const uint64_t units = weight_units(weight_wide(scale, v));
+        if (units != 0) {
+          const int c = gap_class(scale, v);
+          atomicAdd(&mass[c], static_cast<unsigned long long>(units));
+          atomicAdd(&count[c], 1u);
+        }
+      });
+    // exp(v - max), for the log-probability: an exponential's rounding of 2^-23 each, a sum of four in 32 bits, the rest in 64
+    auto plain = [&](float v) { return __builtin_amdgcn_exp2f((v - scale.max) * 1.44269502f); };
+    if (want_sum) sum += static_cast<double>((plain(four.x) + plain(four.y)) + (plain(four.z) + plain(four.w)));
   });
   const size_t place = static_cast<size_t>(row) * parts + part;
   if (drawn) {
@@ -201,52 +281,245 @@ draw_weigh_kernel(const float* __restrict__ logits, int vocab, int part_len, int
     if ((threadIdx.x & 63) == 0) sum_of[threadIdx.x >> 6] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
+#pragma unroll
       for (int w = 1; w < kPartThreads / kWave; ++w) sum += sum_of[w];
       sums[place] = sum;
     }
   }
 }
 
-// running sums over the workgroup's threads, each thread's own included
-__device__ __forceinline__ uint64_t running_sum(uint64_t v, uint64_t* waves) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int offset = 1; offset < 64; offset <<= 1) {
-    const uint64_t below = __shfl_up(v, offset, 64);
-    if (lane >= offset) v += below;
-  }
-  if (lane == 63) waves[wave] = v;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) v += waves[w];
-  __syncthreads();
-  return v;
-}
-
-struct PickShared {
-  uint64_t running_mass[kClasses];          // up to and with each class
-  uint32_t running_count[kClasses];
-  uint64_t list[kListMost];
-  uint64_t waves[kPickThreads / kWave];
-  uint64_t adjust[kClasses];
-  uint32_t adjust_count[kClasses];
-  uint64_t digit_mass[256];
-  uint32_t digit_count[256];
-  uint32_t wanted[kClasses / 32];           // the classes to bring together
-  uint64_t result, result2;
-  int found, size;
+// One token of a class in question: its place in the order, its weight, and of its class the mass and the number of tokens
+// before it and its tokens' range in the list.
+struct Listed {
+  uint64_t key, units, mass_before;
+  uint32_t count_before, begin, end, unused;
+};
+// What the list leaves open of a row: masses that the crossings lie between, and the list's length.
+struct RowState {
+  uint64_t total_lo, total_hi, kept_floor;
+  uint32_t size, cut_k;
 };
 
-// The first class at which the running mass reaches `target` (> 0), or kClasses.
-__device__ int class_reaching(PickShared& s, uint64_t target) {
-  const int c = threadIdx.x;
-  if (c == 0) s.found = kClasses;
-  __syncthreads();
-  const uint64_t before = c > 0 ? s.running_mass[c - 1] : 0;
-  if (s.running_mass[c] >= target && before < target) s.found = c;
-  __syncthreads();
-  const int found = s.found;
-  __syncthreads();
-  return found;
+// Running sums over a wave's lanes, each lane's own included: within the sixteens by shifts, then the sixteens' ends by broadcasts.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ void running_step(uint64_t& mass, uint32_t& count) {
+  const uint32_t low = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(mass), CONTROL, ROWS, 0xf, false);
+  const uint32_t high = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(mass >> 32), CONTROL, ROWS, 0xf, false);
+  mass += (static_cast<uint64_t>(high) << 32) | low;
+  count += __builtin_amdgcn_update_dpp(0, count, CONTROL, ROWS, 0xf, false);
 }
+// Running sums over the workgroup's threads; wave_mass and wave_count: an entry of LDS a wave.
+template <int THREADS>
+__device__ __forceinline__ void running_sums(uint64_t* wave_mass, uint32_t* wave_count, uint64_t& mass, uint32_t& count) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  running_step<0x111, 0xf>(mass, count);                        // row_shr:1, 2, 4, 8
+  running_step<0x112, 0xf>(mass, count);
+  running_step<0x114, 0xf>(mass, count);
+  running_step<0x118, 0xf>(mass, count);
+  running_step<0x142, 0xa>(mass, count);                        // row_bcast:15 into the odd sixteens, row_bcast:31 into the upper half
+  running_step<0x143, 0xc>(mass, count);
+  if (lane == 63) wave_mass[wave] = mass, wave_count[wave] = count;
+  __syncthreads();
+  uint64_t m = 0;
+  uint32_t n = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / kWave; ++w) {
+    const bool before = w < wave;
+    m += before ? wave_mass[w] : 0, n += before ? wave_count[w] : 0;
+  }
+  mass += m, count += n;
+}
+
+struct GatherShared {
+  uint64_t running_mass[kClasses];          // up to and with each class
+  uint32_t running_count[kClasses];
+  uint32_t begin[kClasses];                 // a wanted class's first place in the list, or kNotListed
+  uint32_t place[kClasses];                 // where this part's next token of the class goes
+  uint64_t wave_mass[kGatherThreads / kWave];
+  uint32_t wave_count[kGatherThreads / kWave], listed_count[kGatherThreads / kWave];
+  double powers[kPowers];
+  int found[7];                             // classes, a place for each question
+};
+
+// The answers' bounds are the same in both kernels.
+__device__ __forceinline__ uint64_t goal_of(float u, uint64_t kept) { return (u < 1.f ? share_of(u, kept, false) : kept - 1) + 1; }
+__device__ __forceinline__ uint64_t target_of(float p, uint64_t total) { return max(share_of(fmaxf(p, 0.f), total, true), static_cast<uint64_t>(1)); }
+
+__global__ void __launch_bounds__(kGatherThreads)
+draw_gather_kernel(const float* __restrict__ logits, int vocab, int part_len, int parts, const PartStat* __restrict__ stats,
+                   const float* __restrict__ uniform, const float* __restrict__ temperature, const int* __restrict__ top_k,
+                   const float* __restrict__ top_p, const float* __restrict__ min_p, int shift, const uint64_t* __restrict__ class_mass,
+                   const uint32_t* __restrict__ class_count, RowState* __restrict__ states, Listed* __restrict__ lists) {
+  __shared__ GatherShared s;
+  const int r = blockIdx.y, part = blockIdx.x, tid = threadIdx.x;
+  const float t = temperature ? temperature[r] : 0.f, p_share = top_p ? top_p[r] : 1.f, floor_p = min_p ? min_p[r] : 0.f;
+  const float u = fmaxf(uniform[r], 0.f);                                                 // (a NaN counts as 0)
+  const int k = top_k ? top_k[r] : 0;
+  if (!(t > 0.f)) return;
+  uint64_t best;
+  float least;
+  join_stats(stats + static_cast<size_t>(r) * parts, parts, best, least);
+  if (best == kBadPart || best == 0) return;
+  bring_powers<kGatherThreads>(s.powers, shift);
+  const RowScale scale = row_scale(place_value(best), least, t, shift, s.powers);
+  const uint64_t one = 1ull << shift;
+  // ---- the row's classes, four neighbours a thread; eight parts are asked for together.  (Four waves: with a class a thread, sixteen
+  // waves do what is the same for all of the row, and 64 rows in 8 parts took 20 us) ----
+  constexpr int kOwn = kClasses / kGatherThreads, kParts = 8;
+  static_assert(kOwn == 4, "classes are loaded as 16-byte pieces");
+  uint64_t mass[kOwn] = {};
+  uint32_t count[kOwn] = {}, ahead[kOwn] = {};                    // (ahead: of the parts before this one)
+  for (int p0 = 0; p0 < parts; p0 += kParts) {
+    ulonglong2 m[kParts][2];
+    uint4 n[kParts];
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      const size_t place = (static_cast<size_t>(r) * parts + min(p0 + p, parts - 1)) * kClasses + kOwn * tid;
+      m[p][0] = *reinterpret_cast<const ulonglong2*>(class_mass + place), m[p][1] = *reinterpret_cast<const ulonglong2*>(class_mass + place + 2);
+      n[p] = *reinterpret_cast<const uint4*>(class_count + place);
+    }
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      if (p0 + p >= parts) break;
+      mass[0] += m[p][0].x, mass[1] += m[p][0].y, mass[2] += m[p][1].x, mass[3] += m[p][1].y;
+      if (p0 + p < part) ahead[0] += n[p].x, ahead[1] += n[p].y, ahead[2] += n[p].z, ahead[3] += n[p].w;
+      count[0] += n[p].x, count[1] += n[p].y, count[2] += n[p].z, count[3] += n[p].w;
+    }
+  }
+  uint64_t running[kOwn];
+  uint32_t running_n[kOwn];
+  {
+    uint64_t all = (mass[0] + mass[1]) + (mass[2] + mass[3]);
+    uint32_t all_n = (count[0] + count[1]) + (count[2] + count[3]);
+    const uint64_t own = all;
+    const uint32_t own_n = all_n;
+    if (tid < 7) s.found[tid] = kClasses;
+    running_sums<kGatherThreads>(s.wave_mass, s.wave_count, all, all_n);
+    all -= own, all_n -= own_n;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+      running[j] = all += mass[j], running_n[j] = all_n += count[j];
+      s.running_mass[kOwn * tid + j] = running[j], s.running_count[kOwn * tid + j] = running_n[j];
+    }
+  }
+  __syncthreads();
+  auto mass_upto = [&](int c) -> uint64_t { return c < 0 ? 0 : s.running_mass[min(c, kClasses - 1)]; };
+  auto reaches = [&](int question, uint64_t target) {              // the class (if any) at which the running mass reaches a target > 0
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j)
+      if (running[j] >= target && running[j] - mass[j] < target) s.found[question] = kOwn * tid + j;
+  };
+  bool wanted[kOwn] = {};
+  auto want = [&](int lo, int hi) {
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) wanted[j] = wanted[j] || (kOwn * tid + j >= lo && kOwn * tid + j <= hi);
+  };
+
+  // ---- which classes the crossings can lie in.  A class that is cut leaves what follows with a range of masses ----
+  uint64_t total_lo = s.running_mass[kClasses - 1], total_hi = total_lo;
+  bool cut_k = false;
+  if (k > 0 && static_cast<uint32_t>(k) < s.running_count[kClasses - 1]) {
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j)
+      if (running_n[j] >= static_cast<uint32_t>(k) && running_n[j] - count[j] < static_cast<uint32_t>(k)) s.found[0] = kOwn * tid + j;
+    __syncthreads();
+    const int c = s.found[0];
+    total_hi = mass_upto(c), total_lo = s.running_count[c] == static_cast<uint32_t>(k) ? total_hi : mass_upto(c - 1);
+    cut_k = total_lo != total_hi;
+    if (cut_k) want(c, c);
+  }
+  uint64_t kept_lo = total_lo, kept_hi = total_hi, kept_floor = one;
+  if (p_share < 1.f) {
+    const uint64_t low = target_of(p_share, total_lo);
+    reaches(1, low);
+    reaches(2, cut_k ? target_of(p_share, total_hi) : low);
+    __syncthreads();
+    const int c_lo = s.found[1], c_hi = s.found[2];
+    want(c_lo, c_hi);
+    kept_lo = mass_upto(c_lo - 1), kept_hi = min(kept_hi, mass_upto(c_hi));
+  }
+  if (floor_p > 0.f) {
+    // the class of the gap at which the weight is min_p, and its neighbours, for the rounding of the gap
+    const float gap = fmaxf(-logf(fminf(floor_p, 1.f)) * t, 0.f);
+    const int c = static_cast<int>(fminf(gap * scale.class_scale, static_cast<float>(kClasses - 1)));
+    want(c - 1, c + 1);
+    kept_floor = max(one, mass_upto(c - 2));
+    kept_lo = min(kept_lo, kept_floor), kept_hi = min(kept_hi, mass_upto(c + 1));
+  }
+  kept_lo = max(kept_lo, one), kept_hi = max(kept_hi, one);       // (the first token is always kept)
+  const uint64_t goal = goal_of(u, kept_lo);
+  reaches(3, goal);
+  reaches(4, kept_lo != kept_hi ? goal_of(u, kept_hi) : goal);
+  __syncthreads();
+  want(s.found[3], s.found[4]);
+
+  // ---- their tokens: class after class in the list, and of a class part after part ----
+  uint64_t nothing = 0;
+  uint32_t listed = 0, own_listed;
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) {
+    wanted[j] = wanted[j] && mass[j] != 0;
+    if (wanted[j]) {
+      listed += count[j];
+      atomicMin(&s.found[5], kOwn * tid + j), atomicMin(&s.found[6], kClasses - 1 - (kOwn * tid + j));
+    }
+  }
+  own_listed = listed;
+  running_sums<kGatherThreads>(s.wave_mass, s.listed_count, nothing, listed);
+  listed -= own_listed;
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) {
+    s.begin[kOwn * tid + j] = wanted[j] ? listed : kNotListed;
+    s.place[kOwn * tid + j] = listed + ahead[j];
+    listed += wanted[j] ? count[j] : 0;
+  }
+  uint32_t size = 0;
+#pragma unroll
+  for (int w = 0; w < kGatherThreads / kWave; ++w) size += s.listed_count[w];
+  if (part == 0 && tid == 0) states[r] = RowState{total_lo, total_hi, kept_floor, size, cut_k ? 1u : 0u};
+  if (size > kListMost) return;
+  __syncthreads();
+  // The classes in question are bounded by values, so that the others' tokens cost a comparison (differences of logits are
+  // rounded to 2^-24 of the larger, and the class's bound again: room on either side).
+  const int c_first = s.found[5], c_last = kClasses - 1 - s.found[6];
+  float lower = -3.4028235e38f, upper = INFINITY;
+  if (scale.class_scale > 0.f) {                                  // (else every token is of the first class)
+    const float room = fmaxf(fabsf(scale.max), fabsf(least)) * 2.4e-7f;
+    upper = scale.max - static_cast<float>(c_first) * 0.99999f / scale.class_scale + room;
+    if (c_last < kClasses - 1) lower = scale.max - static_cast<float>(c_last + 1) * 1.00001f / scale.class_scale - room;
+  }
+  const int begin = part * part_len, end = min(vocab, begin + part_len);
+  Listed* list = lists + static_cast<size_t>(r) * kListMost;
+  scan_tokens<kGatherThreads, 8>(logits + static_cast<size_t>(r) * vocab, begin, end, [&](int first, const float4& four) {
+    if (!(fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w)) >= lower && fminf(fminf(four.x, four.y), fminf(four.z, four.w)) <= upper)) return;
+    each_of(first, four, [&](int i, float v) {
+      if (!(v >= lower && v <= upper)) return;
+      const int c = gap_class(scale, v);
+      if (s.begin[c] == kNotListed) return;
+      const uint64_t units = weight_units(weight_wide(scale, v));
+      if (units == 0) return;
+      const uint32_t before = c > 0 ? s.running_count[c - 1] : 0, from = s.begin[c];
+      list[atomicAdd(&s.place[c], 1u)] = Listed{place_key(v, i), units, c > 0 ? s.running_mass[c - 1] : 0, before, from, from + s.running_count[c] - before, 0};
+    });
+  });
+}
+
+struct Entry {
+  uint64_t key, units;
+};
+
+struct PickShared {
+  Entry list[kListMost];                    // bucket by bucket
+  uint64_t bucket_mass[kListMost];          // of a bucket, then up to it
+  uint32_t bucket_count[kListMost], place[kListMost];
+  uint64_t wave_mass[kPickThreads / kWave];
+  uint32_t wave_count[kPickThreads / kWave];
+  double powers[kPowers];
+  uint64_t digit_mass[256];
+  uint32_t digit_count[256];
+  uint64_t answers[4], answer_key;          // of the crossings
+  int found;
+};
 
 // Without a list (more tokens than it holds share the classes in question): the place in the order where the running mass
 // (or count) reaches target, found digit by digit of the place keys, eight passes over the row.  Returns the running mass there.
@@ -255,15 +528,17 @@ __device__ uint64_t descend(PickShared& s, const float* __restrict__ row, int vo
   for (int digit = 7; digit >= 0; --digit) {
     for (int b = threadIdx.x; b < 256; b += kPickThreads) s.digit_mass[b] = 0, s.digit_count[b] = 0;
     __syncthreads();
-    scan_tokens<kPickThreads>(row, 0, vocab, [&](int i, float v) {
-      if (!(v > -INFINITY)) return;
-      const uint64_t place = place_key(v, i);
-      if (digit < 7 && (place >> (8 * digit + 8)) != (prefix >> (8 * digit + 8))) return;
-      const uint64_t units = weight_units(weight_wide(scale, v));
-      if (units == 0) return;
-      const int b = static_cast<int>((place >> (8 * digit)) & 255);
-      atomicAdd(reinterpret_cast<unsigned long long*>(&s.digit_mass[b]), static_cast<unsigned long long>(units));
-      atomicAdd(&s.digit_count[b], 1u);
+    scan_tokens<kPickThreads, 4>(row, 0, vocab, [&](int first, const float4& four) {
+      each_of(first, four, [&](int i, float v) {
+        if (!(v > -INFINITY)) return;
+        const uint64_t place = place_key(v, i);
+        if (digit < 7 && (place >> (8 * digit + 8)) != (prefix >> (8 * digit + 8))) return;
+        const uint64_t units = weight_units(weight_wide(scale, v));
+        if (units == 0) return;
+        const int b = static_cast<int>((place >> (8 * digit)) & 255);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.digit_mass[b]), static_cast<unsigned long long>(units));
+        atomicAdd(&s.digit_count[b], 1u);
+      });
     });
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -273,11 +548,11 @@ __device__ uint64_t descend(PickShared& s, const float* __restrict__ row, int vo
         if ((by_count ? n + s.digit_count[b] : m + s.digit_mass[b]) >= target) break;
         m += s.digit_mass[b], n += s.digit_count[b];
       }
-      s.found = b, s.result = m, s.result2 = n, s.waves[0] = m + s.digit_mass[b];
+      s.found = b, s.wave_mass[0] = m, s.wave_mass[1] = n, s.wave_mass[2] = m + s.digit_mass[b];
     }
     __syncthreads();
     prefix |= static_cast<uint64_t>(s.found) << (8 * digit);
-    mass_before = s.result, count_before = s.result2, mass = s.waves[0];
+    mass_before = s.wave_mass[0], count_before = s.wave_mass[1], mass = s.wave_mass[2];
     __syncthreads();
   }
   *key = prefix;
@@ -287,11 +562,17 @@ __device__ uint64_t descend(PickShared& s, const float* __restrict__ row, int vo
 __global__ void __launch_bounds__(kPickThreads)
 draw_pick_kernel(const float* __restrict__ logits, int vocab, int parts, const PartStat* __restrict__ stats, const float* __restrict__ uniform,
                  const float* __restrict__ temperature, const int* __restrict__ top_k, const float* __restrict__ top_p,
-                 const float* __restrict__ min_p, int shift, const uint64_t* __restrict__ class_mass, const uint32_t* __restrict__ class_count,
+                 const float* __restrict__ min_p, int shift, const RowState* __restrict__ states, const Listed* __restrict__ lists,
                  const double* __restrict__ sums, int* __restrict__ out, float* __restrict__ logprob) {
   __shared__ PickShared s;
+  constexpr int kEach = kListMost / kPickThreads;
   const int r = blockIdx.x, tid = threadIdx.x;
   const float* row = logits + static_cast<size_t>(r) * vocab;
+  const float t = temperature ? temperature[r] : 0.f, p_share = top_p ? top_p[r] : 1.f, floor_p = min_p ? min_p[r] : 0.f;
+  const float u = fmaxf(uniform[r], 0.f);
+  const int k = top_k ? top_k[r] : 0;
+  const Listed* list = lists + static_cast<size_t>(r) * kListMost;
+  const RowState state = states[r];                               // (of a row that is not drawn: anything, not looked at)
   uint64_t best;
   float least;
   join_stats(stats + static_cast<size_t>(r) * parts, parts, best, least);
@@ -302,189 +583,143 @@ draw_pick_kernel(const float* __restrict__ logits, int vocab, int parts, const P
     }
     return;
   }
-  const float t = temperature ? temperature[r] : 0.f;
+  double log_sum = 0.0;
+  if (tid == 0 && logprob) {
+    double sum = 0.0;
+    for (int p = 0; p < parts; ++p) sum += sums[static_cast<size_t>(r) * parts + p];
+    log_sum = log(sum);
+  }
   uint64_t chosen = best;
   if (t > 0.f) {
-    const RowScale scale = row_scale(place_value(best), least, t, shift);
+    const int size = static_cast<int>(min(state.size, static_cast<uint32_t>(kListMost) + 1));
     const uint64_t one = 1ull << shift;
-    // ---- the row's classes, and running sums over them ----
-    uint64_t mass = 0;
-    uint32_t count = 0;
-    for (int p = 0; p < parts; ++p) {
-      const size_t place = (static_cast<size_t>(r) * parts + p) * kClasses + tid;
-      mass += class_mass[place], count += class_count[place];
-    }
-    const uint64_t running = running_sum(mass, s.waves);
-    const uint64_t running_n = running_sum(count, s.waves);
-    s.running_mass[tid] = running, s.running_count[tid] = static_cast<uint32_t>(running_n);
-    if (tid < kClasses / 32) s.wanted[tid] = 0;
-    if (tid == 0) s.size = 0, s.result = 0;
-    __syncthreads();
-    auto mass_upto = [&](int c) { return c < 0 ? 0ull : static_cast<unsigned long long>(s.running_mass[min(c, kClasses - 1)]); };
-    auto want = [&](int lo, int hi) {                              // (every thread: its own class)
-      if (tid >= lo && tid <= hi && mass != 0) atomicOr(&s.wanted[tid >> 5], 1u << (tid & 31));
-    };
-
-    // ---- which classes the crossings can lie in.  A class that is cut leaves what follows with a range of masses. ----
-    const int k = top_k ? top_k[r] : 0;
-    uint64_t total_lo = s.running_mass[kClasses - 1], total_hi = total_lo;
-    bool cut_k = false;
-    if (k > 0 && static_cast<uint32_t>(k) < s.running_count[kClasses - 1]) {
-      if (tid == 0) s.found = 0;
-      __syncthreads();
-      if (running_n >= static_cast<uint64_t>(k) && running_n - count < static_cast<uint64_t>(k)) s.found = tid;
-      __syncthreads();
-      const int c = s.found;
-      __syncthreads();
-      total_hi = mass_upto(c), total_lo = s.running_count[c] == static_cast<uint32_t>(k) ? total_hi : mass_upto(c - 1);
-      cut_k = total_lo != total_hi;
-      if (cut_k) want(c, c);
-    }
-    const float p_share = top_p ? top_p[r] : 1.f;
-    const bool cut_p = p_share < 1.f;
-    uint64_t kept_lo = total_lo, kept_hi = total_hi;
-    if (cut_p) {
-      const float share = fmaxf(p_share, 0.f);
-      const uint64_t low = share_of(share, total_lo, true), high = share_of(share, total_hi, true);
-      const int c_lo = class_reaching(s, low > 0 ? low : 1), c_hi = class_reaching(s, high > 0 ? high : 1);
-      want(c_lo, c_hi);
-      kept_lo = mass_upto(c_lo - 1), kept_hi = min(kept_hi, static_cast<uint64_t>(mass_upto(c_hi)));
-    }
-    const float floor_p = min_p ? min_p[r] : 0.f;
-    const bool cut_m = floor_p > 0.f;
-    uint64_t kept_floor = one;
+    const bool cut_k = state.cut_k != 0, cut_p = p_share < 1.f, cut_m = floor_p > 0.f;
+    bring_powers<kPickThreads>(s.powers, shift);
+    if (tid == 0) s.answers[0] = state.total_hi, s.answers[1] = state.total_hi, s.answers[2] = state.kept_floor, s.answer_key = best;
+    const RowScale scale = row_scale(place_value(best), least, t, shift, s.powers);
     const double least_weight = static_cast<double>(fminf(floor_p, 1.f)) * scale.one;
-    if (cut_m) {
-      // the class of the gap at which the weight is min_p, and its neighbours, for the rounding of the gap
-      const float gap = fmaxf(-logf(fminf(floor_p, 1.f)) * t, 0.f);
-      const int c = static_cast<int>(fminf(gap * scale.class_scale, static_cast<float>(kClasses - 1)));
-      want(c - 1, c + 1);
-      kept_floor = max(one, static_cast<uint64_t>(mass_upto(c - 2)));
-      kept_lo = min(kept_lo, kept_floor), kept_hi = min(kept_hi, static_cast<uint64_t>(mass_upto(c + 1)));
-    }
-    // (the first token is always kept)
-    kept_lo = max(kept_lo, one);
-    const float u = fmaxf(uniform[r], 0.f);                       // (a NaN counts as 0)
-    auto goal_of = [&](uint64_t kept) { return u < 1.f ? share_of(u, kept, false) : kept - 1; };
-    {
-      const int c_lo = class_reaching(s, goal_of(kept_lo) + 1), c_hi = class_reaching(s, goal_of(kept_hi) + 1);
-      want(c_lo, c_hi);
-    }
-    __syncthreads();
-
-    // ---- their tokens, sorted.  The list holds every token of a wanted class, so a token's running mass over the whole row is
-    // the list's own plus what the classes in between, which are not in it, hold. ----
-    {
-      const bool mine = (s.wanted[tid >> 5] >> (tid & 31) & 1u) != 0;
-      const uint64_t listed = running_sum(mine ? mass : 0, s.waves);
-      s.adjust[tid] = running - listed;                           // (of a wanted class: what is missing up to its end, and so at its start)
-      if (cut_k) {
-        const uint64_t listed_n = running_sum(mine ? count : 0, s.waves);
-        s.adjust_count[tid] = static_cast<uint32_t>(running_n - listed_n);
-      }
-    }
-    scan_tokens<kPickThreads>(row, 0, vocab, [&](int i, float v) {
-      if (!(v > -INFINITY)) return;
-      const int c = gap_class(scale, v);
-      if ((s.wanted[c >> 5] >> (c & 31) & 1u) && weight_units(weight_wide(scale, v)) != 0) {
-        const int at = atomicAdd(&s.size, 1);
-        if (at < kListMost) s.list[at] = place_key(v, i);
-      }
-    });
-    __syncthreads();
-    const int size = s.size;
-    uint64_t total = total_lo, kept;
+    uint64_t total = state.total_lo, kept;
     if (size <= kListMost) {
-      int span = 64;
-      while (span < size) span <<= 1;
-      for (int i = size + tid; i < span; i += kPickThreads) s.list[i] = 0;
+      // A token's running mass and rank: up to the class before, and of its own class what stands no later.  The list's tokens go into
+      // as many buckets as they are, a class's tokens into its own by their gap, in the order; what stands in earlier buckets
+      // comes from running sums, and a token is compared with those of its bucket alone.  (Compared with all of its class, 500 tokens
+      // of one class took 90 us.)
+      uint64_t key[kEach], units[kEach] = {}, reached[kEach];
+      uint32_t rank[kEach];
+      Listed own[kEach];
+      int bucket[kEach];
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) s.bucket_mass[kEach * tid + j] = 0, s.bucket_count[kEach * tid + j] = 0;
       __syncthreads();
-      for (int block = 2; block <= span; block <<= 1)
-        for (int step = block >> 1; step > 0; step >>= 1) {
-          for (int i = tid; i < span / 2; i += kPickThreads) {
-            const int a = 2 * i - (i & (step - 1)), b = a + step;
-            const uint64_t x = s.list[a], y = s.list[b];
-            if ((x < y) == ((a & block) == 0)) s.list[a] = y, s.list[b] = x;      // descending
-          }
-          __syncthreads();
-        }
-      // two neighbours of the list a thread
-      uint64_t key[2] = {0, 0}, units[2] = {0, 0}, reached[2] = {0, 0};
-      double wide[2] = {0.0, 0.0};
-      int cls[2] = {0, 0};
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (2 * tid + j < size) {
-          key[j] = s.list[2 * tid + j];
-          const float v = place_value(key[j]);
-          wide[j] = weight_wide(scale, v), units[j] = weight_units(wide[j]), cls[j] = gap_class(scale, v);
-        }
-      const uint64_t both = running_sum(units[0] + units[1], s.waves);
-      reached[0] = both - units[1] + s.adjust[cls[0]], reached[1] = both + s.adjust[cls[1]];
-      auto crossing = [&](uint64_t target, uint64_t otherwise, uint64_t* place) {      // the running mass where it first reaches target
-        if (tid == 0) s.result = otherwise, s.result2 = best;
-        __syncthreads();
+      for (int j = 0; j < kEach; ++j) {
+        const int i = tid + j * kPickThreads;
+        if (i >= size) continue;
+        own[j] = list[i];
+        key[j] = own[j].key, units[j] = own[j].units;
+        const float v = place_value(key[j]);
+        // (the gap in classes without the whole ones, of the last class's tokens possibly more than one)
+        const float x = v < scale.max ? (scale.max - v) * scale.class_scale : 0.f;
+        const float inside = fminf(fmaxf(x - fminf(floorf(x), static_cast<float>(kClasses - 1)), 0.f) * 2048.f, 2047.f);
+        bucket[j] = static_cast<int>(own[j].begin + ((static_cast<uint32_t>(inside) * (own[j].end - own[j].begin)) >> 11));
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.bucket_mass[bucket[j]]), static_cast<unsigned long long>(units[j]));
+        atomicAdd(&s.bucket_count[bucket[j]], 1u);
+      }
+      __syncthreads();
+      {
+        uint64_t mass[kEach], all = 0;
+        uint32_t count[kEach], all_n = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (units[j] != 0 && reached[j] >= target && reached[j] - units[j] < target) s.result = reached[j], s.result2 = key[j];
-        __syncthreads();
-        const uint64_t found = s.result;
-        *place = s.result2;
-        __syncthreads();
-        return found;
-      };
-      uint64_t place;
+        for (int j = 0; j < kEach; ++j) all += mass[j] = s.bucket_mass[kEach * tid + j], all_n += count[j] = s.bucket_count[kEach * tid + j];
+        const uint64_t own_all = all;
+        const uint32_t own_n = all_n;
+        running_sums<kPickThreads>(s.wave_mass, s.wave_count, all, all_n);
+        all -= own_all, all_n -= own_n;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          s.bucket_mass[kEach * tid + j] = all, s.place[kEach * tid + j] = all_n;          // before the bucket
+          all += mass[j], all_n += count[j];
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (units[j] == 0) continue;
+        // (the mass before the bucket in its class: before the class's first bucket the list holds what is not the row's)
+        reached[j] = own[j].mass_before + s.bucket_mass[bucket[j]] - s.bucket_mass[own[j].begin];
+        rank[j] = own[j].count_before + s.place[bucket[j]] - own[j].begin;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (units[j] != 0) s.list[atomicAdd(&s.place[bucket[j]], 1u)] = Entry{key[j], units[j]};
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (units[j] == 0) continue;
+        const uint32_t end = s.place[bucket[j]];
+        for (uint32_t other = end - s.bucket_count[bucket[j]]; other < end; ++other) {
+          const Entry entry = s.list[other];
+          const bool stands = entry.key >= key[j];
+          reached[j] += stands ? entry.units : 0, rank[j] += stands ? 1 : 0;
+        }
+      }
+      auto crosses = [&](int j, uint64_t target) { return units[j] != 0 && reached[j] >= target && reached[j] - units[j] < target; };
       if (cut_k) {
-        if (tid == 0) s.result = total_hi;
-        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (units[j] != 0 && 2 * tid + j + 1 + s.adjust_count[cls[j]] == static_cast<uint32_t>(k)) s.result = reached[j];
+        for (int j = 0; j < kEach; ++j)
+          if (units[j] != 0 && rank[j] == static_cast<uint32_t>(k)) s.answers[0] = reached[j];
         __syncthreads();
-        total = s.result;
-        __syncthreads();
+        total = s.answers[0];
       }
       kept = total;
-      if (cut_p) kept = crossing(max(share_of(fmaxf(p_share, 0.f), total, true), static_cast<uint64_t>(1)), total, &place);
-      if (cut_m) {
-        if (tid == 0) s.result = kept_floor;
-        __syncthreads();
+      if (cut_p) {
+        const uint64_t target = target_of(p_share, total);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (units[j] != 0 && wide[j] >= least_weight) atomicMax(reinterpret_cast<unsigned long long*>(&s.result), static_cast<unsigned long long>(reached[j]));
+        for (int j = 0; j < kEach; ++j)
+          if (crosses(j, target)) s.answers[1] = reached[j];
         __syncthreads();
-        kept = min(kept, s.result);
-        __syncthreads();
+        kept = s.answers[1];
       }
-      crossing(goal_of(kept) + 1, 0, &place);
-      chosen = place;
+      if (cut_m) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+          if (units[j] != 0 && weight_wide(scale, place_value(key[j])) >= least_weight)
+            atomicMax(reinterpret_cast<unsigned long long*>(&s.answers[2]), static_cast<unsigned long long>(reached[j]));
+        __syncthreads();
+        kept = min(kept, s.answers[2]);
+      }
+      const uint64_t goal = goal_of(u, kept);
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (crosses(j, goal)) s.answer_key = key[j];
+      __syncthreads();
+      chosen = s.answer_key;
     } else {
       uint64_t place;
+      __syncthreads();
       if (cut_k) total = descend(s, row, vocab, scale, static_cast<uint64_t>(k), true, &place);
       kept = total;
-      if (cut_p) kept = descend(s, row, vocab, scale, max(share_of(fmaxf(p_share, 0.f), total, true), static_cast<uint64_t>(1)), false, &place);
+      if (cut_p) kept = descend(s, row, vocab, scale, target_of(p_share, total), false, &place);
       if (cut_m) {
-        if (tid == 0) s.result = 0;
+        if (tid == 0) s.answers[3] = 0;
         __syncthreads();
-        scan_tokens<kPickThreads>(row, 0, vocab, [&](int, float v) {
-          const double wide = weight_wide(scale, v);
-          if (v > -INFINITY && wide >= least_weight)
-            atomicAdd(reinterpret_cast<unsigned long long*>(&s.result), static_cast<unsigned long long>(weight_units(wide)));
+        scan_tokens<kPickThreads, 4>(row, 0, vocab, [&](int first, const float4& four) {
+          each_of(first, four, [&](int, float v) {
+            const double wide = weight_wide(scale, v);
+            if (v > -INFINITY && wide >= least_weight)
+              atomicAdd(reinterpret_cast<unsigned long long*>(&s.answers[3]), static_cast<unsigned long long>(weight_units(wide)));
+          });
         });
         __syncthreads();
-        kept = min(kept, max(s.result, one));
-        __syncthreads();
+        kept = min(kept, max(s.answers[3], one));
       }
-      descend(s, row, vocab, scale, goal_of(kept) + 1, false, &chosen);
+      descend(s, row, vocab, scale, goal_of(u, kept), false, &chosen);
     }
   }
   if (tid == 0) {
     out[r] = place_index(chosen);
-    if (logprob) {
-      double sum = 0.0;
-      for (int p = 0; p < parts; ++p) sum += sums[static_cast<size_t>(r) * parts + p];
-      logprob[r] = static_cast<float>(static_cast<double>(place_value(chosen)) - static_cast<double>(place_value(best)) - log(sum));
-    }
+    if (logprob) logprob[r] = static_cast<float>(static_cast<double>(place_value(chosen)) - static_cast<double>(place_value(best)) - log_sum);
   }
 }
 
@@ -492,31 +727,34 @@ draw_pick_kernel(const float* __restrict__ logits, int vocab, int parts, const P
 
 using namespace tlie;
 
-// How the entry's scratch is laid out, for `parts` parts a row: the parts' statistics, their sums, their classes' masses and counts.
-extern "C" long long tlie_draw_scratch_bytes(int rows, int parts) {
-  if (rows <= 0 || parts <= 0) return 0;
-  return static_cast<long long>(rows) * parts * (static_cast<long long>(sizeof(PartStat)) + 8 + kClasses * 12);
-}
+// The entry's scratch, for `parts` parts a row: the rows' lists and states, the parts' statistics, sums, masses and counts of classes.
+constexpr long long kRowBytes = sizeof(RowState) + kListMost * sizeof(Listed), kPartBytes = sizeof(PartStat) + 8 + kClasses * 12;
+static_assert(sizeof(RowState) == 32 && sizeof(Listed) == 40 && sizeof(PartStat) == 16, "the host's face counts them so");
 
-// logits: float [rows, vocab], vocab < 2^24; uniform: float [rows]; temperature, top_k, top_p, min_p: [rows] or null; out: int [rows];
-// logprob: float [rows] or null.  scratch: tlie_draw_scratch_bytes(rows, parts), at a multiple of 16 bytes.
+// logits: float [rows, vocab], vocab < 2^24; uniform: float [rows]; temperature, top_k, top_p, min_p: [rows] or null; parts: 1 to 16;
+// out: int [rows]; logprob: float [rows] or null.  scratch: rows * (kRowBytes + parts * kPartBytes) bytes, at a multiple of 16.
 extern "C" int tlie_draw(const float* logits, int rows, int vocab, const float* uniform, const float* temperature, const int* top_k,
                          const float* top_p, const float* min_p, int parts, void* scratch, int* out, float* logprob, void* stream) {
-  if (rows <= 0 || vocab <= 0 || vocab >= (1 << 24) || parts <= 0 || parts > 65535 || rows > 65535 || scratch == nullptr || uniform == nullptr)
+  if (rows <= 0 || vocab <= 0 || vocab >= (1 << 24) || parts <= 0 || parts > kPartsMost || rows > 65535 || scratch == nullptr || uniform == nullptr)
     return kBadArgument;
   hipStream_t s = (hipStream_t)stream;
   const int part_len = (vocab + parts - 1) / parts;
   int shift = 44;                                   // the weights' sum stays below 2^62
-  while (shift > 36 && (static_cast<long long>(vocab) << shift) >= (1ll << 62)) --shift;
+  while ((static_cast<long long>(vocab) << shift) >= (1ll << 62)) --shift;
   const size_t places = static_cast<size_t>(rows) * parts;
-  PartStat* stats = static_cast<PartStat*>(scratch);
+  Listed* lists = static_cast<Listed*>(scratch);
+  RowState* states = reinterpret_cast<RowState*>(lists + static_cast<size_t>(rows) * kListMost);
+  PartStat* stats = reinterpret_cast<PartStat*>(states + rows);
   double* sums = reinterpret_cast<double*>(stats + places);
   uint64_t* class_mass = reinterpret_cast<uint64_t*>(sums + places);
   uint32_t* class_count = reinterpret_cast<uint32_t*>(class_mass + places * kClasses);
   hipLaunchKernelGGL(draw_best_kernel, dim3(parts, rows), dim3(kPartThreads), 0, s, logits, vocab, part_len, parts, stats);
   hipLaunchKernelGGL(draw_weigh_kernel, dim3(parts, rows), dim3(kPartThreads), 0, s, logits, vocab, part_len, parts, stats, temperature, shift,
                      logprob != nullptr ? 1 : 0, class_mass, class_count, sums);
+  if (temperature != nullptr)
+    hipLaunchKernelGGL(draw_gather_kernel, dim3(parts, rows), dim3(kGatherThreads), 0, s, logits, vocab, part_len, parts, stats, uniform, temperature,
+                     top_k, top_p, min_p, shift, class_mass, class_count, states, lists);
   hipLaunchKernelGGL(draw_pick_kernel, dim3(rows), dim3(kPickThreads), 0, s, logits, vocab, parts, stats, uniform, temperature, top_k, top_p, min_p,
-                     shift, class_mass, class_count, sums, out, logprob);
+                     shift, states, lists, sums, out, logprob);
   return launch_status();
 }

@@ -2098,11 +2098,12 @@ def _one_device(what: str, *tensors) -> None:
 
 
 DRAW_MAX_VOCAB = (1 << 24) - 1
+DRAW_ROW_BYTES, DRAW_PART_BYTES = 32 + 2048 * 40, 24 + 1024 * 12      # of scratch: csrc/draw.hip's kRowBytes and kPartBytes
 
 
 def draw_parts(rows: int, vocab: int) -> int:
-    """Into how many parts `sample_filtered` cuts each row: a thousand workgroups in all, of 2048 tokens at least each."""
-    return max(1, min(1024 // max(rows, 1), 16, (vocab + 2047) // 2048))
+    """Into how many parts `sample_filtered` cuts each row: two workgroups of 512 threads a compute unit, of 2048 tokens at least."""
+    return max(1, min(512 // max(rows, 1), 16, (vocab + 2047) // 2048))
 
 
 def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
@@ -2144,9 +2145,7 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: to
         out_logprobs = torch.empty((rows,), dtype=torch.float32, device=logits.device)
     if rows > 0:
         parts = draw_parts(rows, vocab)
-        size = library().tlie_draw_scratch_bytes
-        size.restype = ctypes.c_longlong
-        scratch = torch.empty((size(rows, parts),), dtype=torch.uint8, device=logits.device)
+        scratch = torch.empty((rows * (DRAW_ROW_BYTES + parts * DRAW_PART_BYTES),), dtype=torch.uint8, device=logits.device)
         _check(library().tlie_draw(_ptr(logits), rows, vocab, _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), parts,
                                    _ptr(scratch), _ptr(out), _ptr(out_logprobs), _stream()), "sample_filtered")
     return (out, out_logprobs) if logprobs else out
