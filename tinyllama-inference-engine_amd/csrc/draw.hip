@@ -380,10 +380,11 @@ draw_gather_kernel(const float* __restrict__ logits, int vocab, int part_len, in
     }
 #pragma unroll
     for (int p = 0; p < kParts; ++p) {
-      if (p0 + p >= parts) break;
-      mass[0] += m[p][0].x, mass[1] += m[p][0].y, mass[2] += m[p][1].x, mass[3] += m[p][1].y;
-      if (p0 + p < part) ahead[0] += n[p].x, ahead[1] += n[p].y, ahead[2] += n[p].z, ahead[3] += n[p].w;
-      count[0] += n[p].x, count[1] += n[p].y, count[2] += n[p].z, count[3] += n[p].w;
+      // (selected, not branched around: the loads would move behind the branch, and each be waited for by itself)
+      const bool is = p0 + p < parts, before = p0 + p < part;
+      mass[0] += is ? m[p][0].x : 0, mass[1] += is ? m[p][0].y : 0, mass[2] += is ? m[p][1].x : 0, mass[3] += is ? m[p][1].y : 0;
+      ahead[0] += before ? n[p].x : 0, ahead[1] += before ? n[p].y : 0, ahead[2] += before ? n[p].z : 0, ahead[3] += before ? n[p].w : 0;
+      count[0] += is ? n[p].x : 0, count[1] += is ? n[p].y : 0, count[2] += is ? n[p].z : 0, count[3] += is ? n[p].w : 0;
     }
   }
   uint64_t running[kOwn];

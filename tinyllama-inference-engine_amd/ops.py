@@ -2102,8 +2102,10 @@ DRAW_ROW_BYTES, DRAW_PART_BYTES = 32 + 2048 * 40, 24 + 1024 * 12      # of scrat
 
 
 def draw_parts(rows: int, vocab: int) -> int:
-    """Into how many parts `sample_filtered` cuts each row: two workgroups of 512 threads a compute unit, of 2048 tokens at least."""
-    return max(1, min(512 // max(rows, 1), 16, (vocab + 2047) // 2048))
+    """Into how many parts `sample_filtered` cuts each row, at most 8: each brings a histogram to write and, by all of them, to read.  Up to
+    16 rows parts of 4096 tokens fill the chip, beyond of 8192, with a thousand workgroups at most (1 row of 32000 tokens in 8 parts 21 us,
+    in 4 22, in 16 23; 64 rows of 32000 in 4 parts 34, in 2 and 8 40; 64 rows of 128256 in 8 parts 54, in 4 62; 256 rows in 4 parts 112, in 8 128)."""
+    return max(1, min(8, 1024 // max(rows, 1), -(-vocab // (4096 if rows <= 16 else 8192))))
 
 
 def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
