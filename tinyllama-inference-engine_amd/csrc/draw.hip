@@ -20,7 +20,7 @@
 
 namespace tlie {
 
-constexpr int kClasses = 1024, kPartThreads = 512, kGatherThreads = 256, kPickThreads = 512, kListMost = 2048, kPartsMost = 16;
+constexpr int kClasses = 1024, kPartThreads = 512, kGatherThreads = 256, kPickThreads = 512, kRowThreads = 1024, kListMost = 2048, kPartsMost = 8;
 
 // 2^(j / 128)
 constexpr int kPowers = 128;
@@ -236,6 +236,20 @@ __device__ __forceinline__ void join_stats(const PartStat* __restrict__ stats, i
   }
 }
 
+__device__ __forceinline__ void weigh_token(const RowScale& scale, float v, unsigned long long* mass, uint32_t* count) {
+  const uint64_t units = weight_units(weight_wide(scale, v));
+  if (units != 0) {
+    const int c = gap_class(scale, v);
+    atomicAdd(&mass[c], static_cast<unsigned long long>(units));
+    atomicAdd(&count[c], 1u);
+  }
+}
+// exp(v - max), for the log-probability: an exponential's rounding of 2^-23 each, a sum of four in 32 bits, the rest in 64
+__device__ __forceinline__ double plain_weights(float max, const float4& v) {
+  auto plain = [&](float x) { return __builtin_amdgcn_exp2f((x - max) * 1.44269502f); };
+  return static_cast<double>((plain(v.x) + plain(v.y)) + (plain(v.z) + plain(v.w)));
+}
+
 __global__ void __launch_bounds__(kPartThreads)
 draw_weigh_kernel(const float* __restrict__ logits, int vocab, int part_len, int parts, const PartStat* __restrict__ stats,
                   const float* __restrict__ temperature, int shift, int want_sum, uint64_t* __restrict__ class_mass,
@@ -258,18 +272,8 @@ draw_weigh_kernel(const float* __restrict__ logits, int vocab, int part_len, int
   const RowScale scale = row_scale(place_value(best), least, t, shift, powers);
   double sum = 0.0;
   scan_tokens<kPartThreads, 4>(logits + static_cast<size_t>(row) * vocab, begin, end, [&](int first, const float4& four) {
-    if (drawn)
-      each_of(first, four, [&](int, float v) {
-        const uint64_t units = weight_units(weight_wide(scale, v));
-        if (units != 0) {
-          const int c = gap_class(scale, v);
-          atomicAdd(&mass[c], static_cast<unsigned long long>(units));
-          atomicAdd(&count[c], 1u);
-        }
-      });
-    // exp(v - max), for the log-probability: an exponential's rounding of 2^-23 each, a sum of four in 32 bits, the rest in 64
-    auto plain = [&](float v) { return __builtin_amdgcn_exp2f((v - scale.max) * 1.44269502f); };
-    if (want_sum) sum += static_cast<double>((plain(four.x) + plain(four.y)) + (plain(four.z) + plain(four.w)));
+    if (drawn) each_of(first, four, [&](int, float v) { weigh_token(scale, v, mass, count); });
+    if (want_sum) sum += plain_weights(scale.max, four);
   });
   const size_t place = static_cast<size_t>(row) * parts + part;
   if (drawn) {
@@ -330,72 +334,48 @@ __device__ __forceinline__ void running_sums(uint64_t* wave_mass, uint32_t* wave
   mass += m, count += n;
 }
 
-struct GatherShared {
-  uint64_t running_mass[kClasses];          // up to and with each class
-  uint32_t running_count[kClasses];
-  uint32_t begin[kClasses];                 // a wanted class's first place in the list, or kNotListed
-  uint32_t place[kClasses];                 // where this part's next token of the class goes
-  uint64_t wave_mass[kGatherThreads / kWave];
-  uint32_t wave_count[kGatherThreads / kWave], listed_count[kGatherThreads / kWave];
-  double powers[kPowers];
-  int found[7];                             // classes, a place for each question
+// What a row asks for.
+struct Ask {
+  float t, p, floor, u;
+  int k;
 };
-
-// The answers' bounds are the same in both kernels.
+__device__ __forceinline__ Ask ask_of(int r, const float* uniform, const float* temperature, const int* top_k, const float* top_p, const float* min_p) {
+  return Ask{temperature ? temperature[r] : 0.f, top_p ? top_p[r] : 1.f, min_p ? min_p[r] : 0.f, fmaxf(uniform[r], 0.f), top_k ? top_k[r] : 0};
+}                                                                 // (a random number that is a NaN counts as 0)
 __device__ __forceinline__ uint64_t goal_of(float u, uint64_t kept) { return (u < 1.f ? share_of(u, kept, false) : kept - 1) + 1; }
 __device__ __forceinline__ uint64_t target_of(float p, uint64_t total) { return max(share_of(fmaxf(p, 0.f), total, true), static_cast<uint64_t>(1)); }
 
-__global__ void __launch_bounds__(kGatherThreads)
-draw_gather_kernel(const float* __restrict__ logits, int vocab, int part_len, int parts, const PartStat* __restrict__ stats,
-                   const float* __restrict__ uniform, const float* __restrict__ temperature, const int* __restrict__ top_k,
-                   const float* __restrict__ top_p, const float* __restrict__ min_p, int shift, const uint64_t* __restrict__ class_mass,
-                   const uint32_t* __restrict__ class_count, RowState* __restrict__ states, Listed* __restrict__ lists) {
-  __shared__ GatherShared s;
-  const int r = blockIdx.y, part = blockIdx.x, tid = threadIdx.x;
-  const float t = temperature ? temperature[r] : 0.f, p_share = top_p ? top_p[r] : 1.f, floor_p = min_p ? min_p[r] : 0.f;
-  const float u = fmaxf(uniform[r], 0.f);                                                 // (a NaN counts as 0)
-  const int k = top_k ? top_k[r] : 0;
-  if (!(t > 0.f)) return;
-  uint64_t best;
-  float least;
-  join_stats(stats + static_cast<size_t>(r) * parts, parts, best, least);
-  if (best == kBadPart || best == 0) return;
-  bring_powers<kGatherThreads>(s.powers, shift);
-  const RowScale scale = row_scale(place_value(best), least, t, shift, s.powers);
-  const uint64_t one = 1ull << shift;
-  // ---- the row's classes, four neighbours a thread; eight parts are asked for together.  (Four waves: with a class a thread, sixteen
-  // waves do what is the same for all of the row, and 64 rows in 8 parts took 20 us) ----
-  constexpr int kOwn = kClasses / kGatherThreads, kParts = 8;
-  static_assert(kOwn == 4, "classes are loaded as 16-byte pieces");
-  uint64_t mass[kOwn] = {};
-  uint32_t count[kOwn] = {}, ahead[kOwn] = {};                    // (ahead: of the parts before this one)
-  for (int p0 = 0; p0 < parts; p0 += kParts) {
-    ulonglong2 m[kParts][2];
-    uint4 n[kParts];
-#pragma unroll
-    for (int p = 0; p < kParts; ++p) {
-      const size_t place = (static_cast<size_t>(r) * parts + min(p0 + p, parts - 1)) * kClasses + kOwn * tid;
-      m[p][0] = *reinterpret_cast<const ulonglong2*>(class_mass + place), m[p][1] = *reinterpret_cast<const ulonglong2*>(class_mass + place + 2);
-      n[p] = *reinterpret_cast<const uint4*>(class_count + place);
-    }
-#pragma unroll
-    for (int p = 0; p < kParts; ++p) {
-      // (selected, not branched around: the loads would move behind the branch, and each be waited for by itself)
-      const bool is = p0 + p < parts, before = p0 + p < part;
-      mass[0] += is ? m[p][0].x : 0, mass[1] += is ? m[p][0].y : 0, mass[2] += is ? m[p][1].x : 0, mass[3] += is ? m[p][1].y : 0;
-      ahead[0] += before ? n[p].x : 0, ahead[1] += before ? n[p].y : 0, ahead[2] += before ? n[p].z : 0, ahead[3] += before ? n[p].w : 0;
-      count[0] += is ? n[p].x : 0, count[1] += is ? n[p].y : 0, count[2] += is ? n[p].z : 0, count[3] += is ? n[p].w : 0;
-    }
-  }
+template <int THREADS>
+struct ClassShared {
+  uint64_t running_mass[kClasses];          // up to and with each class
+  uint32_t running_count[kClasses];
+  uint32_t begin[kClasses];                 // a wanted class's first place in the list, or kNotListed
+  uint32_t place[kClasses];                 // where its next token goes
+  uint64_t wave_mass[THREADS / kWave];
+  uint32_t wave_count[THREADS / kWave], listed_count[THREADS / kWave];
+  int found[7];                             // classes, a place for each question
+};
+
+// From the masses and counts of a thread's own classes (kClasses / THREADS neighbours): which classes the crossings lie in, and
+// where their tokens go in the list, class after class, `ahead` of them left free at each class's start.  The whole workgroup; what it
+// leaves in s may be read at once.
+template <int THREADS>
+__device__ RowState find_classes(ClassShared<THREADS>& s, const RowScale& scale, uint64_t one, const Ask& ask,
+                                 const uint64_t (&mass)[kClasses / THREADS], const uint32_t (&count)[kClasses / THREADS],
+                                 const uint32_t (&ahead)[kClasses / THREADS]) {
+  constexpr int kOwn = kClasses / THREADS;
+  const int tid = threadIdx.x;
   uint64_t running[kOwn];
   uint32_t running_n[kOwn];
   {
-    uint64_t all = (mass[0] + mass[1]) + (mass[2] + mass[3]);
-    uint32_t all_n = (count[0] + count[1]) + (count[2] + count[3]);
+    uint64_t all = 0;
+    uint32_t all_n = 0;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) all += mass[j], all_n += count[j];
     const uint64_t own = all;
     const uint32_t own_n = all_n;
     if (tid < 7) s.found[tid] = kClasses;
-    running_sums<kGatherThreads>(s.wave_mass, s.wave_count, all, all_n);
+    running_sums<THREADS>(s.wave_mass, s.wave_count, all, all_n);
     all -= own, all_n -= own_n;
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) {
@@ -417,46 +397,47 @@ draw_gather_kernel(const float* __restrict__ logits, int vocab, int part_len, in
   };
 
   // ---- which classes the crossings can lie in.  A class that is cut leaves what follows with a range of masses ----
-  uint64_t total_lo = s.running_mass[kClasses - 1], total_hi = total_lo;
-  bool cut_k = false;
-  if (k > 0 && static_cast<uint32_t>(k) < s.running_count[kClasses - 1]) {
+  RowState state;
+  state.total_lo = state.total_hi = s.running_mass[kClasses - 1], state.kept_floor = one, state.cut_k = 0;
+  const uint32_t k = static_cast<uint32_t>(ask.k);
+  if (ask.k > 0 && k < s.running_count[kClasses - 1]) {
 #pragma unroll
     for (int j = 0; j < kOwn; ++j)
-      if (running_n[j] >= static_cast<uint32_t>(k) && running_n[j] - count[j] < static_cast<uint32_t>(k)) s.found[0] = kOwn * tid + j;
+      if (running_n[j] >= k && running_n[j] - count[j] < k) s.found[0] = kOwn * tid + j;
     __syncthreads();
     const int c = s.found[0];
-    total_hi = mass_upto(c), total_lo = s.running_count[c] == static_cast<uint32_t>(k) ? total_hi : mass_upto(c - 1);
-    cut_k = total_lo != total_hi;
-    if (cut_k) want(c, c);
+    state.total_hi = mass_upto(c), state.total_lo = s.running_count[c] == k ? state.total_hi : mass_upto(c - 1);
+    state.cut_k = state.total_lo != state.total_hi;
+    if (state.cut_k) want(c, c);
   }
-  uint64_t kept_lo = total_lo, kept_hi = total_hi, kept_floor = one;
-  if (p_share < 1.f) {
-    const uint64_t low = target_of(p_share, total_lo);
+  uint64_t kept_lo = state.total_lo, kept_hi = state.total_hi;
+  if (ask.p < 1.f) {
+    const uint64_t low = target_of(ask.p, state.total_lo);
     reaches(1, low);
-    reaches(2, cut_k ? target_of(p_share, total_hi) : low);
+    reaches(2, state.cut_k ? target_of(ask.p, state.total_hi) : low);
     __syncthreads();
     const int c_lo = s.found[1], c_hi = s.found[2];
     want(c_lo, c_hi);
     kept_lo = mass_upto(c_lo - 1), kept_hi = min(kept_hi, mass_upto(c_hi));
   }
-  if (floor_p > 0.f) {
+  if (ask.floor > 0.f) {
     // the class of the gap at which the weight is min_p, and its neighbours, for the rounding of the gap
-    const float gap = fmaxf(-logf(fminf(floor_p, 1.f)) * t, 0.f);
+    const float gap = fmaxf(-logf(fminf(ask.floor, 1.f)) * ask.t, 0.f);
     const int c = static_cast<int>(fminf(gap * scale.class_scale, static_cast<float>(kClasses - 1)));
     want(c - 1, c + 1);
-    kept_floor = max(one, mass_upto(c - 2));
-    kept_lo = min(kept_lo, kept_floor), kept_hi = min(kept_hi, mass_upto(c + 1));
+    state.kept_floor = max(one, mass_upto(c - 2));
+    kept_lo = min(kept_lo, state.kept_floor), kept_hi = min(kept_hi, mass_upto(c + 1));
   }
   kept_lo = max(kept_lo, one), kept_hi = max(kept_hi, one);       // (the first token is always kept)
-  const uint64_t goal = goal_of(u, kept_lo);
+  const uint64_t goal = goal_of(ask.u, kept_lo);
   reaches(3, goal);
-  reaches(4, kept_lo != kept_hi ? goal_of(u, kept_hi) : goal);
+  reaches(4, kept_lo != kept_hi ? goal_of(ask.u, kept_hi) : goal);
   __syncthreads();
   want(s.found[3], s.found[4]);
 
-  // ---- their tokens: class after class in the list, and of a class part after part ----
+  // ---- their places in the list ----
   uint64_t nothing = 0;
-  uint32_t listed = 0, own_listed;
+  uint32_t listed = 0;
 #pragma unroll
   for (int j = 0; j < kOwn; ++j) {
     wanted[j] = wanted[j] && mass[j] != 0;
@@ -465,8 +446,8 @@ draw_gather_kernel(const float* __restrict__ logits, int vocab, int part_len, in
       atomicMin(&s.found[5], kOwn * tid + j), atomicMin(&s.found[6], kClasses - 1 - (kOwn * tid + j));
     }
   }
-  own_listed = listed;
-  running_sums<kGatherThreads>(s.wave_mass, s.listed_count, nothing, listed);
+  const uint32_t own_listed = listed;
+  running_sums<THREADS>(s.wave_mass, s.listed_count, nothing, listed);
   listed -= own_listed;
 #pragma unroll
   for (int j = 0; j < kOwn; ++j) {
@@ -474,62 +455,175 @@ draw_gather_kernel(const float* __restrict__ logits, int vocab, int part_len, in
     s.place[kOwn * tid + j] = listed + ahead[j];
     listed += wanted[j] ? count[j] : 0;
   }
-  uint32_t size = 0;
+  state.size = 0;
 #pragma unroll
-  for (int w = 0; w < kGatherThreads / kWave; ++w) size += s.listed_count[w];
-  if (part == 0 && tid == 0) states[r] = RowState{total_lo, total_hi, kept_floor, size, cut_k ? 1u : 0u};
-  if (size > kListMost) return;
+  for (int w = 0; w < THREADS / kWave; ++w) state.size += s.listed_count[w];
   __syncthreads();
-  // The classes in question are bounded by values, so that the others' tokens cost a comparison (differences of logits are
-  // rounded to 2^-24 of the larger, and the class's bound again: room on either side).
+  return state;
+}
+
+// The values between which the classes in question lie, so that the others' tokens cost a comparison (differences of logits are
+// rounded to 2^-24 of the larger, and the class's bound again: room on either side).
+template <int THREADS>
+__device__ __forceinline__ void value_bounds(const ClassShared<THREADS>& s, const RowScale& scale, float least, float& lower, float& upper) {
   const int c_first = s.found[5], c_last = kClasses - 1 - s.found[6];
-  float lower = -3.4028235e38f, upper = INFINITY;
+  lower = -3.4028235e38f, upper = INFINITY;
   if (scale.class_scale > 0.f) {                                  // (else every token is of the first class)
     const float room = fmaxf(fabsf(scale.max), fabsf(least)) * 2.4e-7f;
     upper = scale.max - static_cast<float>(c_first) * 0.99999f / scale.class_scale + room;
     if (c_last < kClasses - 1) lower = scale.max - static_cast<float>(c_last + 1) * 1.00001f / scale.class_scale - room;
   }
-  const int begin = part * part_len, end = min(vocab, begin + part_len);
-  Listed* list = lists + static_cast<size_t>(r) * kListMost;
-  scan_tokens<kGatherThreads, 8>(logits + static_cast<size_t>(r) * vocab, begin, end, [&](int first, const float4& four) {
-    if (!(fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w)) >= lower && fminf(fminf(four.x, four.y), fminf(four.z, four.w)) <= upper)) return;
-    each_of(first, four, [&](int i, float v) {
-      if (!(v >= lower && v <= upper)) return;
-      const int c = gap_class(scale, v);
-      if (s.begin[c] == kNotListed) return;
-      const uint64_t units = weight_units(weight_wide(scale, v));
-      if (units == 0) return;
-      const uint32_t before = c > 0 ? s.running_count[c - 1] : 0, from = s.begin[c];
-      list[atomicAdd(&s.place[c], 1u)] = Listed{place_key(v, i), units, c > 0 ? s.running_mass[c - 1] : 0, before, from, from + s.running_count[c] - before, 0};
-    });
+}
+__device__ __forceinline__ bool any_between(const float4& v, float lower, float upper) {
+  return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= lower && fminf(fminf(v.x, v.y), fminf(v.z, v.w)) <= upper;
+}
+// found(place in the list, key, weight, class) for each token of a group that a wanted class holds
+template <int THREADS, typename F>
+__device__ __forceinline__ void list_group(ClassShared<THREADS>& s, const RowScale& scale, float lower, float upper, int first, const float4& four, F found) {
+  if (!any_between(four, lower, upper)) return;
+  each_of(first, four, [&](int i, float v) {
+    if (!(v >= lower && v <= upper)) return;
+    const int c = gap_class(scale, v);
+    if (s.begin[c] == kNotListed) return;
+    const uint64_t units = weight_units(weight_wide(scale, v));
+    if (units != 0) found(atomicAdd(&s.place[c], 1u), place_key(v, i), units, c);
   });
+}
+template <int THREADS>
+__device__ __forceinline__ Listed listed_of(const ClassShared<THREADS>& s, uint64_t key, uint64_t units, int c) {
+  const uint32_t before = c > 0 ? s.running_count[c - 1] : 0, from = s.begin[c];
+  return Listed{key, units, c > 0 ? s.running_mass[c - 1] : 0, before, from, from + s.running_count[c] - before, 0};
 }
 
 struct Entry {
   uint64_t key, units;
 };
-
-struct PickShared {
+template <int THREADS>
+struct CrossShared {
   Entry list[kListMost];                    // bucket by bucket
   uint64_t bucket_mass[kListMost];          // of a bucket, then up to it
   uint32_t bucket_count[kListMost], place[kListMost];
-  uint64_t wave_mass[kPickThreads / kWave];
-  uint32_t wave_count[kPickThreads / kWave];
-  double powers[kPowers];
+  uint64_t wave_mass[THREADS / kWave];
+  uint32_t wave_count[THREADS / kWave];
   uint64_t digit_mass[256];
   uint32_t digit_count[256];
   uint64_t answers[4], answer_key;          // of the crossings
   int found;
 };
 
+// The chosen token, from the list: entry(i) is its i-th.
+template <int THREADS, typename F>
+__device__ uint64_t cross(CrossShared<THREADS>& s, const RowScale& scale, const Ask& ask, const RowState& state, uint64_t best, F entry) {
+  constexpr int kEach = kListMost / THREADS;
+  const int tid = threadIdx.x, size = static_cast<int>(state.size);
+  // A token's running mass and rank: up to the class before, and of its own class what stands no later.  The list's tokens go into
+  // as many buckets as they are, a class's tokens into its own by their gap, in the order; what stands in earlier buckets
+  // comes from running sums, and a token is compared with those of its bucket alone.  (Compared with all of its class, 500 tokens
+  // of one class took 90 us.)
+  uint64_t key[kEach], units[kEach] = {}, reached[kEach];
+  uint32_t rank[kEach];
+  Listed own[kEach];
+  int bucket[kEach];
+  if (tid == 0) s.answers[0] = state.total_hi, s.answers[1] = state.total_hi, s.answers[2] = state.kept_floor, s.answer_key = best;
+  for (int b = tid; b < kListMost; b += THREADS) s.bucket_mass[b] = 0, s.bucket_count[b] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = tid + j * THREADS;
+    if (i >= size) continue;
+    own[j] = entry(i);
+    key[j] = own[j].key, units[j] = own[j].units;
+    const float v = place_value(key[j]);
+    // (the gap in classes without the whole ones, of the last class's tokens possibly more than one)
+    const float x = v < scale.max ? (scale.max - v) * scale.class_scale : 0.f;
+    const float inside = fminf(fmaxf(x - fminf(floorf(x), static_cast<float>(kClasses - 1)), 0.f) * 2048.f, 2047.f);
+    bucket[j] = static_cast<int>(own[j].begin + ((static_cast<uint32_t>(inside) * (own[j].end - own[j].begin)) >> 11));
+    atomicAdd(reinterpret_cast<unsigned long long*>(&s.bucket_mass[bucket[j]]), static_cast<unsigned long long>(units[j]));
+    atomicAdd(&s.bucket_count[bucket[j]], 1u);
+  }
+  __syncthreads();
+  {
+    uint64_t mass[kEach], all = 0;
+    uint32_t count[kEach], all_n = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) all += mass[j] = s.bucket_mass[kEach * tid + j], all_n += count[j] = s.bucket_count[kEach * tid + j];
+    const uint64_t own_all = all;
+    const uint32_t own_n = all_n;
+    running_sums<THREADS>(s.wave_mass, s.wave_count, all, all_n);
+    all -= own_all, all_n -= own_n;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      s.bucket_mass[kEach * tid + j] = all, s.place[kEach * tid + j] = all_n;              // before the bucket
+      all += mass[j], all_n += count[j];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (units[j] == 0) continue;
+    // (the mass before the bucket in its class: before the class's first bucket the list holds what is not the row's)
+    reached[j] = own[j].mass_before + s.bucket_mass[bucket[j]] - s.bucket_mass[own[j].begin];
+    rank[j] = own[j].count_before + s.place[bucket[j]] - own[j].begin;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (units[j] != 0) s.list[atomicAdd(&s.place[bucket[j]], 1u)] = Entry{key[j], units[j]};
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (units[j] == 0) continue;
+    const uint32_t end = s.place[bucket[j]];
+    for (uint32_t other = end - s.bucket_count[bucket[j]]; other < end; ++other) {
+      const Entry other_entry = s.list[other];
+      const bool stands = other_entry.key >= key[j];
+      reached[j] += stands ? other_entry.units : 0, rank[j] += stands ? 1 : 0;
+    }
+  }
+  auto crosses = [&](int j, uint64_t target) { return units[j] != 0 && reached[j] >= target && reached[j] - units[j] < target; };
+  uint64_t kept = state.total_lo;
+  if (state.cut_k) {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (units[j] != 0 && rank[j] == static_cast<uint32_t>(ask.k)) s.answers[0] = reached[j];
+    __syncthreads();
+    kept = s.answers[0];
+  }
+  if (ask.p < 1.f) {
+    const uint64_t target = target_of(ask.p, kept);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (crosses(j, target)) s.answers[1] = reached[j];
+    __syncthreads();
+    kept = s.answers[1];
+  }
+  if (ask.floor > 0.f) {
+    const double least_weight = static_cast<double>(fminf(ask.floor, 1.f)) * scale.one;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (units[j] != 0 && weight_wide(scale, place_value(key[j])) >= least_weight)
+        atomicMax(reinterpret_cast<unsigned long long*>(&s.answers[2]), static_cast<unsigned long long>(reached[j]));
+    __syncthreads();
+    kept = min(kept, s.answers[2]);
+  }
+  const uint64_t goal = goal_of(ask.u, kept);
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (crosses(j, goal)) s.answer_key = key[j];
+  __syncthreads();
+  return s.answer_key;
+}
+
 // Without a list (more tokens than it holds share the classes in question): the place in the order where the running mass
 // (or count) reaches target, found digit by digit of the place keys, eight passes over the row.  Returns the running mass there.
-__device__ uint64_t descend(PickShared& s, const float* __restrict__ row, int vocab, const RowScale& scale, uint64_t target, bool by_count, uint64_t* key) {
+template <int THREADS>
+__device__ __forceinline__ uint64_t descend(CrossShared<THREADS>& s, const float* __restrict__ row, int vocab, const RowScale& scale, uint64_t target, bool by_count,
+                                         uint64_t* key) {
   uint64_t prefix = 0, mass_before = 0, count_before = 0, mass = 0;
   for (int digit = 7; digit >= 0; --digit) {
-    for (int b = threadIdx.x; b < 256; b += kPickThreads) s.digit_mass[b] = 0, s.digit_count[b] = 0;
+    for (int b = threadIdx.x; b < 256; b += THREADS) s.digit_mass[b] = 0, s.digit_count[b] = 0;
     __syncthreads();
-    scan_tokens<kPickThreads, 4>(row, 0, vocab, [&](int first, const float4& four) {
+    scan_tokens<THREADS, 4>(row, 0, vocab, [&](int first, const float4& four) {
       each_of(first, four, [&](int i, float v) {
         if (!(v > -INFINITY)) return;
         const uint64_t place = place_key(v, i);
@@ -559,19 +653,92 @@ __device__ uint64_t descend(PickShared& s, const float* __restrict__ row, int vo
   *key = prefix;
   return mass;
 }
+template <int THREADS>
+__device__ uint64_t cross_without_list(CrossShared<THREADS>& s, const float* __restrict__ row, int vocab, const RowScale& scale, uint64_t one, const Ask& ask,
+                                       const RowState& state) {
+  uint64_t place = 0, kept = state.total_lo;
+  __syncthreads();
+  for (int step = 0; step < 3; ++step) {                          // top_k, top_p, the draw: a loop, so that the code is there once
+    if ((step == 0 && !state.cut_k) || (step == 1 && !(ask.p < 1.f))) continue;
+    if (step == 2 && ask.floor > 0.f) {
+      const double least_weight = static_cast<double>(fminf(ask.floor, 1.f)) * scale.one;
+      if (threadIdx.x == 0) s.answers[3] = 0;
+      __syncthreads();
+      scan_tokens<THREADS, 4>(row, 0, vocab, [&](int first, const float4& four) {
+        each_of(first, four, [&](int, float v) {
+          const double wide = weight_wide(scale, v);
+          if (v > -INFINITY && wide >= least_weight)
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.answers[3]), static_cast<unsigned long long>(weight_units(wide)));
+        });
+      });
+      __syncthreads();
+      kept = min(kept, max(s.answers[3], one));
+    }
+    const uint64_t target = step == 0 ? static_cast<uint64_t>(ask.k) : step == 1 ? target_of(ask.p, kept) : goal_of(ask.u, kept);
+    kept = descend(s, row, vocab, scale, target, step == 0, &place);
+  }
+  return place;
+}
+
+__global__ void __launch_bounds__(kGatherThreads)
+draw_gather_kernel(const float* __restrict__ logits, int vocab, int part_len, int parts, const PartStat* __restrict__ stats,
+                   const float* __restrict__ uniform, const float* __restrict__ temperature, const int* __restrict__ top_k,
+                   const float* __restrict__ top_p, const float* __restrict__ min_p, int shift, const uint64_t* __restrict__ class_mass,
+                   const uint32_t* __restrict__ class_count, RowState* __restrict__ states, Listed* __restrict__ lists) {
+  __shared__ ClassShared<kGatherThreads> s;
+  __shared__ double powers[kPowers];
+  const int r = blockIdx.y, part = blockIdx.x, tid = threadIdx.x;
+  const Ask ask = ask_of(r, uniform, temperature, top_k, top_p, min_p);
+  if (!(ask.t > 0.f)) return;
+  uint64_t best;
+  float least;
+  join_stats(stats + static_cast<size_t>(r) * parts, parts, best, least);
+  if (best == kBadPart || best == 0) return;
+  bring_powers<kGatherThreads>(powers, shift);
+  const RowScale scale = row_scale(place_value(best), least, ask.t, shift, powers);
+  // the row's classes, four neighbours a thread; all parts are asked for together.  (Four waves: with a class a thread, sixteen
+  // waves do what is the same for all of the row, and 64 rows in 8 parts took 20 us)
+  constexpr int kOwn = kClasses / kGatherThreads;
+  static_assert(kOwn == 4, "classes are loaded as 16-byte pieces");
+  uint64_t mass[kOwn] = {};
+  uint32_t count[kOwn] = {}, ahead[kOwn] = {};                    // (ahead: of the parts before this one)
+  ulonglong2 m[kPartsMost][2];
+  uint4 n[kPartsMost];
+#pragma unroll
+  for (int p = 0; p < kPartsMost; ++p) {
+    const size_t place = (static_cast<size_t>(r) * parts + min(p, parts - 1)) * kClasses + kOwn * tid;
+    m[p][0] = *reinterpret_cast<const ulonglong2*>(class_mass + place), m[p][1] = *reinterpret_cast<const ulonglong2*>(class_mass + place + 2);
+    n[p] = *reinterpret_cast<const uint4*>(class_count + place);
+  }
+#pragma unroll
+  for (int p = 0; p < kPartsMost; ++p) {
+    // (selected, not branched around: the loads would move behind the branch, and each be waited for by itself)
+    const bool is = p < parts, before = p < part;
+    mass[0] += is ? m[p][0].x : 0, mass[1] += is ? m[p][0].y : 0, mass[2] += is ? m[p][1].x : 0, mass[3] += is ? m[p][1].y : 0;
+    ahead[0] += before ? n[p].x : 0, ahead[1] += before ? n[p].y : 0, ahead[2] += before ? n[p].z : 0, ahead[3] += before ? n[p].w : 0;
+    count[0] += is ? n[p].x : 0, count[1] += is ? n[p].y : 0, count[2] += is ? n[p].z : 0, count[3] += is ? n[p].w : 0;
+  }
+  const RowState state = find_classes<kGatherThreads>(s, scale, 1ull << shift, ask, mass, count, ahead);
+  if (part == 0 && tid == 0) states[r] = state;
+  if (state.size > kListMost) return;
+  float lower, upper;
+  value_bounds(s, scale, least, lower, upper);
+  const int begin = part * part_len, end = min(vocab, begin + part_len);
+  Listed* list = lists + static_cast<size_t>(r) * kListMost;
+  scan_tokens<kGatherThreads, 8>(logits + static_cast<size_t>(r) * vocab, begin, end, [&](int first, const float4& four) {
+    list_group(s, scale, lower, upper, first, four, [&](uint32_t place, uint64_t key, uint64_t units, int c) { list[place] = listed_of(s, key, units, c); });
+  });
+}
 
 __global__ void __launch_bounds__(kPickThreads)
 draw_pick_kernel(const float* __restrict__ logits, int vocab, int parts, const PartStat* __restrict__ stats, const float* __restrict__ uniform,
                  const float* __restrict__ temperature, const int* __restrict__ top_k, const float* __restrict__ top_p,
                  const float* __restrict__ min_p, int shift, const RowState* __restrict__ states, const Listed* __restrict__ lists,
                  const double* __restrict__ sums, int* __restrict__ out, float* __restrict__ logprob) {
-  __shared__ PickShared s;
-  constexpr int kEach = kListMost / kPickThreads;
+  __shared__ CrossShared<kPickThreads> s;
+  __shared__ double powers[kPowers];
   const int r = blockIdx.x, tid = threadIdx.x;
-  const float* row = logits + static_cast<size_t>(r) * vocab;
-  const float t = temperature ? temperature[r] : 0.f, p_share = top_p ? top_p[r] : 1.f, floor_p = min_p ? min_p[r] : 0.f;
-  const float u = fmaxf(uniform[r], 0.f);
-  const int k = top_k ? top_k[r] : 0;
+  const Ask ask = ask_of(r, uniform, temperature, top_k, top_p, min_p);
   const Listed* list = lists + static_cast<size_t>(r) * kListMost;
   const RowState state = states[r];                               // (of a row that is not drawn: anything, not looked at)
   uint64_t best;
@@ -591,136 +758,122 @@ draw_pick_kernel(const float* __restrict__ logits, int vocab, int parts, const P
     log_sum = log(sum);
   }
   uint64_t chosen = best;
-  if (t > 0.f) {
-    const int size = static_cast<int>(min(state.size, static_cast<uint32_t>(kListMost) + 1));
-    const uint64_t one = 1ull << shift;
-    const bool cut_k = state.cut_k != 0, cut_p = p_share < 1.f, cut_m = floor_p > 0.f;
-    bring_powers<kPickThreads>(s.powers, shift);
-    if (tid == 0) s.answers[0] = state.total_hi, s.answers[1] = state.total_hi, s.answers[2] = state.kept_floor, s.answer_key = best;
-    const RowScale scale = row_scale(place_value(best), least, t, shift, s.powers);
-    const double least_weight = static_cast<double>(fminf(floor_p, 1.f)) * scale.one;
-    uint64_t total = state.total_lo, kept;
-    if (size <= kListMost) {
-      // A token's running mass and rank: up to the class before, and of its own class what stands no later.  The list's tokens go into
-      // as many buckets as they are, a class's tokens into its own by their gap, in the order; what stands in earlier buckets
-      // comes from running sums, and a token is compared with those of its bucket alone.  (Compared with all of its class, 500 tokens
-      // of one class took 90 us.)
-      uint64_t key[kEach], units[kEach] = {}, reached[kEach];
-      uint32_t rank[kEach];
-      Listed own[kEach];
-      int bucket[kEach];
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) s.bucket_mass[kEach * tid + j] = 0, s.bucket_count[kEach * tid + j] = 0;
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        const int i = tid + j * kPickThreads;
-        if (i >= size) continue;
-        own[j] = list[i];
-        key[j] = own[j].key, units[j] = own[j].units;
-        const float v = place_value(key[j]);
-        // (the gap in classes without the whole ones, of the last class's tokens possibly more than one)
-        const float x = v < scale.max ? (scale.max - v) * scale.class_scale : 0.f;
-        const float inside = fminf(fmaxf(x - fminf(floorf(x), static_cast<float>(kClasses - 1)), 0.f) * 2048.f, 2047.f);
-        bucket[j] = static_cast<int>(own[j].begin + ((static_cast<uint32_t>(inside) * (own[j].end - own[j].begin)) >> 11));
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.bucket_mass[bucket[j]]), static_cast<unsigned long long>(units[j]));
-        atomicAdd(&s.bucket_count[bucket[j]], 1u);
-      }
-      __syncthreads();
-      {
-        uint64_t mass[kEach], all = 0;
-        uint32_t count[kEach], all_n = 0;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) all += mass[j] = s.bucket_mass[kEach * tid + j], all_n += count[j] = s.bucket_count[kEach * tid + j];
-        const uint64_t own_all = all;
-        const uint32_t own_n = all_n;
-        running_sums<kPickThreads>(s.wave_mass, s.wave_count, all, all_n);
-        all -= own_all, all_n -= own_n;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-          s.bucket_mass[kEach * tid + j] = all, s.place[kEach * tid + j] = all_n;          // before the bucket
-          all += mass[j], all_n += count[j];
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        if (units[j] == 0) continue;
-        // (the mass before the bucket in its class: before the class's first bucket the list holds what is not the row's)
-        reached[j] = own[j].mass_before + s.bucket_mass[bucket[j]] - s.bucket_mass[own[j].begin];
-        rank[j] = own[j].count_before + s.place[bucket[j]] - own[j].begin;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        if (units[j] != 0) s.list[atomicAdd(&s.place[bucket[j]], 1u)] = Entry{key[j], units[j]};
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        if (units[j] == 0) continue;
-        const uint32_t end = s.place[bucket[j]];
-        for (uint32_t other = end - s.bucket_count[bucket[j]]; other < end; ++other) {
-          const Entry entry = s.list[other];
-          const bool stands = entry.key >= key[j];
-          reached[j] += stands ? entry.units : 0, rank[j] += stands ? 1 : 0;
-        }
-      }
-      auto crosses = [&](int j, uint64_t target) { return units[j] != 0 && reached[j] >= target && reached[j] - units[j] < target; };
-      if (cut_k) {
-#pragma unroll
-        for (int j = 0; j < kEach; ++j)
-          if (units[j] != 0 && rank[j] == static_cast<uint32_t>(k)) s.answers[0] = reached[j];
-        __syncthreads();
-        total = s.answers[0];
-      }
-      kept = total;
-      if (cut_p) {
-        const uint64_t target = target_of(p_share, total);
-#pragma unroll
-        for (int j = 0; j < kEach; ++j)
-          if (crosses(j, target)) s.answers[1] = reached[j];
-        __syncthreads();
-        kept = s.answers[1];
-      }
-      if (cut_m) {
-#pragma unroll
-        for (int j = 0; j < kEach; ++j)
-          if (units[j] != 0 && weight_wide(scale, place_value(key[j])) >= least_weight)
-            atomicMax(reinterpret_cast<unsigned long long*>(&s.answers[2]), static_cast<unsigned long long>(reached[j]));
-        __syncthreads();
-        kept = min(kept, s.answers[2]);
-      }
-      const uint64_t goal = goal_of(u, kept);
-#pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        if (crosses(j, goal)) s.answer_key = key[j];
-      __syncthreads();
-      chosen = s.answer_key;
-    } else {
-      uint64_t place;
-      __syncthreads();
-      if (cut_k) total = descend(s, row, vocab, scale, static_cast<uint64_t>(k), true, &place);
-      kept = total;
-      if (cut_p) kept = descend(s, row, vocab, scale, target_of(p_share, total), false, &place);
-      if (cut_m) {
-        if (tid == 0) s.answers[3] = 0;
-        __syncthreads();
-        scan_tokens<kPickThreads, 4>(row, 0, vocab, [&](int first, const float4& four) {
-          each_of(first, four, [&](int, float v) {
-            const double wide = weight_wide(scale, v);
-            if (v > -INFINITY && wide >= least_weight)
-              atomicAdd(reinterpret_cast<unsigned long long*>(&s.answers[3]), static_cast<unsigned long long>(weight_units(wide)));
-          });
-        });
-        __syncthreads();
-        kept = min(kept, max(s.answers[3], one));
-      }
-      descend(s, row, vocab, scale, goal_of(u, kept), false, &chosen);
-    }
+  if (ask.t > 0.f) {
+    bring_powers<kPickThreads>(powers, shift);
+    const RowScale scale = row_scale(place_value(best), least, ask.t, shift, powers);
+    if (state.size <= kListMost)
+      chosen = cross(s, scale, ask, state, best, [&](int i) { return list[i]; });
+    else
+      chosen = cross_without_list(s, logits + static_cast<size_t>(r) * vocab, vocab, scale, 1ull << shift, ask, state);
   }
   if (tid == 0) {
     out[r] = place_index(chosen);
     if (logprob) logprob[r] = static_cast<float>(static_cast<double>(place_value(chosen)) - static_cast<double>(place_value(best)) - log_sum);
+  }
+}
+
+struct RowShared {
+  ClassShared<kRowThreads> classes;
+  CrossShared<kRowThreads> cross;
+  double powers[kPowers];
+  uint64_t wave_best[kRowThreads / kWave];
+  float wave_least[kRowThreads / kWave];
+  double wave_sum[kRowThreads / kWave];
+};
+
+// All of the above for a row by one workgroup, in one launch: three passes over the row, of which the later ones find it in the L2.
+// (Kept in registers instead, 64 tokens a thread, every pass is code written out 64 times: 100 KB of it, brought from memory as it
+// runs, 28 us for a row of 32000 tokens.)
+__global__ void __launch_bounds__(kRowThreads)
+draw_row_kernel(const float* __restrict__ logits, int vocab, const float* __restrict__ uniform, const float* __restrict__ temperature,
+                const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p, int shift,
+                int* __restrict__ out, float* __restrict__ logprob) {
+  __shared__ RowShared s;
+  constexpr int kWaves = kRowThreads / kWave, kOwn = kClasses / kRowThreads;
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float* row = logits + static_cast<size_t>(r) * vocab;
+  const Ask ask = ask_of(r, uniform, temperature, top_k, top_p, min_p);
+  // ---- the first token, the least logit, and whether the row can be drawn from ----
+  float most = -INFINITY, least = INFINITY;
+  int at = 0;
+  bool bad = false;
+  scan_tokens<kRowThreads, 4>(row, 0, vocab, [&](int first, const float4& four) {
+    each_of(first, four, [&](int i, float v) {
+      bad = bad || !(v < INFINITY);
+      if (v > most) most = v, at = i;
+      least = v > -INFINITY ? fminf(least, v) : least;
+    });
+  });
+  uint64_t best = most > -INFINITY ? place_key(most, at) : 0;
+  if (bad) best = kBadPart;
+  for (int offset = 32; offset > 0; offset >>= 1) {
+    const uint64_t other = __shfl_xor(best, offset, 64);
+    best = other > best ? other : best;
+    least = fminf(least, __shfl_xor(least, offset, 64));
+  }
+  if (lane == 0) s.wave_best[wave] = best, s.wave_least[wave] = least;
+  bring_powers<kRowThreads>(s.powers, shift);
+  unsigned long long* mass_of = reinterpret_cast<unsigned long long*>(s.classes.running_mass);       // the histogram, until it is summed up
+  uint32_t* count_of = s.classes.running_count;
+  for (int c = tid; c < kClasses; c += kRowThreads) mass_of[c] = 0, count_of[c] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    best = s.wave_best[w] > best ? s.wave_best[w] : best;
+    least = fminf(least, s.wave_least[w]);
+  }
+  if (best == kBadPart || best == 0) {
+    if (tid == 0) {
+      out[r] = -1;
+      if (logprob) logprob[r] = __uint_as_float(0x7fc00000u);
+    }
+    return;
+  }
+  const RowScale scale = row_scale(place_value(best), least, ask.t, shift, s.powers);
+  // ---- the weights, and the sum of the log-probability's ----
+  double sum = 0.0;
+  scan_tokens<kRowThreads, 2>(row, 0, vocab, [&](int first, const float4& four) {
+    if (ask.t > 0.f) each_of(first, four, [&](int, float v) { weigh_token(scale, v, mass_of, count_of); });
+    if (logprob) sum += plain_weights(scale.max, four);
+  });
+  if (logprob) {
+    for (int offset = 32; offset > 0; offset >>= 1) sum += __shfl_xor(sum, offset, 64);
+    if (lane == 0) s.wave_sum[wave] = sum;
+  }
+  uint64_t chosen = best;
+  if (ask.t > 0.f) {
+    __syncthreads();
+    uint64_t mass[kOwn];
+    uint32_t count[kOwn], ahead[kOwn] = {};
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) mass[j] = mass_of[kOwn * tid + j], count[j] = count_of[kOwn * tid + j];
+    const RowState state = find_classes<kRowThreads>(s.classes, scale, 1ull << shift, ask, mass, count, ahead);
+    if (state.size <= kListMost) {
+      float lower, upper;
+      value_bounds(s.classes, scale, least, lower, upper);
+      scan_tokens<kRowThreads, 4>(row, 0, vocab, [&](int first, const float4& four) {
+        list_group(s.classes, scale, lower, upper, first, four,
+                   [&](uint32_t place, uint64_t key, uint64_t units, int) { s.cross.list[place] = Entry{key, units}; });
+      });
+      // (the crossings read an entry before they write the list again, with barriers in between)
+      chosen = cross(s.cross, scale, ask, state, best, [&](int i) {
+        const Entry entry = s.cross.list[i];
+        return listed_of(s.classes, entry.key, entry.units, gap_class(scale, place_value(entry.key)));
+      });
+    } else {
+      chosen = cross_without_list(s.cross, row, vocab, scale, 1ull << shift, ask, state);
+    }
+  } else {
+    __syncthreads();
+  }
+  if (tid == 0) {
+    out[r] = place_index(chosen);
+    if (logprob) {
+      double sum = 0.0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) sum += s.wave_sum[w];
+      logprob[r] = static_cast<float>(static_cast<double>(place_value(chosen)) - static_cast<double>(place_value(best)) - log(sum));
+    }
   }
 }
 
@@ -732,16 +885,23 @@ using namespace tlie;
 constexpr long long kRowBytes = sizeof(RowState) + kListMost * sizeof(Listed), kPartBytes = sizeof(PartStat) + 8 + kClasses * 12;
 static_assert(sizeof(RowState) == 32 && sizeof(Listed) == 40 && sizeof(PartStat) == 16, "the host's face counts them so");
 
-// logits: float [rows, vocab], vocab < 2^24; uniform: float [rows]; temperature, top_k, top_p, min_p: [rows] or null; parts: 1 to 16;
+// logits: float [rows, vocab], vocab < 2^24; uniform: float [rows]; temperature, top_k, top_p, min_p: [rows] or null; parts: 1 to 8, or 0: a row by
+// one workgroup (scratch is then null);
 // out: int [rows]; logprob: float [rows] or null.  scratch: rows * (kRowBytes + parts * kPartBytes) bytes, at a multiple of 16.
 extern "C" int tlie_draw(const float* logits, int rows, int vocab, const float* uniform, const float* temperature, const int* top_k,
                          const float* top_p, const float* min_p, int parts, void* scratch, int* out, float* logprob, void* stream) {
-  if (rows <= 0 || vocab <= 0 || vocab >= (1 << 24) || parts <= 0 || parts > kPartsMost || rows > 65535 || scratch == nullptr || uniform == nullptr)
+  if (rows <= 0 || vocab <= 0 || vocab >= (1 << 24) || parts < 0 || parts > kPartsMost || rows > 65535 ||
+      uniform == nullptr || (parts > 0 && scratch == nullptr))
     return kBadArgument;
   hipStream_t s = (hipStream_t)stream;
-  const int part_len = (vocab + parts - 1) / parts;
   int shift = 44;                                   // the weights' sum stays below 2^62
   while ((static_cast<long long>(vocab) << shift) >= (1ll << 62)) --shift;
+  if (parts == 0) {
+    hipLaunchKernelGGL(draw_row_kernel, dim3(rows), dim3(kRowThreads), 0, s, logits, vocab, uniform, temperature, top_k, top_p, min_p, shift, out,
+                       logprob);
+    return launch_status();
+  }
+  const int part_len = (vocab + parts - 1) / parts;
   const size_t places = static_cast<size_t>(rows) * parts;
   Listed* lists = static_cast<Listed*>(scratch);
   RowState* states = reinterpret_cast<RowState*>(lists + static_cast<size_t>(rows) * kListMost);

@@ -2102,9 +2102,14 @@ DRAW_ROW_BYTES, DRAW_PART_BYTES = 32 + 2048 * 40, 24 + 1024 * 12      # of scrat
 
 
 def draw_parts(rows: int, vocab: int) -> int:
-    """Into how many parts `sample_filtered` cuts each row, at most 8: each brings a histogram to write and, by all of them, to read.  Up to
-    16 rows parts of 4096 tokens fill the chip, beyond of 8192, with a thousand workgroups at most (1 row of 32000 tokens in 8 parts 21 us,
-    in 4 22, in 16 23; 64 rows of 32000 in 4 parts 34, in 2 and 8 40; 64 rows of 128256 in 8 parts 54, in 4 62; 256 rows in 4 parts 112, in 8 128)."""
+    """Into how many parts `sample_filtered` cuts each row; 0: a row by one workgroup, in one launch instead of four.
+
+    One workgroup a row where the rows fill the chip or are short (1 row of 16000 tokens 19.2 us, in parts 20.6, of 32000 24.7 and 20.8; 64 of
+    32000 32.8 and 34.2, of 128256 85 and 53; 256 of 128256 94 and 112).  Else at most 8 parts, each brings a histogram to write and, by all
+    of them, to read: of 4096 tokens up to 16 rows, of 8192 beyond, a thousand workgroups at most (7 rows of 50261 in 8 parts 25 us, in 4 28;
+    64 rows of 128256 in 8 parts 53, in 4 61; 256 rows in 4 parts 112, in 8 128)."""
+    if vocab <= 512 * (rows + 40):
+        return 0
     return max(1, min(8, 1024 // max(rows, 1), -(-vocab // (4096 if rows <= 16 else 8192))))
 
 
@@ -2147,7 +2152,7 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: to
         out_logprobs = torch.empty((rows,), dtype=torch.float32, device=logits.device)
     if rows > 0:
         parts = draw_parts(rows, vocab)
-        scratch = torch.empty((rows * (DRAW_ROW_BYTES + parts * DRAW_PART_BYTES),), dtype=torch.uint8, device=logits.device)
+        scratch = torch.empty((rows * (DRAW_ROW_BYTES + parts * DRAW_PART_BYTES),), dtype=torch.uint8, device=logits.device) if parts else None
         _check(library().tlie_draw(_ptr(logits), rows, vocab, _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), parts,
                                    _ptr(scratch), _ptr(out), _ptr(out_logprobs), _stream()), "sample_filtered")
     return (out, out_logprobs) if logprobs else out
