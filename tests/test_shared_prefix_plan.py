@@ -28,16 +28,17 @@ def drawn_step(rng):
     return np.concatenate([[0], np.cumsum(counts)]).astype(np.int64), np.array(lengths, dtype=np.int64), groups, prefix
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(32, 4, 64), (32, 8, 128), (8, 8, 256), (40, 1, 64), (12, 4, 48)])
-def test_every_key_of_every_column_is_in_one_item(heads, kv_heads, dim):
+def test_every_key_of_every_column_is_in_one_item(heads, kv_heads, dim, dtype):
     rng, group = random.Random(heads), heads // kv_heads
     for _ in range(40):
         start, lengths, groups, prefix = drawn_step(rng)
-        items, part_first, wide = ops.shared_prefix_items(start, lengths, groups, heads, kv_heads, dim)
+        items, part_first = ops.shared_prefix_items(start, lengths, groups, heads, kv_heads, dim, dtype)
         covered, written = {}, set()
         for sequence, tok0, tokens, col0, low, high, own, part in items.tolist():
             assert low < high
-            for column in range(col0, min(col0 + (16 * wide if tokens * group - col0 > 16 else 16), tokens * group)):
+            for column in range(col0, min(col0 + ops.prefix_tile_columns(tokens * group - col0, dim, dtype), tokens * group)):
                 token, head = tok0 + column // group, column % group
                 seq = int(np.searchsorted(start, token, side="right") - 1)
                 position = lengths[seq] - start[seq + 1] + token
@@ -86,7 +87,7 @@ def test_arguments_on_the_host_are_refused():
     logits, number = torch.zeros(2, 8), torch.zeros(2)
     with pytest.raises(EngineError):
         ops.sample_filtered(logits, number)
-    plan = ops.SharedPrefixPlan(torch.zeros(1, 8, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 1, 1, 1, 1, 1, (2, 1, 16, torch.float32))
+    plan = ops.SharedPrefixPlan(torch.zeros(1, 8, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 1, 1, 1, 1, (2, 1, 16, torch.float32))
     with pytest.raises(EngineError):
         ops.attention_shared_prefix(torch.zeros(1, 32), torch.zeros(1, 2, 1, 256), torch.zeros(1, 1, dtype=torch.int32),
                                     torch.zeros(1, dtype=torch.int32), plan, 2, 1, 16, 1.0)

@@ -31,6 +31,27 @@ struct PrefixItem {
 };
 
 constexpr int kPrefixWaves = 4;
+// Powers may grow to 2^6 before what they are relative to moves: sums and values are float, and the rounding of a probability to
+// bfloat16 is relative.  Without slack a wave of 32 columns rescales in almost every block of an item (30000 keys, 128 columns on 8 key
+// heads: 70 us against 66).
+constexpr float kSlack = 6.f;
+
+// 128 neighbouring entries of a sequence's block table, two a lane: a block's page numbers come from registers, so that its keys and
+// values are asked for without waiting for a page number from memory first (3 us a block in the middle of a walk).
+struct TableWindow {
+  int first, low, high;
+  __device__ __forceinline__ void load(const int* __restrict__ pages, int max_blocks, int from) {
+    const int lane = threadIdx.x & 63;
+    first = from;
+    low = pages[min(from + lane, max_blocks - 1)];
+    high = pages[min(from + 64 + lane, max_blocks - 1)];
+  }
+  __device__ __forceinline__ int page(int index) const {          // index: the same for every lane, within the window
+    const int place = __builtin_amdgcn_readfirstlane(index - first);
+    const int a = __builtin_amdgcn_readlane(low, place & 63), b = __builtin_amdgcn_readlane(high, place & 63);
+    return place < 64 ? a : b;
+  }
+};
 
 template <int DT, bool FLOAT, int CT>
 __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, const void* __restrict__ q_any, const void* __restrict__ cache_any,
@@ -82,11 +103,12 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
     Values v[DT][TILES];
   };
   // Rows outside the item's keys are read with the others (their page is in the table, or page 0 stands there) and masked.
+  TableWindow window;
   auto load = [&](int kb, Block& block) {
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
       const int first = kb + t * 16;
-      const int page = __builtin_amdgcn_readfirstlane(pages[min(first >> page_shift, max_blocks - 1)]);
+      const int page = window.page(first >> page_shift);
       const Elem* keys = k_base + (static_cast<size_t>(page) * page_stride + (first & page_mask)) * D;
       const Elem* values = v_base + static_cast<size_t>(page) * page_stride * D + (first & page_mask);
 #pragma unroll
@@ -107,9 +129,9 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
     for (int dt = 0; dt < DT; ++dt) o[ct][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto work = [&](int kb, Block& block, auto masked_tag) {
-    constexpr bool kMasked = decltype(masked_tag)::value;
-    if (kMasked) {
+  auto work = [&](int kb, Block& block) {
+    const bool ragged = kb < open_lo || kb + BLOCK > open_hi;     // (the same for the whole wave)
+    if (ragged) {
       // rows that are not the item's may hold anything: 0 * NaN must not arise
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -154,6 +176,18 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
             s[ct][t][j] = 1.f - (FLOAT ? 2.f / grown : 2.f * __builtin_amdgcn_rcpf(grown));
           }
     }
+    if (ragged) {
+      settle(s);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = kb + t * 16 + grp * 4 + j;
+            s[ct][t][j] = key >= item.key_lo && key < item.key_hi && key <= last_key[ct] ? s[ct][t][j] : -INFINITY;
+          }
+    }
     float lane_top[CT];
     bool exceeds = false;
 #pragma unroll
@@ -162,18 +196,12 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (kMasked) {
-            const int key = kb + t * 16 + grp * 4 + j;
-            s[ct][t][j] = key >= item.key_lo && key < item.key_hi && key <= last_key[ct] ? s[ct][t][j] : -INFINITY;
-          }
-          lane_top[ct] = fmaxf(lane_top[ct], s[ct][t][j]);
-        }
+        for (int j = 0; j < 4; ++j) lane_top[ct] = fmaxf(lane_top[ct], s[ct][t][j]);
       lane_top[ct] *= scale_log2;                           // (the scale is positive)
-      exceeds = exceeds || lane_top[ct] > top[ct];
+      exceeds = exceeds || lane_top[ct] > top[ct] + kSlack;
     }
-    // A column's maximum is shared by its four lane groups and moves only when a block holds a larger score, which is rare
-    // after the first blocks: rescaling sits behind a branch of the wave.
+    // What the scores are taken relative to (shared by a column's four lane groups) is a maximum of earlier blocks, and moves only when
+    // a block exceeds it by more than the slack: rare after the first block, so rescaling sits behind a branch of the wave.
     if (__builtin_amdgcn_ballot_w64(exceeds) != 0) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
@@ -193,7 +221,7 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
     float p[CT][TILES * 4];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const float below = kMasked && top[ct] == -INFINITY ? 0.f : top[ct];         // (nothing seen yet: 2^(-inf - 0) = 0)
+      const float below = top[ct] == -INFINITY ? 0.f : top[ct];         // (nothing seen yet: 2^(-inf - 0) = 0)
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
@@ -230,20 +258,21 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
   // two blocks in registers: while one is worked on the other is on its way
   constexpr int kStride = BLOCK * kPrefixWaves;
   Block ring[2];
-  const int begin = (item.key_lo & ~(BLOCK - 1)) + BLOCK * wave;
-  if (begin < item.key_hi) {
-    load(begin, ring[0]);
-    if (begin + kStride < item.key_hi) load(begin + kStride, ring[1]);
-    for (int kb = begin; kb < item.key_hi; kb += 2 * kStride) {
+  for (int begin = item.key_lo & ~31; begin < item.key_hi;) {
+    window.load(pages, max_blocks, begin >> page_shift);
+    const int end = min(item.key_hi, (window.first + 128) << page_shift);        // (a multiple of 32, or the item's)
+    const int mine_first = begin + BLOCK * wave, last = (end - 1) & ~(BLOCK - 1);
+    load(min(mine_first, last), ring[0]);
+    load(min(mine_first + kStride, last), ring[1]);
+    for (int kb = mine_first; kb < end; kb += 2 * kStride) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int mine = kb + r * kStride;
-        if (mine >= item.key_hi) break;
-        if (mine >= open_lo && mine + BLOCK <= open_hi) work(mine, ring[r], std::false_type{});
-        else work(mine, ring[r], std::true_type{});
-        if (mine + 2 * kStride < item.key_hi) load(mine + 2 * kStride, ring[r]);
+        if (mine < end) work(mine, ring[r]);
+        load(min(mine + 2 * kStride, last), ring[r]);              // (past the last block the last again: as many loads on every path)
       }
     }
+    begin = end;
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -296,12 +325,248 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
   }
 }
 
-template <int DT, bool FLOAT, int CT>
-__global__ void __launch_bounds__(64 * kPrefixWaves)
+// An item of many columns, bfloat16: each wave has 16 * CT columns of its own, and every block of 32 keys and values is brought once
+// for all four, through LDS.  Blocks are asked for two ahead of their turn and wait in registers; two buffers in turn, so that one
+// barrier a block is enough (a wave writes a buffer again only behind the barrier that every wave reaches after it has read it).
+// Keys lie as [key][piece of 16 bytes], a key's pieces rotated by key / kPeriod so that the 16 keys that a read takes the same piece of
+// are spread over the banks; values as [half of 16 keys][dim][16 keys], of which a read takes 512 bytes in a row.
+template <int DT, int CT>
+__device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh, const uint16_t* __restrict__ q, const uint16_t* __restrict__ cache,
+                                                 const int* __restrict__ pages, int max_blocks, const int* __restrict__ positions,
+                                                 const int* __restrict__ part_first, float* __restrict__ part_o, float* __restrict__ part_ml,
+                                                 int nq, int nkv, int page_shift, float scale_log2, float cap_pre, unsigned char* lds) {
+  constexpr int D = DT * 16, KS = (DT + 1) / 2, kPieces = 2 * DT;           // pieces of a key
+  constexpr int kPeriod = 16 / (kPieces % 16 == 0 ? 16 : kPieces % 8 == 0 ? 8 : kPieces % 4 == 0 ? 4 : 2);
+  constexpr int kBytes = 64 * D;                                            // of a block's keys, and of its values
+  constexpr int kCalls = (2 * DT + 3) / 4;                                  // pieces a thread brings of a block: 2 * DT times 64 in all
+  typedef uint32_t Piece __attribute__((ext_vector_type(4)));
+  typedef uint32_t Half __attribute__((ext_vector_type(2)));
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int G = nq / nkv, ncols = item.ntok * G, page_mask = (1 << page_shift) - 1;
+  const int pos0 = item.own ? __builtin_amdgcn_readfirstlane(positions[item.tok0]) : 0;
+  const int col0 = item.col0 + wave * 16 * CT;
+  const bool active = col0 < ncols;
+  auto has_dims = [&](int ks) { return DT % 2 == 0 || ks < KS - 1 || grp < 2; };
+
+  int tok[CT], head[CT], last_key[CT];
+  bool valid[CT];
+  Piece query[CT][KS];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = col0 + ct * 16 + col;
+    valid[ct] = c < ncols;
+    tok[ct] = item.tok0 + (valid[ct] ? c / G : 0);
+    head[ct] = kvh * G + (valid[ct] ? c % G : 0);
+    last_key[ct] = !valid[ct] ? -1 : item.own ? pos0 + c / G : 0x7fffffff;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      query[ct][ks] = Piece{0, 0, 0, 0};
+      if (valid[ct] && has_dims(ks))
+        query[ct][ks] = *reinterpret_cast<const Piece*>(q + (static_cast<size_t>(tok[ct]) * nq + head[ct]) * D + (ks * 4 + grp) * 8);
+    }
+  }
+  // the wave's keys end with those of its last column; keys that all its columns see need no mask
+  const int last_col = min(col0 + 16 * CT, ncols) - 1;
+  const int high = !active ? 0 : item.own ? min(item.key_hi, pos0 + last_col / G + 1) : item.key_hi;
+  const int open_hi = item.own ? min(item.key_hi, pos0 + col0 / G + 1) : item.key_hi;
+
+  const size_t page_stride = static_cast<size_t>(2 * nkv) << page_shift;    // in rows of D
+  const uint16_t* k_base = cache + (static_cast<size_t>(kvh) << page_shift) * D;
+  const uint16_t* v_base = cache + (static_cast<size_t>(nkv + kvh) << page_shift) * D;
+  int from[kCalls];                                                          // a piece's place behind its half's page and row
+  int to[kCalls];                                                            // and in the buffer, in bytes
+  bool second[kCalls], of_values[kCalls];
+#pragma unroll
+  for (int i = 0; i < kCalls; ++i) {
+    const int call = min(wave + 4 * i, 2 * DT - 1), piece = (call % DT) * 64 + lane;     // (past the last: the last again, the same bytes)
+    of_values[i] = call >= DT;
+    if (!of_values[i]) {
+      const int key = piece / kPieces, place = piece % kPieces;
+      second[i] = key >= 16;
+      from[i] = (key & 15) * D + place * 8;
+      to[i] = (key * kPieces + (place + key / kPeriod) % kPieces) * 16;
+    } else {
+      const int rest = piece % (2 * D);
+      second[i] = piece >= 2 * D;
+      from[i] = ((rest >> 1) << page_shift) + (rest & 1) * 8;
+      to[i] = kBytes + piece * 16;
+    }
+  }
+  Piece staged[2][kCalls];
+  TableWindow window;
+  auto bring = [&](int kb, Piece (&into)[kCalls]) {
+    const size_t at_a = static_cast<size_t>(window.page(kb >> page_shift)) * page_stride * D;
+    const size_t at_b = static_cast<size_t>(window.page((kb + 16) >> page_shift)) * page_stride * D;
+    const int row_a = kb & page_mask, row_b = (kb + 16) & page_mask;
+#pragma unroll
+    for (int i = 0; i < kCalls; ++i) {
+      const uint16_t* a = of_values[i] ? v_base + at_a + row_a : k_base + at_a + row_a * D;
+      const uint16_t* b = of_values[i] ? v_base + at_b + row_b : k_base + at_b + row_b * D;
+      into[i] = *reinterpret_cast<const Piece*>((second[i] ? b : a) + from[i]);
+    }
+  };
+
+  float top[CT], sum[CT];
+  floatx4 o[CT][DT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    top[ct] = -INFINITY, sum[ct] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[ct][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int key_place = col * kPieces * 16;                                  // the lane's key in its half, and how far its pieces are rotated
+  const int turned_a = col / kPeriod, turned_b = (col + 16) / kPeriod;
+
+  // (one copy of the code, its masks behind branches of the wave: with a copy with and one without masks the compiler keeps 42 registers
+  // in memory, and waits for the blocks on their way each time it fetches one: 67 us against 37 for the kernel)
+  auto work = [&](int kb, const unsigned char* buffer) {
+    const bool ragged = kb < item.key_lo || kb + 32 > open_hi;
+    floatx4 s[CT][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) s[ct][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int place = (min(ks * 4 + grp, kPieces - 1) + (t ? turned_b : turned_a)) % kPieces;
+        Piece k = *reinterpret_cast<const Piece*>(buffer + key_place + t * 16 * kPieces * 16 + place * 16);
+        if (!has_dims(ks)) k = Piece{0, 0, 0, 0};
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&k), *reinterpret_cast<const bf16x8*>(&query[ct][ks]),
+                                                             s[ct][t], 0, 0, 0);
+      }
+    }
+    if (cap_pre > 0.f) {
+      settle(s);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s[ct][t][j] = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[ct][t][j] * (cap_pre * 2.8853900817779268f)) + 1.f);
+    }
+    if (ragged) {
+      settle(s);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = kb + t * 16 + grp * 4 + j;
+            s[ct][t][j] = key >= item.key_lo && key < item.key_hi && key <= last_key[ct] ? s[ct][t][j] : -INFINITY;
+          }
+    }
+    float lane_top[CT];
+    bool exceeds = false;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      lane_top[ct] = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lane_top[ct] = fmaxf(lane_top[ct], s[ct][t][j]);
+      lane_top[ct] *= scale_log2;
+      exceeds = exceeds || lane_top[ct] > top[ct] + kSlack;
+    }
+    if (__builtin_amdgcn_ballot_w64(exceeds) != 0) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        float most = lane_top[ct];
+        most = fmaxf(most, __shfl_xor(most, 16, 64));
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        most = fmaxf(most, top[ct]);
+        const float down = most == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[ct] - most);
+        top[ct] = most;
+        sum[ct] *= down;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[ct][dt][j] *= down;
+      }
+    }
+    Piece packed[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const float below = top[ct] == -INFINITY ? 0.f : top[ct];
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[ct][i >> 2][i & 3], scale_log2, -below));
+      sum[ct] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) packed[ct][i] = pack_bf16(p[2 * i], p[2 * i + 1]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      Half a = *reinterpret_cast<const Half*>(buffer + kBytes + (dt * 16 + col) * 32 + grp * 8);
+      Half b = *reinterpret_cast<const Half*>(buffer + kBytes + D * 32 + (dt * 16 + col) * 32 + grp * 8);
+      if (ragged) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = kb + grp * 4 + j;
+          const uint32_t mask = (j & 1) ? 0x0000ffffu : 0xffff0000u;
+          if (key < item.key_lo || key >= item.key_hi) a[j >> 1] &= mask;
+          if (key + 16 < item.key_lo || key + 16 >= item.key_hi) b[j >> 1] &= mask;
+        }
+      }
+      const Piece v = Piece{a[0], a[1], b[0], b[1]};
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&v), *reinterpret_cast<const bf16x8*>(&packed[ct]),
+                                                            o[ct][dt], 0, 0, 0);
+    }
+  };
+  auto turn = [&](int kb, int last, int buffer, Piece (&waiting)[kCalls]) {
+    unsigned char* place = lds + buffer * 2 * kBytes;
+#pragma unroll
+    for (int i = 0; i < kCalls; ++i) *reinterpret_cast<Piece*>(place + to[i]) = waiting[i];
+    lds_barrier();
+    bring(min(kb + 64, last), waiting);                        // (past the last block the last again: as many loads on every path)
+    if (kb <= last && kb < high) work(kb, place);
+  };
+  for (int begin = item.key_lo & ~31; begin < item.key_hi;) {
+    window.load(pages, max_blocks, begin >> page_shift);
+    const int end = min(item.key_hi, (window.first + 128) << page_shift), last = (end - 1) & ~31;
+    bring(begin, staged[0]);
+    bring(min(begin + 32, last), staged[1]);
+    for (int kb = begin; kb <= last; kb += 64) {
+      turn(kb, last, 0, staged[0]);
+      turn(kb + 32, last, 1, staged[1]);
+    }
+    lds_barrier();                                             // (the next window's first block reuses the first buffer)
+    begin = end;
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    sum[ct] += __shfl_xor(sum[ct], 16, 64);
+    sum[ct] += __shfl_xor(sum[ct], 32, 64);
+  }
+  settle(o);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int first_part = part_first[tok[ct]];
+    if (!valid[ct] || item.part >= part_first[tok[ct] + 1] - first_part) continue;
+    const size_t slot = static_cast<size_t>(first_part + item.part) * nq + head[ct];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      *reinterpret_cast<float4*>(part_o + slot * D + dt * 16 + grp * 4) = make_float4(o[ct][dt][0], o[ct][dt][1], o[ct][dt][2], o[ct][dt][3]);
+    if (grp == 0) part_ml[slot * 2] = top[ct], part_ml[slot * 2 + 1] = sum[ct];
+  }
+}
+
+// Columns that a tile has: 16 where there are no more (four waves share its keys); else 64, or 128 in bfloat16 for head sizes up to
+// 128 where there are more than 64 (each wave has columns of its own).  Float items have up to 32, always by the first form.
+template <int DT, bool FLOAT>
+__global__ void __launch_bounds__(64 * kPrefixWaves, DT <= 8 && !FLOAT ? 2 : 1)
 prefix_items_kernel(const void* __restrict__ q, const void* __restrict__ cache, const int* __restrict__ block_table, int max_blocks,
                     const int* __restrict__ items, const int* __restrict__ positions, const int* __restrict__ part_first, float* __restrict__ part_o,
                     float* __restrict__ part_ml, int nq, int nkv, int page_shift, float scale_log2, float cap_pre) {
-  __shared__ __attribute__((aligned(16))) float lds[kPrefixWaves * (CT * 32 + DT * 256)];
+  constexpr int kFloatWide = DT <= 8 ? 2 : 1;
+  constexpr int kNarrow = kPrefixWaves * ((FLOAT ? kFloatWide : 1) * 32 + DT * 256) * 4, kWideBytes = FLOAT ? 0 : 4 * 64 * DT * 16;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kNarrow > kWideBytes ? kNarrow : kWideBytes];
   const int kvh = blockIdx.x % nkv;
   PrefixItem item;
   {
@@ -313,55 +578,88 @@ prefix_items_kernel(const void* __restrict__ q, const void* __restrict__ cache, 
   }
   if (item.ntok <= 0) return;                                  // a list of fixed size ends in items without tokens
   const int* pages = block_table + static_cast<size_t>(item.table) * max_blocks;
-  // an item of few columns is served by the form for 16 whatever the launch's width
-  if (CT > 1 && item.ntok * (nq / nkv) - item.col0 > 16)
-    prefix_item<DT, FLOAT, CT>(item, kvh, q, cache, pages, max_blocks, positions, part_first, part_o, part_ml, nq, nkv, page_shift, scale_log2, cap_pre, lds);
-  else
-    prefix_item<DT, FLOAT, 1>(item, kvh, q, cache, pages, max_blocks, positions, part_first, part_o, part_ml, nq, nkv, page_shift, scale_log2, cap_pre, lds);
+  const int columns = item.ntok * (nq / nkv) - item.col0;      // (of the tile and those behind it)
+#define TLIE_ARGS max_blocks, positions, part_first, part_o, part_ml, nq, nkv, page_shift, scale_log2, cap_pre
+  if constexpr (FLOAT) {
+    if (kFloatWide > 1 && columns > 16)
+      prefix_item<DT, true, kFloatWide>(item, kvh, q, cache, pages, TLIE_ARGS, reinterpret_cast<float*>(lds));
+    else
+      prefix_item<DT, true, 1>(item, kvh, q, cache, pages, TLIE_ARGS, reinterpret_cast<float*>(lds));
+  } else {
+    const uint16_t* q16 = static_cast<const uint16_t*>(q);
+    const uint16_t* cache16 = static_cast<const uint16_t*>(cache);
+    if (columns <= 16)
+      prefix_item<DT, false, 1>(item, kvh, q, cache, pages, TLIE_ARGS, reinterpret_cast<float*>(lds));
+    else if (DT > 8 || columns <= 64)
+      prefix_wide_item<DT, 1>(item, kvh, q16, cache16, pages, TLIE_ARGS, lds);
+    else
+      prefix_wide_item<DT, (DT <= 8 ? 2 : 1)>(item, kvh, q16, cache16, pages, TLIE_ARGS, lds);
+  }
+#undef TLIE_ARGS
 }
 
-// out[t][h] = sum_i w_i o_i / (sum_i w_i l_i + w_sink) over the token's parts, in their order.  A wave a (token, head).
+// out[t][h] = sum_i w_i o_i / (sum_i w_i l_i + w_sink) over the token's parts.  A wave a (token, head): the lanes have a part's weight
+// each first, then a sixteenth byte of it: d / 4 lanes take a part, the others the next ones.  Four loads a lane are on their way at a
+// time, and the order of the additions is fixed by the number of parts.
 template <bool FLOAT>
 __global__ void __launch_bounds__(256)
 prefix_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ part_first,
                    const float* __restrict__ sink, void* __restrict__ out, int rows, int nq, int d) {
-  const int row = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  __shared__ float weights[4][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int row = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + wave));
   if (row >= rows) return;
-  const int lane = threadIdx.x & 63, token = row / nq, head = row - token * nq;
-  const int first = part_first[token], count = part_first[token + 1] - first;
+  const int token = row / nq, head = row - token * nq;
+  const int first = __builtin_amdgcn_readfirstlane(part_first[token]), count = __builtin_amdgcn_readfirstlane(part_first[token + 1]) - first;
   const float own = sink != nullptr ? sink[head] * 1.4426950408889634f : -INFINITY;
-  float most = own;
-  for (int p = 0; p < count; ++p) most = fmaxf(most, part_ml[(static_cast<size_t>(first + p) * nq + head) * 2]);
-  const float below = most == -INFINITY ? 0.f : most;
-  float total = sink != nullptr ? __builtin_amdgcn_exp2f(own - below) : 0.f;
-  for (int p = 0; p < count; ++p) {
-    const size_t slot = static_cast<size_t>(first + p) * nq + head;
-    total += __builtin_amdgcn_exp2f(part_ml[slot * 2] - below) * part_ml[slot * 2 + 1];
-  }
-  const float inv = total > 0.f ? 1.f / total : 0.f;           // a token that no sequence brings has no parts, and gets zeros
-  for (int i = lane; i < d; i += 64) {
-    float value = 0.f;
-    for (int p = 0; p < count; ++p) {
-      const size_t slot = static_cast<size_t>(first + p) * nq + head;
-      value += __builtin_amdgcn_exp2f(part_ml[slot * 2] - below) * part_o[slot * d + i];
+  const int per = d >> 2, together = 64 / per, mine = lane / per, at = lane - mine * per;     // lanes a part, parts at a time
+  const float* base = part_o + (static_cast<size_t>(first) * nq + head) * d + at * 4;
+  const float* ml = part_ml + (static_cast<size_t>(first) * nq + head) * 2;
+  float most = own, total = sink != nullptr ? 1.f : 0.f;        // (in units of 2^most)
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < count; p0 += 64) {                      // 64 parts at a time
+    const int here = min(64, count - p0);
+    const float2 stat = lane < here ? *reinterpret_cast<const float2*>(ml + static_cast<size_t>(p0 + lane) * nq * 2) : make_float2(-INFINITY, 0.f);
+    const float next = fmaxf(most, wave_max(stat.x)), below = next == -INFINITY ? 0.f : next;
+    const float down = __builtin_amdgcn_exp2f(most - below), weight = __builtin_amdgcn_exp2f(stat.x - below);
+    total = total * down + wave_sum(weight * stat.y);
+    sum.x *= down, sum.y *= down, sum.z *= down, sum.w *= down;
+    most = next;
+    weights[wave][lane] = weight;
+    __builtin_amdgcn_wave_barrier();
+    if (mine < together) {
+      constexpr int kAhead = 4;
+      for (int p = mine; p < here; p += kAhead * together) {
+        float4 part[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) part[u] = *reinterpret_cast<const float4*>(base + static_cast<size_t>(p0 + min(p + u * together, here - 1)) * nq * d);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const float w = p + u * together < here ? weights[wave][min(p + u * together, here - 1)] : 0.f;
+          sum.x += w * part[u].x, sum.y += w * part[u].y, sum.z += w * part[u].z, sum.w += w * part[u].w;
+        }
+      }
     }
-    if (FLOAT) static_cast<float*>(out)[static_cast<size_t>(row) * d + i] = value * inv;
-    else static_cast<uint16_t*>(out)[static_cast<size_t>(row) * d + i] = __bfloat16_as_ushort(__float2bfloat16(value * inv));
+    __builtin_amdgcn_wave_barrier();
   }
+  float4 all = sum;
+  for (int other = 1; other < together; ++other) {              // (all lanes shuffle; the first part's lanes keep the sum)
+    const int from = (at + other * per) & 63;
+    all.x += __shfl(sum.x, from, 64), all.y += __shfl(sum.y, from, 64), all.z += __shfl(sum.z, from, 64), all.w += __shfl(sum.w, from, 64);
+  }
+  if (mine != 0) return;
+  const float inv = total > 0.f ? 1.f / total : 0.f;            // a token that no sequence brings has no parts, and gets zeros
+  all.x *= inv, all.y *= inv, all.z *= inv, all.w *= inv;
+  if (FLOAT) *reinterpret_cast<float4*>(static_cast<float*>(out) + static_cast<size_t>(row) * d + at * 4) = all;
+  else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + static_cast<size_t>(row) * d + at * 4) = make_uint2(pack_bf16(all.x, all.y), pack_bf16(all.z, all.w));
 }
 
 template <bool FLOAT, int DT>
-static int launch_items(int wide, const void* q, const void* cache, const int* block_table, int max_blocks, const int* items, int num_items,
+static int launch_items(const void* q, const void* cache, const int* block_table, int max_blocks, const int* items, int num_items,
                         const int* positions, const int* part_first, float* part_o, float* part_ml, int nq, int nkv, int page_shift,
                         float scale_log2, float cap_pre, hipStream_t stream) {
-  constexpr int kWide = DT <= 8 ? 2 : 1;
-  if (wide != 1 && wide != kWide) return kBadArgument;
-  if (wide == 1)
-    hipLaunchKernelGGL((prefix_items_kernel<DT, FLOAT, 1>), dim3(num_items * nkv), dim3(64 * kPrefixWaves), 0, stream, q, cache, block_table,
-                       max_blocks, items, positions, part_first, part_o, part_ml, nq, nkv, page_shift, scale_log2, cap_pre);
-  else
-    hipLaunchKernelGGL((prefix_items_kernel<DT, FLOAT, kWide>), dim3(num_items * nkv), dim3(64 * kPrefixWaves), 0, stream, q, cache, block_table,
-                       max_blocks, items, positions, part_first, part_o, part_ml, nq, nkv, page_shift, scale_log2, cap_pre);
+  hipLaunchKernelGGL((prefix_items_kernel<DT, FLOAT>), dim3(num_items * nkv), dim3(64 * kPrefixWaves), 0, stream, q, cache, block_table, max_blocks,
+                     items, positions, part_first, part_o, part_ml, nq, nkv, page_shift, scale_log2, cap_pre);
   return launch_status();
 }
 
@@ -370,11 +668,11 @@ static int launch_items(int wide, const void* q, const void* cache, const int* b
 using namespace tlie;
 
 // q, out: [tokens, nq, d]; cache: [pages, 2, nkv, page_size * d] (keys [row][dim], values [dim][row]); both of `dtype`.
-// items: int32 [num_items, 8] (see PrefixItem), in columns of 16 * wide; part_first: int32 [tokens + 1], the first part of
+// items: int32 [num_items, 8] (see PrefixItem; tiles of columns as prefix_items_kernel has them); part_first: int32 [tokens + 1], the first part of
 // each token, so that part_first[tokens] is their number; part_o: float [parts, nq, d], part_ml: float [parts, nq, 2].
 // sink: float [nq] or null.  softcap: 0, or the cap of the scaled scores.
 extern "C" int tlie_attention_prefix(const void* q, const void* cache, int dtype, const int* block_table, int max_blocks, const int* items,
-                                     int num_items, int wide, const int* positions, const int* part_first, float* part_o, float* part_ml,
+                                     int num_items, const int* positions, const int* part_first, float* part_o, float* part_ml,
                                      const float* sink, void* out, int tokens, int nq, int nkv, int d, int page_size, float scale,
                                      float softcap, void* stream) {
   if (tokens <= 0 || num_items <= 0 || nq <= 0 || nkv <= 0 || nq % nkv != 0 || d <= 0 || d > 256 || d % 16 != 0 || page_size < 16 ||
@@ -387,9 +685,9 @@ extern "C" int tlie_attention_prefix(const void* q, const void* cache, int dtype
   int status = kBadArgument;
 #define TLIE_CASE(DT)                                                                                                                              \
   case DT:                                                                                                                                         \
-    status = dtype == kF32 ? launch_items<true, DT>(wide, q, cache, block_table, max_blocks, items, num_items, positions, part_first, part_o,      \
+    status = dtype == kF32 ? launch_items<true, DT>(q, cache, block_table, max_blocks, items, num_items, positions, part_first, part_o,      \
                                                     part_ml, nq, nkv, page_shift, scale_log2, cap_pre, s)                                          \
-                           : launch_items<false, DT>(wide, q, cache, block_table, max_blocks, items, num_items, positions, part_first, part_o,     \
+                           : launch_items<false, DT>(q, cache, block_table, max_blocks, items, num_items, positions, part_first, part_o,     \
                                                      part_ml, nq, nkv, page_shift, scale_log2, cap_pre, s);                                        \
     break;
   switch (d / 16) {

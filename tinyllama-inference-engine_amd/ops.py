@@ -2738,21 +2738,26 @@ class SharedPrefixPlan:
     part_first: torch.Tensor       # int32 [tokens + 1]: the first part of each token
     tokens: int
     parts: int
-    wide: int                      # column groups of 16 that a tile has
     sequences: int
     longest: int
     sizes: tuple                   # (num_heads, num_kv_heads, head_dim, dtype)
 
 
-PREFIX_ALIGN = 128         # keys that the four waves of a workgroup take in one turn (bfloat16)
+def prefix_tile_columns(columns: int, head_dim: int, dtype: torch.dtype) -> int:
+    """How many columns (token, query head of a kv head) the tile takes that has so many of its item before it, itself included."""
+    if columns <= 16:
+        return 16
+    if dtype == torch.float32:
+        return 32 if head_dim <= 128 else 16
+    return 128 if columns > 64 and head_dim <= 128 else 64
 
 
-def prefix_wide(head_dim: int) -> int:
-    return 2 if head_dim <= 128 else 1
+PREFIX_COST = {16: 1.0, 32: 1.0, 64: 3.0, 128: 5.0}    # of a key, by the tile's columns
+PREFIX_LEAST = {16: 128, 32: 128, 64: 256, 128: 256}   # keys that a part has at least
 
 
-def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, compute_units: int = 256):
-    """The host's half of `shared_prefix_plan`: (items [n, 8], part_first [tokens + 1], wide), int32 arrays of numpy."""
+def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, compute_units: int = 256):
+    """The host's half of `shared_prefix_plan`: (items [n, 8], part_first [tokens + 1]), int32 arrays of numpy."""
     import numpy as np
     seq_start, seq_len = np.asarray(seq_start, dtype=np.int64), np.asarray(seq_len, dtype=np.int64)
     if seq_start.ndim != 1 or seq_len.ndim != 1 or seq_start.shape[0] != seq_len.shape[0] + 1:
@@ -2775,56 +2780,67 @@ def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads
         if prefix > 0 and seq_start[first + count] > seq_start[first]:
             shared.append((first, count, prefix))
             prefix_of[members] = prefix
-    wide = prefix_wide(head_dim)
 
     def tiles(tokens: int):
+        """First columns and widths of an item's tiles: of one width but the last, which has what is left."""
         columns = tokens * group
-        return np.arange(0, columns, 16 if columns <= 16 else 16 * wide, dtype=np.int64), (16 if columns <= 16 else 16 * wide)
+        step = prefix_tile_columns(columns, head_dim, dtype)
+        col0 = np.arange(0, columns, step, dtype=np.int64)
+        width = np.full(col0.shape[0], step, dtype=np.int64)
+        width[-1] = prefix_tile_columns(columns - int(col0[-1]), head_dim, dtype)
+        return col0, width
 
-    # (sequence, first token, tokens, first column, first key, end of the keys, own)
+    # (sequence, first token, tokens, first column, first key, end of the keys, own, width)
     rows = []
     for first, count, prefix in shared:
         begin, total = int(seq_start[first]), int(seq_start[first + count] - seq_start[first])
-        col0, _ = tiles(total)
-        block = np.zeros((col0.shape[0], 7), dtype=np.int64)
-        block[:, 0], block[:, 1], block[:, 2], block[:, 3], block[:, 5] = first, begin, total, col0, prefix
+        col0, width = tiles(total)
+        block = np.zeros((col0.shape[0], 8), dtype=np.int64)
+        block[:, 0], block[:, 1], block[:, 2], block[:, 3], block[:, 5], block[:, 7] = first, begin, total, col0, prefix, width
         rows.append(block)
     for seq in np.nonzero(counts > 0)[0]:
         total = int(counts[seq])
         col0, width = tiles(total)
-        block = np.zeros((col0.shape[0], 7), dtype=np.int64)
-        block[:, 0], block[:, 1], block[:, 2], block[:, 3], block[:, 4], block[:, 6] = seq, seq_start[seq], total, col0, prefix_of[seq], 1
+        block = np.zeros((col0.shape[0], 8), dtype=np.int64)
+        block[:, 0], block[:, 1], block[:, 2], block[:, 3], block[:, 4], block[:, 6], block[:, 7] = seq, seq_start[seq], total, col0, prefix_of[seq], 1, width
         block[:, 5] = seq_len[seq] - total + np.minimum(total - 1, (col0 + width - 1) // group) + 1
         rows.append(block)
     tokens = int(seq_start[-1])
     if not rows:
-        return np.zeros((0, 8), dtype=np.int32), np.zeros(tokens + 1, dtype=np.int32), wide
+        return np.zeros((0, 8), dtype=np.int32), np.zeros(tokens + 1, dtype=np.int32)
     rows = np.concatenate(rows)
-    # parts of equal length, so many that the step makes about two workgroups a compute unit
-    work = int((rows[:, 5] - rows[:, 4]).sum()) * num_kv_heads
-    part = max(1, -(-work // (2 * compute_units * PREFIX_ALIGN))) * PREFIX_ALIGN
-    # a group's prefix in even parts (they are all there is to cut of it); a sequence's own keys every `part` positions
     lengths = rows[:, 5] - rows[:, 4]
+    cost = np.array([PREFIX_COST[int(width)] for width in rows[:, 7]])
+    # Parts of about equal cost, so many that the step makes about two workgroups a compute unit.  All tiles of a group's prefix, and all
+    # of a sequence's own keys, are cut alike: at the parts of their widest.
+    budget = float((lengths * cost).sum()) * num_kv_heads / (2 * compute_units)
+    key = rows[:, 0] * 2 + rows[:, 6]
+    part = np.zeros(rows.shape[0], dtype=np.int64)
+    for which in np.unique(key):
+        mine = key == which
+        width, longest = int(rows[mine, 7].max()), int(lengths[mine].max())
+        count = max(1, min(-(-longest // PREFIX_LEAST[width]), int(round(longest * PREFIX_COST[width] / max(budget, 1.0))), 64))
+        part[mine] = -(-(-(-longest // count)) // 32) * 32
     cuts = -(-lengths // part)
-    even = np.where(rows[:, 6] == 0, -(-(-(-lengths // cuts)) // 32) * 32, part)
-    cuts = -(-lengths // even)
     index = np.repeat(np.arange(rows.shape[0]), cuts)
     place = np.arange(index.shape[0]) - np.repeat(np.cumsum(cuts) - cuts, cuts)
     items = np.empty((index.shape[0], 8), dtype=np.int32)
-    items[:, :7] = rows[index]
-    items[:, 4] = rows[index, 4] + place * even[index]
-    items[:, 5] = np.minimum(rows[index, 5], items[:, 4] + even[index])
+    items[:, :7] = rows[index, :7]
+    items[:, 4] = rows[index, 4] + place * part[index]
+    items[:, 5] = np.minimum(rows[index, 5], items[:, 4] + part[index])
     # parts of a token: its group's, then its own
-    ahead = np.zeros(sequences, dtype=np.int64)
+    ahead, own_part = np.zeros(sequences, dtype=np.int64), np.ones(sequences, dtype=np.int64)
     for first, count, prefix in shared:
         ahead[first:first + count] = cuts[np.nonzero((rows[:, 6] == 0) & (rows[:, 0] == first))[0][0]]
+    is_own = rows[:, 6] == 1
+    own_part[rows[is_own, 0]] = part[is_own]
     items[:, 7] = place + np.where(items[:, 6] == 1, ahead[items[:, 0]], 0)
     owner = np.repeat(np.arange(sequences), counts)
     position = seq_len[owner] - counts[owner] + np.arange(tokens) - seq_start[owner]
-    parts = ahead[owner] + -(-(position + 1 - prefix_of[owner]) // part)
+    parts = ahead[owner] + -(-(position + 1 - prefix_of[owner]) // own_part[owner])
     part_first = np.zeros(tokens + 1, dtype=np.int32)
     part_first[1:] = np.cumsum(parts)
-    return items, part_first, wide
+    return items, part_first
 
 
 def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device) -> SharedPrefixPlan:
@@ -2835,13 +2851,13 @@ def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads:
     positions 0 .. prefix - 1; all their tokens stand behind it.  Sequences in no group share nothing."""
     dtype_code(dtype)
     device = torch.device(device)
-    items, part_first, wide = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim,
-                                                  _compute_units(device) if device.type == "cuda" else 256)
+    items, part_first = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype,
+                                            _compute_units(device) if device.type == "cuda" else 256)
     if int(part_first[-1]) * num_heads >= 1 << 31 or items.shape[0] * num_kv_heads >= 1 << 31:
         raise invalid_shape("shared_prefix_plan: the step is beyond what one launch takes")
     longest = max((int(length) for length in seq_len), default=0)
     return SharedPrefixPlan(torch.from_numpy(items).to(device), torch.from_numpy(part_first).to(device), part_first.shape[0] - 1, int(part_first[-1]),
-                            wide, len(seq_len), longest, (num_heads, num_kv_heads, head_dim, dtype))
+                            len(seq_len), longest, (num_heads, num_kv_heads, head_dim, dtype))
 
 
 def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, plan: SharedPrefixPlan,
@@ -2887,7 +2903,7 @@ def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: t
     part_o = torch.empty((plan.parts * num_heads, head_dim), dtype=torch.float32, device=q.device)
     part_ml = torch.empty((plan.parts * num_heads, 2), dtype=torch.float32, device=q.device)
     _check(library().tlie_attention_prefix(_ptr(q), _ptr(cache), dtype_code(q.dtype), _ptr(block_table), block_table.shape[1], _ptr(plan.items),
-                                           plan.items.shape[0], plan.wide, _ptr(positions), _ptr(plan.part_first), _ptr(part_o), _ptr(part_ml),
+                                           plan.items.shape[0], _ptr(positions), _ptr(plan.part_first), _ptr(part_o), _ptr(part_ml),
                                            _ptr(sink), _ptr(out), tokens, num_heads, num_kv_heads, head_dim, page_size, ctypes.c_float(scale),
                                            ctypes.c_float(softcap or 0.0), _stream()), "attention_shared_prefix")
     return out
