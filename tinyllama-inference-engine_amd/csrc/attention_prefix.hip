@@ -329,7 +329,7 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
 // for all four, through LDS.  Blocks are asked for two ahead of their turn and wait in registers; two buffers in turn, so that one
 // barrier a block is enough (a wave writes a buffer again only behind the barrier that every wave reaches after it has read it).
 // Keys lie as [key][piece of 16 bytes], a key's pieces rotated by key / kPeriod so that the 16 keys that a read takes the same piece of
-// are spread over the banks; values as [half of 16 keys][dim][16 keys], of which a read takes 512 bytes in a row.
+// are spread over the banks; values as [half of 16 keys][16 dims][4 keys][dim], of which a read takes 512 bytes in the order of the lanes.
 template <int DT, int CT>
 __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh, const uint16_t* __restrict__ q, const uint16_t* __restrict__ cache,
                                                  const int* __restrict__ pages, int max_blocks, const int* __restrict__ positions,
@@ -349,21 +349,18 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
   const bool active = col0 < ncols;
   auto has_dims = [&](int ks) { return DT % 2 == 0 || ks < KS - 1 || grp < 2; };
 
-  int tok[CT], head[CT], last_key[CT];
-  bool valid[CT];
+  int last_key[CT];
   Piece query[CT][KS];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int c = col0 + ct * 16 + col;
-    valid[ct] = c < ncols;
-    tok[ct] = item.tok0 + (valid[ct] ? c / G : 0);
-    head[ct] = kvh * G + (valid[ct] ? c % G : 0);
-    last_key[ct] = !valid[ct] ? -1 : item.own ? pos0 + c / G : 0x7fffffff;
+    const bool valid = c < ncols;
+    const int tok = item.tok0 + (valid ? c / G : 0), head = kvh * G + (valid ? c % G : 0);
+    last_key[ct] = !valid ? -1 : item.own ? pos0 + c / G : 0x7fffffff;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       query[ct][ks] = Piece{0, 0, 0, 0};
-      if (valid[ct] && has_dims(ks))
-        query[ct][ks] = *reinterpret_cast<const Piece*>(q + (static_cast<size_t>(tok[ct]) * nq + head[ct]) * D + (ks * 4 + grp) * 8);
+      if (valid && has_dims(ks)) query[ct][ks] = *reinterpret_cast<const Piece*>(q + (static_cast<size_t>(tok) * nq + head) * D + (ks * 4 + grp) * 8);
     }
   }
   // the wave's keys end with those of its last column; keys that all its columns see need no mask
@@ -374,14 +371,16 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
   const size_t page_stride = static_cast<size_t>(2 * nkv) << page_shift;    // in rows of D
   const uint16_t* k_base = cache + (static_cast<size_t>(kvh) << page_shift) * D;
   const uint16_t* v_base = cache + (static_cast<size_t>(nkv + kvh) << page_shift) * D;
-  int from[kCalls];                                                          // a piece's place behind its half's page and row
-  int to[kCalls];                                                            // and in the buffer, in bytes
-  bool second[kCalls], of_values[kCalls];
+  // A piece's place behind its half's page and row, and in the buffer, in bytes.  At 128 dims (two calls a half) a thread brings the
+  // same place of both halves, so that one of each is kept for the keys and one for the values: every register counts there.
+  constexpr bool kAlike = DT == 8;
+  constexpr int kPlaces = kAlike ? 2 : kCalls;
+  int from[kPlaces], to[kPlaces];
+  bool second[kPlaces];
 #pragma unroll
-  for (int i = 0; i < kCalls; ++i) {
-    const int call = min(wave + 4 * i, 2 * DT - 1), piece = (call % DT) * 64 + lane;     // (past the last: the last again, the same bytes)
-    of_values[i] = call >= DT;
-    if (!of_values[i]) {
+  for (int i = 0; i < kPlaces; ++i) {
+    const int call = min(kAlike ? wave + 8 * i : wave + 4 * i, 2 * DT - 1), piece = (call % DT) * 64 + lane;      // (past the last: the last again, the same bytes)
+    if (call < DT) {
       const int key = piece / kPieces, place = piece % kPieces;
       second[i] = key >= 16;
       from[i] = (key & 15) * D + place * 8;
@@ -390,20 +389,29 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
       const int rest = piece % (2 * D);
       second[i] = piece >= 2 * D;
       from[i] = ((rest >> 1) << page_shift) + (rest & 1) * 8;
-      to[i] = kBytes + piece * 16;
+      to[i] = kBytes + (second[i] ? D * 32 : 0) + ((rest >> 5) * 64 + (rest & 1) * 32 + ((rest >> 1) & 15)) * 8;
     }
   }
+  auto is_values = [&](int i) { return kAlike ? i >= 2 : min(wave + 4 * i, 2 * DT - 1) >= DT; };       // (the same for the whole wave)
+  auto to_of = [&](int i) { return kAlike ? to[i >> 1] + (i & 1) * (kBytes / 2) : to[i]; };
   Piece staged[2][kCalls];
   TableWindow window;
   auto bring = [&](int kb, Piece (&into)[kCalls]) {
     const size_t at_a = static_cast<size_t>(window.page(kb >> page_shift)) * page_stride * D;
     const size_t at_b = static_cast<size_t>(window.page((kb + 16) >> page_shift)) * page_stride * D;
     const int row_a = kb & page_mask, row_b = (kb + 16) & page_mask;
+    const uint16_t *keys_a = k_base + at_a + row_a * D, *keys_b = k_base + at_b + row_b * D;
+    const uint16_t *values_a = v_base + at_a + row_a, *values_b = v_base + at_b + row_b;
 #pragma unroll
     for (int i = 0; i < kCalls; ++i) {
-      const uint16_t* a = of_values[i] ? v_base + at_a + row_a : k_base + at_a + row_a * D;
-      const uint16_t* b = of_values[i] ? v_base + at_b + row_b : k_base + at_b + row_b * D;
-      into[i] = *reinterpret_cast<const Piece*>((second[i] ? b : a) + from[i]);
+      const uint16_t* base;
+      if constexpr (kAlike) {
+        base = i == 0 ? keys_a : i == 1 ? keys_b : i == 2 ? values_a : values_b;
+      } else {
+        const bool of_values = is_values(i);
+        base = second[i] ? (of_values ? values_b : keys_b) : (of_values ? values_a : keys_a);
+      }
+      into[i] = *reinterpret_cast<const Piece*>(base + from[kAlike ? i >> 1 : i]);
     }
   };
 
@@ -437,6 +445,26 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
           s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&k), *reinterpret_cast<const bf16x8*>(&query[ct][ks]),
                                                              s[ct][t], 0, 0, 0);
       }
+    }
+    // (the values are asked for here, so that they are there when the probabilities are)
+    Piece values[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const unsigned char* place = buffer + kBytes + (dt * 64 + lane) * 8;
+      const Half a = *reinterpret_cast<const Half*>(place), b = *reinterpret_cast<const Half*>(place + D * 32);
+      values[dt] = Piece{a[0], a[1], b[0], b[1]};
+    }
+    if (ragged) {
+      uint32_t keep[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int key = kb + (w >> 1) * 16 + grp * 4 + (w & 1) * 2;
+        keep[w] = (key >= item.key_lo && key < item.key_hi ? 0x0000ffffu : 0u) | (key + 1 >= item.key_lo && key + 1 < item.key_hi ? 0xffff0000u : 0u);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) values[dt][w] &= keep[w];
     }
     if (cap_pre > 0.f) {
       settle(s);
@@ -500,29 +528,23 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
       for (int i = 0; i < 4; ++i) packed[ct][i] = pack_bf16(p[2 * i], p[2 * i + 1]);
     }
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      Half a = *reinterpret_cast<const Half*>(buffer + kBytes + (dt * 16 + col) * 32 + grp * 8);
-      Half b = *reinterpret_cast<const Half*>(buffer + kBytes + D * 32 + (dt * 16 + col) * 32 + grp * 8);
-      if (ragged) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = kb + grp * 4 + j;
-          const uint32_t mask = (j & 1) ? 0x0000ffffu : 0xffff0000u;
-          if (key < item.key_lo || key >= item.key_hi) a[j >> 1] &= mask;
-          if (key + 16 < item.key_lo || key + 16 >= item.key_hi) b[j >> 1] &= mask;
-        }
-      }
-      const Piece v = Piece{a[0], a[1], b[0], b[1]};
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
-        o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&v), *reinterpret_cast<const bf16x8*>(&packed[ct]),
+        o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&values[dt]), *reinterpret_cast<const bf16x8*>(&packed[ct]),
                                                             o[ct][dt], 0, 0, 0);
-    }
   };
   auto turn = [&](int kb, int last, int buffer, Piece (&waiting)[kCalls]) {
     unsigned char* place = lds + buffer * 2 * kBytes;
 #pragma unroll
-    for (int i = 0; i < kCalls; ++i) *reinterpret_cast<Piece*>(place + to[i]) = waiting[i];
+    for (int i = 0; i < kCalls; ++i) {
+      unsigned char* there = place + to_of(i);
+      if (is_values(i)) {
+        *reinterpret_cast<Half*>(there) = Half{waiting[i][0], waiting[i][1]}, *reinterpret_cast<Half*>(there + 128) = Half{waiting[i][2], waiting[i][3]};
+      } else {
+        *reinterpret_cast<Piece*>(there) = waiting[i];
+      }
+    }
     lds_barrier();
     bring(min(kb + 64, last), waiting);                        // (past the last block the last again: as many loads on every path)
     if (kb <= last && kb < high) work(kb, place);
@@ -545,15 +567,19 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
     sum[ct] += __shfl_xor(sum[ct], 32, 64);
   }
   settle(o);
+  int lane_again = threadIdx.x & 63;                             // (formed again: kept over the walk, the columns' places cost registers)
+  asm volatile("" : "+v"(lane_again));
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int first_part = part_first[tok[ct]];
-    if (!valid[ct] || item.part >= part_first[tok[ct] + 1] - first_part) continue;
-    const size_t slot = static_cast<size_t>(first_part + item.part) * nq + head[ct];
+    const int c = col0 + ct * 16 + (lane_again & 15), group = lane_again >> 4;
+    if (c >= ncols) continue;
+    const int tok = item.tok0 + c / G, head = kvh * G + c % G, first_part = part_first[tok];
+    if (item.part >= part_first[tok + 1] - first_part) continue;
+    const size_t slot = static_cast<size_t>(first_part + item.part) * nq + head;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
-      *reinterpret_cast<float4*>(part_o + slot * D + dt * 16 + grp * 4) = make_float4(o[ct][dt][0], o[ct][dt][1], o[ct][dt][2], o[ct][dt][3]);
-    if (grp == 0) part_ml[slot * 2] = top[ct], part_ml[slot * 2 + 1] = sum[ct];
+      *reinterpret_cast<float4*>(part_o + slot * D + dt * 16 + group * 4) = make_float4(o[ct][dt][0], o[ct][dt][1], o[ct][dt][2], o[ct][dt][3]);
+    if (group == 0) part_ml[slot * 2] = top[ct], part_ml[slot * 2 + 1] = sum[ct];
   }
 }
 
