@@ -326,8 +326,8 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
 }
 
 // An item of many columns, bfloat16: each wave has 16 * CT columns of its own, and every block of 32 keys and values is brought once
-// for all four, through LDS.  Blocks are asked for two ahead of their turn and wait in registers; two buffers in turn, so that one
-// barrier a block is enough (a wave writes a buffer again only behind the barrier that every wave reaches after it has read it).
+// for all four, through LDS, two at a time.  They are asked for two ahead of their turn and wait in registers; two buffers in turn, so
+// that one barrier a turn is enough (a wave writes a buffer again only behind the barrier that every wave reaches after it has read it).
 // Keys lie as [key][piece of 16 bytes], a key's pieces rotated by key / kPeriod so that the 16 keys that a read takes the same piece of
 // are spread over the banks; values as [half of 16 keys][16 dims][4 keys][dim], of which a read takes 512 bytes in the order of the lanes.
 template <int DT, int CT>
@@ -534,8 +534,7 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
         o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&values[dt]), *reinterpret_cast<const bf16x8*>(&packed[ct]),
                                                             o[ct][dt], 0, 0, 0);
   };
-  auto turn = [&](int kb, int last, int buffer, Piece (&waiting)[kCalls]) {
-    unsigned char* place = lds + buffer * 2 * kBytes;
+  auto put = [&](unsigned char* place, const Piece (&waiting)[kCalls]) {
 #pragma unroll
     for (int i = 0; i < kCalls; ++i) {
       unsigned char* there = place + to_of(i);
@@ -545,20 +544,25 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
         *reinterpret_cast<Piece*>(there) = waiting[i];
       }
     }
-    lds_barrier();
-    bring(min(kb + 64, last), waiting);                        // (past the last block the last again: as many loads on every path)
-    if (kb <= last && kb < high) work(kb, place);
   };
+  int buffer = 0;
   for (int begin = item.key_lo & ~31; begin < item.key_hi;) {
     window.load(pages, max_blocks, begin >> page_shift);
     const int end = min(item.key_hi, (window.first + 128) << page_shift), last = (end - 1) & ~31;
     bring(begin, staged[0]);
     bring(min(begin + 32, last), staged[1]);
     for (int kb = begin; kb <= last; kb += 64) {
-      turn(kb, last, 0, staged[0]);
-      turn(kb + 32, last, 1, staged[1]);
+      unsigned char* place = lds + buffer * 4 * kBytes;
+      put(place, staged[0]);
+      put(place + 2 * kBytes, staged[1]);
+      lds_barrier();
+      bring(min(kb + 64, last), staged[0]);                    // (past the last block the last again: as many loads on every path)
+      bring(min(kb + 96, last), staged[1]);
+#pragma unroll 1
+      for (int u = 0; u < 2; ++u)
+        if (kb + 32 * u <= last && kb + 32 * u < high) work(kb + 32 * u, place + u * 2 * kBytes);
+      buffer ^= 1;
     }
-    lds_barrier();                                             // (the next window's first block reuses the first buffer)
     begin = end;
   }
 #pragma unroll
@@ -591,7 +595,7 @@ prefix_items_kernel(const void* __restrict__ q, const void* __restrict__ cache, 
                     const int* __restrict__ items, const int* __restrict__ positions, const int* __restrict__ part_first, float* __restrict__ part_o,
                     float* __restrict__ part_ml, int nq, int nkv, int page_shift, float scale_log2, float cap_pre) {
   constexpr int kFloatWide = DT <= 8 ? 2 : 1;
-  constexpr int kNarrow = kPrefixWaves * ((FLOAT ? kFloatWide : 1) * 32 + DT * 256) * 4, kWideBytes = FLOAT ? 0 : 4 * 64 * DT * 16;
+  constexpr int kNarrow = kPrefixWaves * ((FLOAT ? kFloatWide : 1) * 32 + DT * 256) * 4, kWideBytes = FLOAT ? 0 : 8 * 64 * DT * 16;
   __shared__ __attribute__((aligned(16))) unsigned char lds[kNarrow > kWideBytes ? kNarrow : kWideBytes];
   const int kvh = blockIdx.x % nkv;
   PrefixItem item;
