@@ -2089,6 +2089,24 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor | None = None, top_p:
     return out
 
 
+_bound_entries: dict = {}
+
+
+def _entry(name: str, kinds: str):
+    """The library's entry `name` with its arguments' types set, a letter each (p: a pointer, as an int or None; i: int; f: float): a
+    call then builds no object an argument (of 20 arguments 3 us, a quarter of what the host needs for a call of two launches)."""
+    found = _bound_entries.get(name)
+    if found is None:
+        found = getattr(library(), name)
+        found.argtypes = [{"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}[kind] for kind in kinds]
+        _bound_entries[name] = found
+    return found
+
+
+def _address(tensor: torch.Tensor | None):
+    return None if tensor is None else tensor.data_ptr()
+
+
 def _one_device(what: str, *tensors) -> None:
     """All tensors (None: absent) lie on the current device, whose current stream the kernels go to."""
     current = torch._C._cuda_getDevice()
@@ -2153,8 +2171,9 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: to
     if rows > 0:
         parts = draw_parts(rows, vocab)
         scratch = torch.empty((rows * (DRAW_ROW_BYTES + parts * DRAW_PART_BYTES),), dtype=torch.uint8, device=logits.device) if parts else None
-        _check(library().tlie_draw(_ptr(logits), rows, vocab, _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), parts,
-                                   _ptr(scratch), _ptr(out), _ptr(out_logprobs), _stream()), "sample_filtered")
+        _check(_entry("tlie_draw", "piipppppipppp")(logits.data_ptr(), rows, vocab, uniform.data_ptr(), _address(temperature), _address(top_k), _address(top_p),
+                                                    _address(min_p), parts, _address(scratch), out.data_ptr(), _address(out_logprobs), _stream()),
+               "sample_filtered")
     return (out, out_logprobs) if logprobs else out
 
 
@@ -2906,12 +2925,14 @@ def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: t
         return out
     if plan.items.shape[0] == 0:
         return out.zero_()
-    part_o = torch.empty((plan.parts * num_heads, head_dim), dtype=torch.float32, device=q.device)
-    part_ml = torch.empty((plan.parts * num_heads, 2), dtype=torch.float32, device=q.device)
-    _check(library().tlie_attention_prefix(_ptr(q), _ptr(cache), dtype_code(q.dtype), _ptr(block_table), block_table.shape[1], _ptr(plan.items),
-                                           plan.items.shape[0], _ptr(positions), _ptr(plan.part_first), _ptr(part_o), _ptr(part_ml),
-                                           _ptr(sink), _ptr(out), tokens, num_heads, num_kv_heads, head_dim, page_size, ctypes.c_float(scale),
-                                           ctypes.c_float(softcap or 0.0), _stream()), "attention_shared_prefix")
+    # the parts' results: their values (a part and head's at a multiple of 64 bytes), then their maxima and sums
+    rows = plan.parts * num_heads
+    parts = torch.empty((rows * (head_dim + 2),), dtype=torch.float32, device=q.device)
+    address = parts.data_ptr()
+    _check(_entry("tlie_attention_prefix", "ppipipippppppiiiiiffp")(
+        q.data_ptr(), cache.data_ptr(), dtype_code(q.dtype), block_table.data_ptr(), block_table.shape[1], plan.items.data_ptr(), plan.items.shape[0],
+        positions.data_ptr(), plan.part_first.data_ptr(), address, address + rows * head_dim * 4, _address(sink), out.data_ptr(), tokens, num_heads,
+        num_kv_heads, head_dim, page_size, scale, softcap or 0.0, _stream()), "attention_shared_prefix")
     return out
 
 
