@@ -1,0 +1,197 @@
+"""Requests that share their first positions' pages: the allocator's holders, forks in the cache manager, and families in the
+scheduler, on the host."""
+import random
+
+import pytest
+import torch
+
+from tlie_amd.cache.manager import CacheManager, RunNeed
+from tlie_amd.cache.pages import PageAllocator
+from tlie_amd.engine.scheduler import Request, SamplingParams, Scheduler
+from tlie_amd.errors import EngineError
+from tlie_amd.parts.base import CacheNeed, StateNeed
+
+
+def manager(pages=40, requests=8, page_size=4, window=None, state=False):
+    need = RunNeed(cache_of=0, cache=CacheNeed((2, 1), 3, window), state=StateNeed((2,)) if state else None)
+    return CacheManager([need], page_size, pages, requests, torch.float32, "cpu")
+
+
+def grow(cache, request, count):
+    cache.reserve(request, count)
+    cache.commit(request, count)
+
+
+def test_a_page_comes_back_with_its_last_holder():
+    pages = PageAllocator(3)
+    held = pages.alloc(2)
+    pages.share(held)
+    pages.release(held)
+    assert pages.num_free == 1 and all(pages.in_use(page) for page in held)
+    pages.release(held)
+    assert pages.num_free == 3 and not any(pages.in_use(page) for page in held)
+    for wrong in ([held[0]], [99], [-1]):
+        with pytest.raises(EngineError):
+            pages.share(wrong)
+
+
+@pytest.mark.parametrize("length", [1, 3, 4, 5, 8, 10])
+def test_a_fork_holds_the_same_pages_and_a_copy_of_the_last(length):
+    cache = manager()
+    cache.admit("a")
+    grow(cache, "a", 10)
+    pool = cache.bindings[0].cache
+    pool.copy_(torch.randn_like(pool))
+    cache.fork("a", "b", length)
+    mine, its = cache.page_list("b", 0), cache.page_list("a", 0)
+    whole = length // 4
+    assert mine[:whole] == its[:whole] and len(mine) == (length + 3) // 4 and cache.length("b") == length
+    if length % 4:
+        assert mine[-1] not in its and torch.equal(pool[mine[-1]], pool[its[whole]])
+    cache.check()
+    held = [cache.held(name) for name in "ab"]
+    assert all((info.family != 0) == (whole > 0) for info in held)
+    assert not whole or held[0].family == held[1].family and min(info.shared for info in held) == whole * 4
+    grow(cache, "b", 7)
+    grow(cache, "a", 2)
+    cache.check()
+    cache.release("a")
+    cache.check()
+    cache.release("b")
+    assert cache.free_pages() == [40]
+    cache.check()
+
+
+def test_forks_of_forks_claim_no_more_than_they_share():
+    cache = manager()
+    cache.admit("a")
+    grow(cache, "a", 12)
+    cache.fork("a", "b", 8)
+    grow(cache, "b", 12)
+    cache.fork("b", "c", 20)                     # more than b has in common with a
+    cache.fork("b", "d", 4)
+    lists = {name: cache.page_list(name, 0) for name in "abcd"}
+    held = {name: cache.held(name) for name in "abcd"}
+    for one in "abcd":
+        for other in "abcd":
+            blocks = min(held[one].shared, held[other].shared) // 4
+            assert held[one].family == held[other].family and lists[one][:blocks] == lists[other][:blocks]
+    cache.check()
+
+
+def test_forks_that_are_refused_take_nothing():
+    cache = manager(pages=3, requests=2)
+    cache.admit("a")
+    grow(cache, "a", 10)
+    for source, length in (("a", 11), ("a", 0), ("x", 2)):
+        with pytest.raises(EngineError):
+            cache.fork(source, "b", length)
+    with pytest.raises(EngineError):
+        cache.fork("a", "b", 5)                  # no page for the copy
+    assert not cache.is_live("b") and cache.free_slots == 1
+    cache.fork("a", "b", 8)
+    with pytest.raises(EngineError):
+        cache.fork("a", "c", 4)                  # no slot
+    cache.check()
+    for kind in (dict(window=8), dict(state=True)):
+        other = manager(**kind)
+        other.admit("a")
+        grow(other, "a", 10)
+        assert not other.can_fork
+        with pytest.raises(EngineError):
+            other.fork("a", "b", 4)
+
+
+def family_of(count, prompt, **params):
+    family = []
+    for index in range(count):
+        family.append(Request(id=("answer", index), prompt=list(prompt), params=SamplingParams(**params), family=family))
+    return family
+
+
+def run(scheduler, cache, steps=400):
+    """Plans and commits; tokens are their place in the request.  Returns the planned tokens of every step."""
+    seen = []
+    for _ in range(steps):
+        if not scheduler.has_work():
+            break
+        plan = scheduler.schedule()
+        assert plan
+        assert cache.reserve_all([(item.request.id, item.count) for item in plan])
+        for item in plan:
+            cache.commit(item.request.id, item.count)
+        cache.check()
+        seen.append([(item.request.id, item.first, item.count) for item in plan])
+        scheduler.update(plan, [item.first + item.count for item in plan if item.samples])
+    assert not scheduler.has_work()
+    return seen
+
+
+def test_answers_compute_the_prompt_once():
+    cache = manager(pages=60)
+    scheduler = Scheduler(cache)
+    family = family_of(4, range(21), max_tokens=5)
+    for request in family:
+        scheduler.add(request)
+    seen = run(scheduler, cache)
+    brought = {request.id: sum(count for step in seen for name, _, count in step if name == request.id) for request in family}
+    assert brought[family[0].id] == 21 + 4 and all(brought[request.id] == 1 + 4 for request in family[1:])
+    assert all(len(request.generated) == 5 for request in family)
+    assert cache.free_pages() == [60]
+
+
+def test_a_family_stands_side_by_side():
+    cache = manager(pages=100, requests=8)
+    scheduler = Scheduler(cache)
+    one, two = family_of(3, range(9), max_tokens=6), family_of(3, range(13), max_tokens=6)
+    for request in two:
+        request.id = ("other", request.id[1])
+    for first in range(3):
+        scheduler.add(one[first])
+        scheduler.add(two[first])
+    for step in run(scheduler, cache):
+        kinds = [name[0] for name, _, _ in step]
+        assert kinds == sorted(kinds, key=kinds.index)
+
+
+def test_short_prompts_and_caches_that_cannot_fork_run_as_ever():
+    for cache, length in ((manager(pages=60), 4), (manager(pages=60, window=8), 21), (manager(pages=60, state=True), 21)):
+        scheduler = Scheduler(cache)
+        family = family_of(3, range(length), max_tokens=3)
+        for request in family:
+            scheduler.add(request)
+        seen = run(scheduler, cache)
+        assert all(sum(count for step in seen for name, _, count in step if name == request.id) == length + 2 for request in family)
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_pools_too_small_for_all_lose_nothing(seed):
+    """Preempted, readmitted, aborted members: every request gets its tokens, every page comes back."""
+    rng = random.Random(seed)
+    cache = manager(pages=rng.randint(12, 30), requests=rng.randint(2, 6))
+    scheduler = Scheduler(cache, max_tokens_per_step=rng.randint(3, 30), chunk_size=rng.randint(2, 12), admit_partial=rng.random() < 0.5)
+    families = [family_of(rng.randint(1, 5), range(rng.randint(1, 25)), max_tokens=rng.randint(1, 14)) for _ in range(3)]
+    for index, family in enumerate(families):
+        for request in family:
+            request.id = (index, request.id[1])
+            scheduler.add(request)
+    victim = families[0][0].id
+    scheduler.abort(victim)
+    run(scheduler, cache, steps=3000)
+    for family in families:
+        for request in family:
+            assert len(request.generated) == request.params.max_tokens or request.id == victim
+    assert cache.free_pages() == [cache.num_pages] and cache.free_slots == cache.max_requests
+
+
+@pytest.mark.parametrize("bad", [dict(top_k=-1), dict(top_k=1 << 31), dict(min_p=-0.1), dict(min_p=1.5), dict(min_p=float("nan"))])
+def test_sampling_options_that_are_refused(bad):
+    with pytest.raises(EngineError):
+        SamplingParams(**bad).validate()
+
+
+def test_the_numbers_of_many_rows_are_the_numbers_of_each():
+    from tlie_amd.sampling.sampler import uniform01, uniforms01
+    rng = random.Random(0)
+    seeds, counters = [rng.randrange(-2 ** 63, 2 ** 64) for _ in range(100)], [rng.randrange(1 << 20) for _ in range(100)]
+    assert uniforms01(seeds, counters).tolist() == [uniform01(seed, counter) for seed, counter in zip(seeds, counters)]

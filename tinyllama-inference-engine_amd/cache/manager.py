@@ -16,11 +16,16 @@ how many values per position, of which type) is the mixer's `CacheNeed`; how pos
 lie inside it is the mixer's own business, and nothing here knows of keys or values.  A windowed
 group gives a page back as soon as every position on it is out of every later token's window.
 
+Requests with the same first positions may hold the same pages (`fork`): the pages that those positions fill are
+one request's as much as the other's, and go back when the last of them has given them back; no request writes on a page that
+another one holds, since each writes behind its own length, on pages of its own.
+
 Nothing is cleared when pages or slots come back: a kernel reads only rows that were written for
 the request that now owns the page, so what an earlier owner left cannot reach a result.
 """
 from __future__ import annotations
 
+from collections import Counter
 from dataclasses import dataclass, field
 from typing import Hashable
 
@@ -55,6 +60,8 @@ class RequestPages:
     length: int = 0                                        # positions committed so far
     pages: list[list[int]] = field(default_factory=list)   # per group: block index -> page or ABSENT
     serial: int = 0                                        # which admission this is: no two ever share one
+    family: int = 0                                        # requests of one family (not 0) hold the same pages
+    shared: int = 0                                        # for so many positions, or as many as the other does if that is fewer
 
 
 class CacheManager:
@@ -143,6 +150,42 @@ class CacheManager:
             area[slot].zero_()
         self._admissions += 1
         self._requests[request] = RequestPages(slot=slot, pages=[[] for _ in self.groups], serial=self._admissions)
+        return slot
+
+    @property
+    def can_fork(self) -> bool:
+        """Whether what a request keeps is pages alone, all of them for good: state at an earlier length, and positions out of a
+        window, are not there to be shared."""
+        return bool(self.groups) and not self.state_areas and all(group.window is None for group in self.groups)
+
+    def fork(self, source: Hashable, request: Hashable, length: int) -> int:
+        """Takes a request slot for a request whose first `length` positions are those of `source` (live, at least that long): it
+        holds the pages that they fill together with it, and a copy of the one that they end on.  `out_of_memory` when a slot or a
+        page for that copy is not free (then nothing is taken)."""
+        entry = self._entry(source)
+        if not self.can_fork:
+            raise invalid_argument("requests that keep state, or a window of positions, cannot be forked")
+        if not 0 < length <= entry.length:
+            raise invalid_argument(f"request {source!r} has {entry.length} positions, of which {length} cannot be shared")
+        whole, rest = length // self.page_size, length % self.page_size
+        if rest and any(group.allocator.num_free < 1 for group in self.groups):
+            raise out_of_memory(f"request {request!r} needs a page for the positions that end inside one, free are {self.free_pages()}")
+        slot = self.admit(request)
+        forked = self._requests[request]
+        for index, group in enumerate(self.groups):
+            pages = entry.pages[index][:whole]
+            group.allocator.share(pages)
+            if rest:
+                pages = pages + group.allocator.alloc(1)
+                for run in group.owners:
+                    pool = self.bindings[run].cache
+                    pool[pages[-1]].copy_(pool[entry.pages[index][whole]])
+            forked.pages[index] = pages
+        forked.length = length
+        if whole:
+            if not entry.family:
+                entry.family, entry.shared = entry.serial, whole * self.page_size
+            forked.family, forked.shared = entry.family, min(whole * self.page_size, entry.shared)
         return slot
 
     def is_live(self, request: Hashable) -> bool:
@@ -290,16 +333,19 @@ class CacheManager:
 
     # ---- bookkeeping checks (used by tests and by debug runs) ----------------------------------
     def check(self) -> None:
-        """No page lost, none held twice, none both free and held; the same for slots."""
+        """No page lost, none held by more requests than it has holders, none both free and held; the same for slots."""
         for group_index, group in enumerate(self.groups):
             held = [page for entry in self._requests.values() for page in entry.pages[group_index] if page != ABSENT]
             free = group.allocator.free_pages()
-            if len(set(held)) != len(held):
+            holders = Counter(held)
+            if any(group.allocator.holders(page) < count for page, count in holders.items()):
                 raise AssertionError(f"group {group_index}: a page is held twice")
+            if any(group.allocator.holders(page) > count for page, count in holders.items()):
+                raise AssertionError(f"group {group_index}: a page has a holder that is no request")
             if set(held) & set(free):
                 raise AssertionError(f"group {group_index}: a page is both held and free")
-            if len(held) + len(free) != group.allocator.num_pages or len(set(free)) != len(free):
-                raise AssertionError(f"group {group_index}: {group.allocator.num_pages - len(held) - len(free)} pages are lost")
+            if len(holders) + len(free) != group.allocator.num_pages or len(set(free)) != len(free):
+                raise AssertionError(f"group {group_index}: {group.allocator.num_pages - len(holders) - len(free)} pages are lost")
             if any(not group.allocator.in_use(page) for page in held):
                 raise AssertionError(f"group {group_index}: a held page is not marked in use")
         slots = [entry.slot for entry in self._requests.values()]

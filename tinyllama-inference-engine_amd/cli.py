@@ -16,7 +16,9 @@ under the scheduler (continuous batching): `ids:1,2,3;ids:4,5` (token ids only),
 holds `{"greedy_tokens": [...]}` and the (first prompt's) generated tokens must begin it
 (app/cuda_reference.cu:198-211).
 Options (after the positionals): --dtype bfloat16|float32, --temperature T, --top-p P, --seed S
-(the reference's request options of the same names, app/server.cpp:601-613); the cache and the
+(the reference's request options of the same names, app/server.cpp:601-613), --top-k K, --min-p P (both narrow the draw further);
+--answers N (so many to each prompt, which share its cache; the output then has `answers`, a list per prompt under `requests`), --logprobs
+(the tokens' log-probabilities beside them); the cache and the
 scheduler: --max-cache-tokens N (positions the page pool holds), --page-size P, --max-requests R
 (request slots), --max-tokens-per-step T (a step's token budget), --chunk-size C (the most tokens of
 one prompt in a step), --prompt-tokens-beside-decodes N (the most prompt tokens in a step that also
@@ -37,8 +39,8 @@ USAGE = ("usage: tinyllama_amd generate MODEL_DIR PROMPT MAX_TOKENS [GOLDEN_JSON
          "       tinyllama_amd benchmark MODEL_DIR CONTEXT OUTPUT_TOKENS WARMUP SAMPLES\n"
          "       tinyllama_amd batch MODEL_DIR CONTEXT OUTPUT_TOKENS WARMUP SAMPLES\n"
          "       tinyllama_amd random MODEL_DIR CONFIG_JSON SEED\n"
-         "options: [--dtype bfloat16|float32] [--temperature T] [--top-p P] [--seed S] [--expect-sha256 HEX]\n"
-         "         [--max-cache-tokens N] [--page-size P] [--max-requests R] [--max-tokens-per-step T] [--chunk-size C]\n"
+         "options: [--dtype bfloat16|float32] [--temperature T] [--top-p P] [--top-k K] [--min-p P] [--seed S] [--answers N] [--logprobs]\n"
+         "         [--expect-sha256 HEX] [--max-cache-tokens N] [--page-size P] [--max-requests R] [--max-tokens-per-step T] [--chunk-size C]\n"
          "         [--prompt-tokens-beside-decodes N] [--admit-partial] [--prompts-file FILE] [--batch N] [--min-ratio X]\n")
 
 
@@ -111,14 +113,19 @@ def command_generate(args) -> int:
     max_tokens = parse_integer(args.rest[0], "MAX_TOKENS", 1)
     prompts, tokenizer = all_prompts(args)
     ids = prompts[0]
-    engine = _engine(args, sum(len(prompt) + max_tokens for prompt in prompts), len(prompts))
+    if args.answers < 1:
+        raise invalid_argument("--answers must be an integer >= 1")
+    engine = _engine(args, sum(len(prompt) + max_tokens for prompt in prompts) * args.answers, len(prompts) * args.answers)
     started = time.perf_counter()
-    timings, stats = {}, {}
+    timings, stats, logprobs = {}, {}, [] if args.logprobs else None
     outputs = engine.generate(prompts, max_tokens=max_tokens, temperature=args.temperature, top_p=args.top_p,
                               seed=args.seed, timings=timings, stats=stats,
                               max_tokens_per_step=args.max_tokens_per_step or 2048, chunk_size=args.chunk_size or None,
                               prompt_tokens_beside_decodes=args.prompt_tokens_beside_decodes or None,
-                              admit_partial=args.admit_partial)
+                              admit_partial=args.admit_partial, top_k=args.top_k, min_p=args.min_p, answers=args.answers, logprobs=logprobs)
+    answers, logprob_answers = outputs, logprobs
+    if args.answers > 1:                                  # (the other keys hold each prompt's first answer)
+        outputs, logprobs = [row[0] for row in outputs], [row[0] for row in logprobs] if logprobs is not None else None
     generated = outputs[0]
     elapsed = (time.perf_counter() - started) * 1e3
     if len(args.rest) > 1:
@@ -133,11 +140,19 @@ def command_generate(args) -> int:
               "steps": stats.get("steps"), "preemptions": stats.get("preemptions")}
     if tokenizer is not None:
         result["text"] = tokenizer.decode(generated)
+    if logprobs is not None:
+        result["logprobs"] = logprobs[0]
+    if args.answers > 1:
+        result["answers"] = answers[0]
+        if logprobs is not None:
+            result["answer_logprobs"] = logprob_answers[0]
     if len(prompts) > 1:
         # one row per prompt, in the order given; the top-level keys stay the first prompt's
         result["requests"] = [{"prompt_tokens": len(prompt), "generated_tokens": output,
-                               **({"text": tokenizer.decode(output)} if tokenizer is not None else {})}
-                              for prompt, output in zip(prompts, outputs)]
+                               **({"text": tokenizer.decode(output)} if tokenizer is not None else {}),
+                               **({"logprobs": logprobs[index]} if logprobs is not None else {}),
+                               **({"answers": answers[index]} if args.answers > 1 else {})}
+                              for index, (prompt, output) in enumerate(zip(prompts, outputs))]
     print(json.dumps(result))
     return 0
 
@@ -318,6 +333,10 @@ def main(argv=None) -> int:
     parser.add_argument("--dtype", default="bfloat16")
     parser.add_argument("--temperature", type=float, default=0.0)
     parser.add_argument("--top-p", type=float, default=1.0)
+    parser.add_argument("--top-k", type=int, default=0)
+    parser.add_argument("--min-p", type=float, default=0.0)
+    parser.add_argument("--answers", type=int, default=1)
+    parser.add_argument("--logprobs", action="store_true")
     parser.add_argument("--seed", type=int, default=0)
     parser.add_argument("--max-cache-tokens", type=int, default=0)
     parser.add_argument("--page-size", type=int, default=0)

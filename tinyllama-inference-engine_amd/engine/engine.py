@@ -128,7 +128,8 @@ class Engine:
                  top_p: float = 1.0, seed: int = 0, stop_on_eos: bool = False, max_tokens_per_step: int = 2048,
                  max_seqs_per_step: int | None = None, chunk_size: int | None = None,
                  timings: dict | None = None, stats: dict | None = None,
-                 prompt_tokens_beside_decodes: int | None = None, admit_partial: bool = False) -> list[list[int]]:
+                 prompt_tokens_beside_decodes: int | None = None, admit_partial: bool = False, top_k: int = 0, min_p: float = 0.0,
+                 answers: int = 1, logprobs: list | None = None) -> list:
         """Token ids in, generated token ids out, one list per prompt.  Request i samples with
         seed + i.  All prompts run together under the scheduler (continuous batching, prompts cut
         into portions under the token budget).  `timings`: a dict that receives the sums of the
@@ -136,18 +137,31 @@ class Engine:
         only decode (the keys of the reference's `generate`, app/cuda_reference.cu:216-224).
         `stats`: a dict that receives what the scheduler counted (steps, prompt and decoded tokens,
         preemptions) and how many matrix products of this process fell from the vendor's library to the
-        plain kernel (`library_fallbacks`).  prompt_tokens_beside_decodes, admit_partial: see `Scheduler`."""
+        plain kernel (`library_fallbacks`).  prompt_tokens_beside_decodes, admit_partial: see `Scheduler`.
+        top_k, min_p: see `ops.sample_filtered`.  answers: so many to each prompt, answer a of prompt i with seed + i * answers + a;
+        more than one, and there is a list of answers per prompt in place of a list of tokens.  Where the model's caches allow it
+        (`CacheManager.can_fork`) the answers hold the prompt's pages together, so that its keys are computed once, and read once a step
+        for all of them.  logprobs: a list that receives, laid out as the result, every token's log-probability (of the model's own
+        distribution: log softmax of the logits, whatever the temperature and filters)."""
         scheduler = Scheduler(self.cache, max_tokens_per_step=max_tokens_per_step,
                               max_seqs_per_step=max_seqs_per_step or self.cache.max_requests, chunk_size=chunk_size,
                               max_positions=self.spec.max_positions, eos_token_id=self.spec.eos_token_id,
                               prompt_tokens_beside_decodes=prompt_tokens_beside_decodes, admit_partial=admit_partial)
+        if answers < 1:
+            raise invalid_argument("answers must be an integer >= 1")
         requests = []
         for index, prompt in enumerate(prompts):
-            params = SamplingParams(max_tokens=max_tokens, temperature=temperature, top_p=top_p, seed=seed + index,
-                                    stop_on_eos=stop_on_eos)
-            request = Request(id=("generate", index), prompt=[int(token) for token in prompt], params=params)
-            scheduler.add(request)
-            requests.append(request)
+            family = []
+            for answer in range(answers):
+                place = index * answers + answer
+                params = SamplingParams(max_tokens=max_tokens, temperature=temperature, top_p=top_p, seed=seed + place,
+                                        stop_on_eos=stop_on_eos, top_k=top_k, min_p=min_p, logprobs=logprobs is not None)
+                family.append(Request(id=("generate", place), prompt=[int(token) for token in prompt], params=params,
+                                      family=family if answers > 1 else None))
+            requests += family
+        for first in range(answers):                      # (each prompt's first answer before any second: it computes the prompt's keys)
+            for request in requests[first::answers]:
+                scheduler.add(request)
         try:
             self.run(scheduler, timings)
             if stats is not None:
@@ -161,7 +175,11 @@ class Engine:
                 if self.cache.is_live(request.id):
                     self.cache.release(request.id)
             raise
-        return [request.generated for request in requests]
+        def by_prompt(values: list) -> list:
+            return values if answers == 1 else [values[first:first + answers] for first in range(0, len(values), answers)]
+        if logprobs is not None:
+            logprobs[:] = by_prompt([request.logprobs for request in requests])
+        return by_prompt([request.generated for request in requests])
 
     def run(self, scheduler: Scheduler, timings: dict | None = None, max_steps: int | None = None) -> int:
         """The engine loop: plan a step, run it, sample, record; until nothing is left, or for
@@ -183,7 +201,7 @@ class Engine:
         def settle():
             nonlocal behind
             if behind is not None:
-                scheduler.resolve(behind[0], behind[1].read())
+                scheduler.resolve(behind[0], behind[1].read(), behind[1].read_logprobs())
                 behind = None
 
         try:
@@ -218,7 +236,7 @@ class Engine:
                     behind = (plan, pending, {item.request.id: row for row, item in enumerate(sampling)})
                     self.stats["steps_ahead"] += 1
                 else:
-                    scheduler.update(plan, pending.read())
+                    scheduler.update(plan, pending.read(), pending.read_logprobs())
         except BaseException:
             if behind is not None:
                 # the requests get the tokens that were sampled for them before the step that raised;
@@ -227,14 +245,14 @@ class Engine:
                 plan, pending, _ = behind
                 behind = None
                 try:
-                    scheduler.resolve(plan, pending.read())
+                    scheduler.resolve(plan, pending.read(), pending.read_logprobs())
                 except Exception:
                     pass
             raise
         if behind is not None:
             plan, pending, _ = behind
             behind = None
-            scheduler.resolve(plan, pending.read())
+            scheduler.resolve(plan, pending.read(), pending.read_logprobs())
         return steps
 
     def _device_sources(self, plan, behind):

@@ -27,6 +27,10 @@ prompts, cut into portions.  Pages are taken as a request grows, so they can run
     against the 107 thousand of an ample pool).  `admit_partial=True` admits as soon as a first
     portion fits.
 
+Requests of one family (`Request.family`: several answers to one prompt) share the prompt's pages where the cache can: a member is
+admitted as a fork of one that has the prompt's keys already, and waits while one is still computing them; all it brings then
+is the prompt's last token, whose logits its first token is drawn from.
+
 The scheduler owns no device memory and calls no kernel: it plans with the cache manager's
 counts, and the engine loop runs what it plans.
 """
@@ -43,12 +47,21 @@ from ..errors import invalid_argument, out_of_bounds, out_of_memory
 @dataclass
 class SamplingParams:
     """Names as the reference's request options (app/server.cpp:601-613): max_tokens,
-    temperature (0 = greedy), top_p in (0, 1]; the seed is the request's own."""
+    temperature (0 = greedy), top_p in (0, 1]; the seed is the request's own.  top_k (0: all) and min_p (0: none) narrow the
+    draw further (see `ops.sample_filtered`); logprobs: the request keeps its tokens' log-probabilities."""
     max_tokens: int = 16
     temperature: float = 0.0
     top_p: float = 1.0
     seed: int = 0
     stop_on_eos: bool = False
+    top_k: int = 0
+    min_p: float = 0.0
+    logprobs: bool = False
+
+    @property
+    def filtered(self) -> bool:
+        """Whether the row's draw is one that `ops.sample` does not make."""
+        return self.top_k > 0 or self.min_p > 0.0
 
     def validate(self) -> None:
         if self.max_tokens < 1:
@@ -57,6 +70,10 @@ class SamplingParams:
             raise invalid_argument("temperature must be >= 0")
         if not 0.0 < self.top_p <= 1.0:
             raise invalid_argument("top_p must be in (0, 1]")
+        if not 0 <= self.top_k < 1 << 31:
+            raise invalid_argument("top_k must be an integer >= 0")
+        if not 0.0 <= self.min_p <= 1.0:
+            raise invalid_argument("min_p must be in [0, 1]")
 
 
 PENDING = -1        # in a request's generated tokens: sampled, but not yet read from the device
@@ -68,6 +85,8 @@ class Request:
     prompt: list[int]
     params: SamplingParams
     generated: list[int] = field(default_factory=list)
+    logprobs: list[float] = field(default_factory=list)      # of the generated tokens, when the request asks for them
+    family: list | None = None        # the requests with this one's prompt, itself included: they may share its pages
     state: str = "waiting"            # waiting, running, finished
     finish_reason: str | None = None  # length, eos, aborted
     computed: int = 0                 # tokens of prompt + generated whose keys are in the cache
@@ -176,6 +195,10 @@ class Scheduler:
             if plan or len(self.running) <= 1:
                 break
             self._preempt(max(self.running, key=lambda candidate: candidate.order), [], [0] * len(self.cache.groups))
+        if any(item.request.family for item in plan):
+            # members of a family beside one another, where the first of them stands: what they share is read once for neighbours
+            place: dict = {}
+            plan.sort(key=lambda item: place.setdefault(id(item.request.family or item.request), len(place)))
         self.stats["steps"] += 1
         for item in plan:
             self.stats["decode_tokens" if item.count == 1 and item.first > 0 and item.samples else "prefill_tokens"] += item.count
@@ -238,13 +261,14 @@ class Scheduler:
         # 3. new requests, first come first served, while a slot, budget and pages allow
         while self.waiting and budget > 0 and len(plan) < self.max_seqs_per_step and self.cache.free_slots > 0:
             request = self.waiting[0]
-            self.cache.admit(request.id)
-            if self.running and not self.admit_partial and not self._fits_whole(request):
-                self.cache.release(request.id)
+            if not self._enter(request, planned_pages):
                 break
-            count = self._portion(request, budget, planned_pages)
+            count = 0
+            if not self.running or self.admit_partial or self._fits_whole(request):
+                count = self._portion(request, budget, planned_pages)
             if count <= 0:
                 self.cache.release(request.id)
+                request.computed = 0
                 break
             self.waiting.popleft()
             request.state = "running"
@@ -253,6 +277,21 @@ class Scheduler:
             self.running.append(request)
             take(request, count)
         return plan
+
+    def _enter(self, request: Request, planned_pages: list[int]) -> bool:
+        """Gives a waiting request its slot, as a fork of a member of its family where that has the prompt's keys.  False: it waits, for a
+        member that is still computing them, or for a page."""
+        base = len(request.prompt) - 1            # (the last token runs again: its logits are asked for)
+        members = [member for member in request.family or () if member is not request and member.state == "running"]
+        if not members or base < self.cache.page_size or not self.cache.can_fork:
+            self.cache.admit(request.id)
+            return True
+        source = next((member for member in members if self.cache.length(member.id) >= base), None)
+        if source is None or any(free <= planned for free, planned in zip(self.cache.free_pages(), planned_pages)):
+            return False
+        self.cache.fork(source.id, request.id, base)
+        request.computed = base
+        return True
 
     def _fits_whole(self, request: Request) -> bool:
         """Whether the pools have room for all of the (just admitted) request's tokens after what the
@@ -300,9 +339,9 @@ class Scheduler:
         return removed
 
     # ---- after the step ----------------------------------------------------------------------------
-    def update(self, plan: list[Scheduled], sampled: list[int] | None) -> list[Request]:
-        """`sampled` holds one token for each planned item with `samples`, in plan order.
-        Returns the requests that finished.
+    def update(self, plan: list[Scheduled], sampled: list[int] | None, logprobs: list[float] | None = None) -> list[Request]:
+        """`sampled` holds one token for each planned item with `samples`, in plan order, `logprobs` (if there are any) its
+        log-probability.  Returns the requests that finished.
 
         `sampled` may be None when the tokens are not on the host yet: PENDING stands in their
         place, and `resolve` writes them later.  Everything a plan depends on is known without
@@ -316,6 +355,8 @@ class Scheduler:
             if not item.samples:
                 continue
             token = PENDING if sampled is None else int(sampled[cursor])
+            if request.params.logprobs and sampled is not None:
+                request.logprobs.append(logprobs[cursor])
             cursor += 1
             request.generated.append(token)
             if len(request.generated) >= request.params.max_tokens:
@@ -332,7 +373,7 @@ class Scheduler:
         return all(not item.request.params.stop_on_eos for item in plan if item.samples)
 
     @staticmethod
-    def resolve(plan: list[Scheduled], sampled: list[int]) -> None:
+    def resolve(plan: list[Scheduled], sampled: list[int], logprobs: list[float] | None = None) -> None:
         """The tokens of a plan that `update` took without them.  Item i's token is the one it
         appended: at index first + count - len(prompt) of the request's generated tokens."""
         cursor = 0
@@ -344,6 +385,8 @@ class Scheduler:
             if not (0 <= index < len(request.generated)) or request.generated[index] != PENDING:
                 raise invalid_argument(f"request {request.id!r} has no token pending at {index}")
             request.generated[index] = int(sampled[cursor])
+            if request.params.logprobs:
+                request.logprobs.append(logprobs[cursor])
             cursor += 1
 
     def _finish(self, request: Request, reason: str) -> None:

@@ -19,7 +19,9 @@ import numpy as np
 import torch
 
 from ..cache.manager import ABSENT, CacheManager
+from ..ops import RecordedPrefixPlan as ops_RecordedPrefixPlan
 from ..ops import feed_tokens as ops_feed_tokens
+from ..ops import shared_prefix_pays as ops_shared_prefix_pays
 from ..errors import invalid_argument, out_of_bounds, out_of_memory
 
 
@@ -85,6 +87,11 @@ class StepContext:
     host: dict                     # the same arrays as numpy, by name
     wants_all_rows: bool = False   # the wanted rows are all the step's tokens, in order
     compute_units: int = 256       # of the device: how many workgroups start at once
+    # groups (first sequence, sequences, prefix) of the step's sequences that hold the same pages for their first positions, where reading
+    # those once pays; parts that can do so (`takes_shared_prefix`) ask `ops.step_prefix_plan` for the step's work.  prefix_owner: in a
+    # recorded step, whoever keeps that plan at fixed addresses
+    shared: list = field(default_factory=list)
+    prefix_owner: object = None
     # int32 [S], a step of single tokens (see `orders_sequences`): its sequences, longest first; None: any order will do
     seq_order: torch.Tensor | None = None
     # a recorded step of prompt portions: work lists that parts make on the host live at fixed
@@ -118,6 +125,9 @@ class ModelRunner:
         # capture=False: the steps a recording would serve are still padded to its sizes and run on
         # its fixed arrays, but launched kernel by kernel every time (what a replay must equal bit for bit)
         self.capture = capture
+        mixers = [block.mixer for block in getattr(model, "blocks", ())]
+        self._prefix_sizes = {(mixer.nkv, mixer.d) for mixer in mixers if getattr(mixer, "takes_shared_prefix", False)}
+        self._shared_graphs: dict[tuple[int, int], "SharedDecodeGraph"] = {}   # of steps whose sequences share prefixes
         self.device_tokens: torch.Tensor | None = None     # int32, where sampling leaves a step's tokens (set by the engine)
         self._graphs: dict[tuple[int, int], "DecodeGraph"] = {}      # by (most sequences, longest sequence)
         self._portion_graphs: dict[tuple[int, int, int], "PortionGraph"] = {}   # by (most tokens, most sequences, longest sequence)
@@ -150,6 +160,20 @@ class ModelRunner:
 
     def build_context(self, entries: Sequence[StepEntry]) -> StepContext:
         return build_context(self.cache, entries, self.device)
+
+    def shared_groups(self, entries: Sequence[StepEntry]) -> list[tuple[int, int, int]]:
+        """The step's groups (first sequence, sequences, prefix) of neighbouring entries that hold the same pages, when reading those
+        pages once for all of them pays; else none."""
+        if not self._prefix_sizes or len(entries) < 2 or self.cache.page_size < 16:
+            return []
+        groups, held = [], [self.cache.held(entry.request) for entry in entries]
+        first = 0
+        for index in range(1, len(held) + 1):
+            if index == len(held) or held[index].family != held[first].family or not held[first].family:
+                if index - first > 1:
+                    groups.append((first, index - first, min(info.shared for info in held[first:index])))
+                first = index
+        return groups if groups and any(ops_shared_prefix_pays(groups, *sizes) for sizes in self._prefix_sizes) else []
 
     def _length_bucket(self, longest: int) -> int:
         """The sequence length a recording is made for: the next power of two from 256 on, up to
@@ -211,7 +235,17 @@ class ModelRunner:
         try:
             if marks:
                 marks[0].record()
-            if trace is None and self.replays(entries):
+            shared = self.shared_groups(entries)
+            if trace is None and shared and self.replays(entries):
+                longest = max(self.cache.length(request) + count for request, count in wanted)
+                key = (DecodeGraph.bucket_of(len(entries)), self._length_bucket(longest))
+                if key not in self._shared_graphs:
+                    self._shared_graphs[key] = SharedDecodeGraph(self, *key)
+                self._shared_graphs[key].shared = shared
+                logits = self._shared_graphs[key].run(entries, marks[1] if marks else None)
+                if keep:
+                    logits = logits.clone()
+            elif trace is None and self.replays(entries):
                 longest = max(self.cache.length(request) + count for request, count in wanted)
                 key = (DecodeGraph.bucket_of(len(entries)), self._length_bucket(longest))
                 if key not in self._graphs:
@@ -219,7 +253,7 @@ class ModelRunner:
                 logits = self._graphs[key].run(entries, marks[1] if marks else None)
                 if keep:
                     logits = logits.clone()
-            elif trace is None and (sizes := self.records(entries)) is not None:
+            elif trace is None and not shared and (sizes := self.records(entries)) is not None:
                 longest = max(self.cache.length(request) + count for request, count in wanted)
                 key = (*sizes, self._length_bucket(longest))
                 if key not in self._portion_graphs:
@@ -231,6 +265,7 @@ class ModelRunner:
                 if any(entry.source is not None for entry in entries):
                     raise invalid_argument("a token that is still on the device can only feed a replayed decode step")
                 ctx = self.build_context(entries)
+                ctx.shared = shared
                 ctx.trace = trace
                 ctx.trace_serving_route = trace_serving_route
                 if marks:
@@ -247,7 +282,7 @@ class ModelRunner:
             # their committed positions lie on), so that a later step finds the lists it expects
             for request, _ in wanted:
                 self.cache.unreserve(request)
-            for recording in (*self._graphs.values(), *self._portion_graphs.values()):
+            for recording in (*self._graphs.values(), *self._shared_graphs.values(), *self._portion_graphs.values()):
                 recording.forget()                      # (a page list that shrank and grew again is not the list a row remembers)
             raise
         for request, count in wanted:
@@ -443,6 +478,34 @@ class DecodeGraph:
 
     def _send_lists(self) -> None:
         """Work lists that depend on how the step is cut (a decode step has none)."""
+
+
+class SharedDecodeGraph(DecodeGraph):
+    """A recorded decode step whose sequences share prefixes (`shared`: the step's groups): the plan of the attention that reads them
+    once has a fixed size too, and is filled again before every replay."""
+
+    def __init__(self, runner: "ModelRunner", bucket: int, longest: int):
+        super().__init__(runner, bucket, longest)
+        self.shared: list = []
+        self._plans: dict = {}            # by sizes
+        self.ctx.shared, self.ctx.prefix_owner = [(0, 0, 0)], self     # (not empty; what it holds is the plans')
+
+    def prefix_plan(self, num_heads: int, num_kv_heads: int, head_dim: int, dtype):
+        key = (num_heads, num_kv_heads, head_dim, dtype)
+        if key not in self._plans:
+            if torch.cuda.is_current_stream_capturing():
+                raise invalid_argument("a plan first asked for inside a recording")
+            self._plans[key] = ops_RecordedPrefixPlan(self.bucket, self.longest, *key, self.device_flat.device)
+            self._fill_plan(self._plans[key])
+        return self._plans[key].plan
+
+    def _fill_plan(self, plan) -> None:
+        live = self._rows_filled
+        plan.fill(self.host["seq_start"][:live + 1], self.host["seq_len"][:live], self.shared)
+
+    def _send_lists(self) -> None:
+        for plan in self._plans.values():
+            self._fill_plan(plan)
 
 
 class PortionGraph(DecodeGraph):

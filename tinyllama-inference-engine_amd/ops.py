@@ -2782,8 +2782,10 @@ def prefix_part_cost(total: float, compute_units: int) -> float:
     return max(total / (2 * compute_units), min(total / compute_units, 2600.0))
 
 
-def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, compute_units: int = 256):
-    """The host's half of `shared_prefix_plan`: (items [n, 8], part_first [tokens + 1]), int32 arrays of numpy."""
+def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, compute_units: int = 256,
+                        most_parts: int = PREFIX_PARTS):
+    """The host's half of `shared_prefix_plan`: (items [n, 8], part_first [tokens + 1]), int32 arrays of numpy.  most_parts: a limit to
+    the parts that a prefix, and a sequence's own keys, are cut into."""
     import numpy as np
     seq_start, seq_len = np.asarray(seq_start, dtype=np.int64), np.asarray(seq_len, dtype=np.int64)
     if seq_start.ndim != 1 or seq_len.ndim != 1 or seq_start.shape[0] != seq_len.shape[0] + 1:
@@ -2844,7 +2846,7 @@ def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads
     for which in np.unique(key):
         mine = key == which
         width, longest = int(rows[mine, 7].max()), int(lengths[mine].max())
-        count = max(1, min(-(-longest // PREFIX_LEAST), int(round(longest * PREFIX_COST[width] / max(budget, 1.0))), PREFIX_PARTS))
+        count = max(1, min(-(-longest // PREFIX_LEAST), int(round(longest * PREFIX_COST[width] / max(budget, 1.0))), most_parts))
         part[mine] = -(-(-(-longest // count)) // 32) * 32
     cuts = -(-lengths // part)
     index = np.repeat(np.arange(rows.shape[0]), cuts)
@@ -2883,6 +2885,58 @@ def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads:
     longest = max((int(length) for length in seq_len), default=0)
     return SharedPrefixPlan(torch.from_numpy(items).to(device), torch.from_numpy(part_first).to(device), part_first.shape[0] - 1, int(part_first[-1]),
                             len(seq_len), longest, (num_heads, num_kv_heads, head_dim, dtype))
+
+
+def shared_prefix_pays(groups, num_kv_heads: int, head_dim: int) -> bool:
+    """Whether a decode step of these groups is faster through `attention_shared_prefix` than through `attention_mfma`: from four million
+    elements of keys on that are not read again (32 heads of 64 on 4, 64 sequences behind 1024 positions 13.4 us against 12.5, behind 2048 16.1 against 18.4;
+    of 128 on 8, 2 behind 1024 10.5 and 10.4, 8 behind 1024 10.0 against 13.6, 64 behind 2048 20.6 against 56.7; on 32, 4 behind 256 10.5 and 10.3)."""
+    return sum((count - 1) * prefix for _, count, prefix in groups) * num_kv_heads * head_dim >= 4_000_000
+
+
+class RecordedPrefixPlan:
+    """A `SharedPrefixPlan` at fixed addresses and of fixed size, for a recorded step of up to `tokens` single tokens: `fill` writes a
+    step's work into it.  Items and parts beyond the step's have no tokens."""
+
+    def __init__(self, tokens: int, longest: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device):
+        group, step = num_heads // num_kv_heads, prefix_tile_columns(17, head_dim, dtype)
+        # with one part each, a token has ceil(G / step) items of its own and the groups ceil(columns / step) each; room for parts beside
+        self.items = tokens * -(-group // step) + -(-tokens * group // step) + tokens // 2 + 64
+        self.parts = tokens * 24 + 256
+        self._host = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, pin_memory=True)
+        self._device = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, device=device)
+        self.plan = SharedPrefixPlan(self._device[:self.items * 8].view(self.items, 8), self._device[self.items * 8:], tokens, self.parts, tokens,
+                                     longest, (num_heads, num_kv_heads, head_dim, dtype))
+
+    def fill(self, seq_start, seq_len, groups) -> None:
+        num_heads, num_kv_heads, head_dim, dtype = self.plan.sizes
+        most = PREFIX_PARTS
+        while True:
+            items, part_first = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype,
+                                                    _compute_units(self._device.device), most)
+            if items.shape[0] <= self.items and int(part_first[-1]) <= self.parts:
+                break
+            if most == 1:
+                raise invalid_shape("a recorded step's shared prefixes do not fit its plan")
+            most //= 2
+        host, begin = self._host.numpy(), self.items * 8
+        host[:items.size] = items.ravel()
+        host[items.size:begin] = 0
+        host[begin:begin + part_first.shape[0]] = part_first
+        host[begin + part_first.shape[0]:] = part_first[-1]
+        self._device.copy_(self._host, non_blocking=True)
+
+
+def step_prefix_plan(ctx, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype) -> SharedPrefixPlan:
+    """The plan of the step that `ctx` describes (whose `shared` is not empty), for layers of these sizes: made once, kept in `ctx.scratch`."""
+    key = ("shared_prefix", num_heads, num_kv_heads, head_dim, dtype)
+    if key not in ctx.scratch:
+        if ctx.prefix_owner is not None:
+            ctx.scratch[key] = ctx.prefix_owner.prefix_plan(num_heads, num_kv_heads, head_dim, dtype)
+        else:
+            ctx.scratch[key] = shared_prefix_plan(ctx.host["seq_start"], ctx.host["seq_len"], ctx.shared, num_heads, num_kv_heads, head_dim, dtype,
+                                                  ctx.tokens.device)
+    return ctx.scratch[key]
 
 
 def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, plan: SharedPrefixPlan,

@@ -222,6 +222,16 @@ class Attention(Mixer):
             return None
         return StateNeed((ops.short_conv_state_floats((self.nq + self.nkv) * self.d + self.nkv * self.dv, self.taps),), torch.float32)
 
+    @property
+    def takes_shared_prefix(self) -> bool:
+        """Whether the layer's attention may read what sequences of a step have in common once for all of them (`ops.attention_shared_prefix`)."""
+        return self.dv == self.d and self.window is None and self.chunk is None and self.d % 16 == 0
+
+    def _attend_shared(self, q, ctx, pages, binding):
+        plan = ops.step_prefix_plan(ctx, self.nq, self.nkv, self.d, self.dtype)
+        return ops.attention_shared_prefix(q, binding.cache, pages.block_table, ctx.positions, plan, self.nq, self.nkv, self.d, self.scale,
+                                           softcap=self.softcap, sink=self.sink)
+
     def _place_by_conv(self, fused, ctx, pages, binding, inv_freq, rot_dim):
         norm = "rms" if self.qk_norm == "head" else None
         segments = [ops.ConvSegment(self.nq * self.d, self.d, norm, self.q_norm, self.norm_eps, rotated=inv_freq is not None),
@@ -254,7 +264,9 @@ class Attention(Mixer):
                           rot_dim, binding.cache, self.nq, 0 if self.reads_other_cache else self.nkv, self.d, self.dv, self.dtype,
                           q_norm=self.q_norm, k_norm=self.k_norm, norm_eps=self.norm_eps, values_are_keys=self.values_are_keys,
                           q_temp=self.q_temp, head_scale=self.temp, extra_cols=self.gate_cols)
-        if self.dv == self.d and ops.attention_mfma_takes(self.dtype, self.d, binding.cache.shape[3] // self.d):
+        if ctx.shared and self.takes_shared_prefix:
+            attended = self._attend_shared(q, ctx, pages, binding)
+        elif self.dv == self.d and ops.attention_mfma_takes(self.dtype, self.d, binding.cache.shape[3] // self.d):
             # bfloat16, one head size: the kernel on the matrix cores (scores, softmax and sink float)
             extra = self.chunk is not None or self.sink is not None or self.softcap is not None
             tiles, col_tiles, nsplit, split_len, waves, shared = ops.attention_plan(ctx, self.nq // self.nkv, self.nkv, self.d, self.reach, extra)
@@ -293,7 +305,9 @@ class Attention(Mixer):
             q = ops.rope_cache(q, ctx.positions, slot_map, inv_freq, rot_dim, binding.cache, self.nq, self.nkv, self.d,
                                self.dtype, paired=self.paired, extra_cols=self.gate_cols, head_scale=self.temp, runs=ops.slots_follow(ctx))
         page_size = binding.cache.shape[3] // self.d
-        if ops.attention_mfma_takes(self.dtype, self.d, page_size):
+        if ctx.shared and self.takes_shared_prefix:
+            attended = self._attend_shared(q, ctx, pages, binding)
+        elif ops.attention_mfma_takes(self.dtype, self.d, page_size):
             tiles, col_tiles, nsplit, split_len, waves, shared = ops.attention_plan(ctx, self.nq // self.nkv, self.nkv, self.d, self.reach)
             attended = ops.attention_mfma(q, binding.cache, pages.block_table, tiles, ctx.positions, self.nq, self.nkv,
                                           self.d, self.window, self.scale, nsplit, split_len, col_tiles, waves, shared, order=ctx.seq_order)
