@@ -163,9 +163,9 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
           }
         }
       }
+    settle(s);                                            // (branches follow, behind which the scores are read)
     if (cap_pre > 0.f) {
       // cap * tanh(s * scale / cap) = cap * (1 - 2 / (2^(2 log2(e) s scale / cap) + 1)); the cap is part of scale_log2
-      settle(s);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -177,7 +177,6 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
           }
     }
     if (ragged) {
-      settle(s);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -454,6 +453,7 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
       const Half a = *reinterpret_cast<const Half*>(place), b = *reinterpret_cast<const Half*>(place + D * 32);
       values[dt] = Piece{a[0], a[1], b[0], b[1]};
     }
+    settle(s);                                               // (branches follow, behind which the scores are read)
     if (ragged) {
       uint32_t keep[4];
 #pragma unroll
@@ -467,7 +467,6 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
         for (int w = 0; w < 4; ++w) values[dt][w] &= keep[w];
     }
     if (cap_pre > 0.f) {
-      settle(s);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -477,7 +476,6 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
             s[ct][t][j] = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[ct][t][j] * (cap_pre * 2.8853900817779268f)) + 1.f);
     }
     if (ragged) {
-      settle(s);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
