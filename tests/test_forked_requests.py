@@ -1,7 +1,9 @@
 """Requests that share their first positions' pages: the allocator's holders, forks in the cache manager, and families in the
 scheduler, on the host."""
 import random
+from types import SimpleNamespace
 
+import numpy as np
 import pytest
 import torch
 
@@ -195,3 +197,28 @@ def test_the_numbers_of_many_rows_are_the_numbers_of_each():
     rng = random.Random(0)
     seeds, counters = [rng.randrange(-2 ** 63, 2 ** 64) for _ in range(100)], [rng.randrange(1 << 20) for _ in range(100)]
     assert uniforms01(seeds, counters).tolist() == [uniform01(seed, counter) for seed, counter in zip(seeds, counters)]
+
+
+def test_a_family_of_two_prompts_is_refused():
+    cache = manager()
+    scheduler = Scheduler(cache, max_tokens_per_step=64)
+    family = family_of(2, range(1, 12), max_tokens=2)
+    family[1].prompt[3] = 40
+    scheduler.add(family[0])
+    with pytest.raises(EngineError):
+        scheduler.add(family[1])
+
+
+def test_a_plan_made_within_a_step_is_waited_for_by_the_next(monkeypatch):
+    """The host's buffer of a recorded plan is written again only behind the event that stands after its last transfer."""
+    from tlie_amd.engine import step
+    log = []
+    monkeypatch.setattr(step, "ops_RecordedPrefixPlan", lambda *sizes: SimpleNamespace(plan="plan", fill=lambda *work: log.append("fill")))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    graph = step.SharedDecodeGraph.__new__(step.SharedDecodeGraph)
+    graph.bucket, graph.longest, graph._plans, graph.shared, graph._rows_filled = 4, 256, {}, [(0, 2, 64)], 2
+    graph.host = {"seq_start": np.arange(5), "seq_len": np.array([70, 71, 1, 1])}
+    graph.device_flat, graph.copied = torch.zeros(1), SimpleNamespace(record=lambda: log.append("record"))
+    assert graph.prefix_plan(8, 2, 64, torch.bfloat16) == "plan"
+    assert log == ["fill", "record"]
+    assert graph.prefix_plan(8, 2, 64, torch.bfloat16) == "plan" and log == ["fill", "record"]

@@ -86,7 +86,8 @@ class Request:
     params: SamplingParams
     generated: list[int] = field(default_factory=list)
     logprobs: list[float] = field(default_factory=list)      # of the generated tokens, when the request asks for them
-    family: list | None = None        # the requests with this one's prompt, itself included: they may share its pages
+    # the requests with this one's prompt, itself included: they may share its pages
+    family: list | None = field(default=None, repr=False, compare=False)
     state: str = "waiting"            # waiting, running, finished
     finish_reason: str | None = None  # length, eos, aborted
     computed: int = 0                 # tokens of prompt + generated whose keys are in the cache
@@ -164,6 +165,8 @@ class Scheduler:
         request.params.validate()
         if not request.prompt:
             raise invalid_argument("a request needs a prompt of at least one token")
+        if request.family and request.family[0].prompt != request.prompt:
+            raise invalid_argument("requests of one family have one prompt")
         total = len(request.prompt) + request.params.max_tokens
         # the last sampled token is never fed back, so it needs no position
         if self.max_positions is not None and total > self.max_positions:

@@ -164,7 +164,7 @@ class ModelRunner:
     def shared_groups(self, entries: Sequence[StepEntry]) -> list[tuple[int, int, int]]:
         """The step's groups (first sequence, sequences, prefix) of neighbouring entries that hold the same pages, when reading those
         pages once for all of them pays; else none."""
-        if not self._prefix_sizes or len(entries) < 2 or self.cache.page_size < 16:
+        if not self._prefix_sizes or len(entries) < 2 or not 16 <= self.cache.page_size <= 65536:
             return []
         groups, held = [], [self.cache.held(entry.request) for entry in entries]
         first = 0
@@ -497,6 +497,7 @@ class SharedDecodeGraph(DecodeGraph):
                 raise invalid_argument("a plan first asked for inside a recording")
             self._plans[key] = ops_RecordedPrefixPlan(self.bucket, self.longest, *key, self.device_flat.device)
             self._fill_plan(self._plans[key])
+            self.copied.record()                             # (the next step's plan waits for this transfer too)
         return self._plans[key].plan
 
     def _fill_plan(self, plan) -> None:
