@@ -198,3 +198,65 @@ def test_refusals_and_no_rows():
     for change in bad:
         with pytest.raises(EngineError):
             ops.sample_filtered(**{"logits": logits, "uniform": uniform, **change})
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 60000), (20, 3000)])
+def test_two_calls_at_once_and_replays_beside_eager_calls(rows, vocab):
+    """Both forms (a row in parts, a row by one workgroup) on two streams, and in a recording with eager calls between its replays."""
+    logits, uniform, gen = rows_of(11, rows, vocab)
+    filters = {name: value.to(DEV) for name, value in filters_of(gen, rows).items()}
+    logits, uniform = logits.to(DEV), uniform.to(DEV)
+    inputs = [(logits, uniform), (logits.flip(0).contiguous(), uniform.flip(0).contiguous())]
+    run = lambda i: ops.sample_filtered(*inputs[i], **filters, logprobs=True)
+    want = [run(0), run(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for tokens, logprobs in got[i]:
+            assert torch.equal(tokens, want[i][0]) and torch.equal(logprobs, want[i][1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = run(0)
+    for _ in range(4):
+        uniform.copy_(torch.rand((rows,), generator=gen).to(DEV))
+        graph.replay()
+        replayed = [value.clone() for value in recorded]
+        run(1)
+        eager = run(0)
+        assert torch.equal(replayed[0], eager[0]) and torch.equal(replayed[1], eager[1])
+
+
+def test_rows_that_start_anywhere():
+    """Rows of a vocabulary that is no multiple of four, in a tensor that itself starts past such a place."""
+    for offset in (1, 2, 3):
+        logits, uniform, gen = rows_of(12 + offset, 5, 30001)
+        filters = {name: value.to(DEV) for name, value in filters_of(gen, 5).items()}
+        shifted = torch.cat([torch.full((offset,), math.inf), logits.flatten(), torch.full((3,), math.inf)]).to(DEV)[offset:offset + logits.numel()].view(logits.shape)
+        want = ops.sample_filtered(logits.to(DEV), uniform.to(DEV), **filters, logprobs=True)
+        got = ops.sample_filtered(shifted, uniform.to(DEV), **filters, logprobs=True)
+        assert torch.equal(got[0], want[0])
+        check(logits, uniform, **{name: value.cpu() for name, value in filters.items()})
+
+
+def test_more_logits_than_32_bits_count():
+    """Rows past the 2^31st element (8.6 GB): the last rows draw what they draw alone."""
+    rows, vocab = 65535, 32800
+    logits = torch.zeros((rows, vocab), device=DEV)
+    few, uniform, gen = rows_of(16, 8, vocab)
+    filters = {name: value.to(DEV) for name, value in filters_of(gen, 8).items()}
+    logits[-8:] = few.to(DEV)
+    numbers = torch.zeros(rows, device=DEV)
+    numbers[-8:] = uniform.to(DEV)
+    spread = {"temperature": torch.zeros(rows, device=DEV), "top_k": torch.zeros(rows, dtype=torch.int32, device=DEV),
+              "top_p": torch.ones(rows, device=DEV), "min_p": torch.zeros(rows, device=DEV)}
+    for name, value in spread.items():
+        value[-8:] = filters[name]
+    got = ops.sample_filtered(logits, numbers, **spread)
+    assert torch.equal(got[-8:], ops.sample_filtered(few.to(DEV), uniform.to(DEV), **filters))
+    assert not got[:-8].any()

@@ -231,3 +231,61 @@ def test_refusals(change):
         q = torch.cat([q, q], dim=1)[:, :512]
     with pytest.raises(EngineError):
         ops.attention_shared_prefix(q, cache, table, positions, plan, heads, 2, dim, scale, softcap=softcap, sink=sink)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,lengths,prefix", [(4, [49, 81, 50, 17], 48), (40, [49, 81, 50, 17], 47), (64, [65, 97, 66, 1], 64)])
+def test_table_entries_of_no_use_are_not_followed(dtype, heads, lengths, prefix):
+    """Entries that none of a row's own positions lie on (behind its end, and in the group's other rows the shared blocks) are -1: the
+    page before the cache's first, which the buffer around it holds here, with NaN.  Prefixes and ends lie on odd pages of 16 rows, in the middle
+    of a block of 32 keys."""
+    step = make_step(12, dtype, heads, 2, 64, 16, [(length, 1) for length in lengths], [(0, 3, prefix)])
+    want, bound = oracle(step)
+    for row, length in enumerate(lengths):
+        step["table"][row, (length + 15) // 16:] = -1
+        if row in (1, 2):
+            step["table"][row, :prefix // 16] = -1
+    around = torch.cat([torch.full_like(step["cache"][:1], math.nan), step["cache"]]).to(DEV)
+    step["cache"] = around[1:]
+    excess = (call(step).double().cpu() - want).abs() - bound
+    assert float(excess.max()) <= 0.0
+
+
+def test_two_calls_at_once():
+    """On two streams, each with its own scratch: both have the results that each has alone."""
+    steps = [make_step(13 + i, BF16, 32, 4, 64, 16, [(900 + 40 * i + j, 1) for j in range(8)], [(0, 8, 890)]) for i in range(2)]
+    on = [{name: step[name].to(DEV) for name in ("q", "cache", "table", "positions")} for step in steps]
+    plans = [ops.shared_prefix_plan(step["start"], step["lengths"], step["groups"], 32, 4, 64, BF16, DEV) for step in steps]
+    run = lambda i: ops.attention_shared_prefix(on[i]["q"], on[i]["cache"], on[i]["table"], on[i]["positions"], plans[i], 32, 4, 64, 0.125)
+    want = [run(0), run(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(one, want[i]) for one in got[i])
+
+
+def test_starts_that_are_not_aligned_are_refused():
+    step = make_step(15, BF16, 8, 2, 64, 16, [(50, 1), (60, 1)], [(0, 2, 40)])
+    plan = ops.shared_prefix_plan(step["start"], step["lengths"], step["groups"], 8, 2, 64, BF16, DEV)
+    q, cache, table, positions = (step[name].to(DEV) for name in ("q", "cache", "table", "positions"))
+    shifted = lambda tensor: torch.cat([tensor.flatten()[:1], tensor.flatten()])[1:].view(tensor.shape)
+    ops.attention_shared_prefix(q, cache, table, positions, plan, 8, 2, 64, 0.125)
+    for first, second in ((shifted(q), cache), (q, shifted(cache))):
+        with pytest.raises(EngineError):
+            ops.attention_shared_prefix(first, second, table, positions, plan, 8, 2, 64, 0.125)
+    for scale, softcap in ((1e-60, None), (math.inf, None), (1.0, 1e-60), (1.0, math.inf), (1e30, 1e-30), (math.nan, None), (1.0, math.nan)):
+        with pytest.raises(EngineError):
+            ops.attention_shared_prefix(q, cache, table, positions, plan, 8, 2, 64, scale, softcap=softcap)
+
+
+def test_a_longer_table_of_small_pages_than_a_window_holds():
+    """A walk over more than 128 pages, parts that begin on odd pages, and one token alone."""
+    check(make_step(16, BF16, 4, 1, 64, 16, [(4500, 1), (4490, 1)], [(0, 2, 4400)]))
+    check(make_step(17, BF16, 24, 1, 64, 16, [(4500, 1), (4490, 1)], [(0, 2, 4400)]))
+    check(make_step(18, F32, 4, 1, 32, 16, [(4500, 1)], []))

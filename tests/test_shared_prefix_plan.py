@@ -72,10 +72,16 @@ def test_every_key_of_every_column_is_in_one_item(heads, kv_heads, dim, dtype):
     ([0, 1, 2], [9, 9], [(0, 0, 4)], 8),           # a group of none
     ([0, 1, 2], [9, 9], [(0, 2, -1)], 8),          # a negative prefix
     ([0, 1, 2], [9, 9], [], 9),                    # heads that do not share kv heads evenly
+    ([0, 1], [(1 << 30) + 1], [], 8),              # positions whose blocks a kernel cannot count in 32 bits
 ])
 def test_plans_that_are_refused(start, lengths, groups, heads):
     with pytest.raises(EngineError):
         ops.shared_prefix_plan(start, lengths, groups, heads, 4, 64, torch.bfloat16, "cpu")
+
+
+def test_a_prefix_is_read_through_a_sequence_that_holds_it():
+    items, part_first = ops.shared_prefix_items([0, 0, 1, 2], [3, 9, 12], [(0, 3, 4)], 8, 4, 64, torch.bfloat16)
+    assert items[items[:, 6] == 0][:, 0].tolist() == [1] and part_first.tolist() == [0, 2, 4]
 
 
 def test_other_types_are_refused():

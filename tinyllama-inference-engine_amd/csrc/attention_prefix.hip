@@ -102,13 +102,15 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
     Piece k[TILES][KS];
     Values v[DT][TILES];
   };
-  // Rows outside the item's keys are read with the others (their page is in the table, or page 0 stands there) and masked.
+  // Rows of a page outside the item's keys are read with the others and masked; pages that hold none of them are not: the first or
+  // last page of the keys is read again in their place, whatever the table says there.
   TableWindow window;
+  const int page_lo = item.key_lo >> page_shift, page_hi = (item.key_hi - 1) >> page_shift;
   auto load = [&](int kb, Block& block) {
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
       const int first = kb + t * 16;
-      const int page = window.page(first >> page_shift);
+      const int page = window.page(min(max(first >> page_shift, page_lo), page_hi));
       const Elem* keys = k_base + (static_cast<size_t>(page) * page_stride + (first & page_mask)) * D;
       const Elem* values = v_base + static_cast<size_t>(page) * page_stride * D + (first & page_mask);
 #pragma unroll
@@ -395,9 +397,10 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
   auto to_of = [&](int i) { return kAlike ? to[i >> 1] + (i & 1) * (kBytes / 2) : to[i]; };
   Piece staged[2][kCalls];
   TableWindow window;
+  const int page_lo = item.key_lo >> page_shift, page_hi = (item.key_hi - 1) >> page_shift;       // (as above: other entries of the table are not followed)
   auto bring = [&](int kb, Piece (&into)[kCalls]) {
-    const size_t at_a = static_cast<size_t>(window.page(kb >> page_shift)) * page_stride * D;
-    const size_t at_b = static_cast<size_t>(window.page((kb + 16) >> page_shift)) * page_stride * D;
+    const size_t at_a = static_cast<size_t>(window.page(max(kb >> page_shift, page_lo))) * page_stride * D;
+    const size_t at_b = static_cast<size_t>(window.page(min(max((kb + 16) >> page_shift, page_lo), page_hi))) * page_stride * D;
     const int row_a = kb & page_mask, row_b = (kb + 16) & page_mask;
     const uint16_t *keys_a = k_base + at_a + row_a * D, *keys_b = k_base + at_b + row_b * D;
     const uint16_t *values_a = v_base + at_a + row_a, *values_b = v_base + at_b + row_b;
@@ -703,11 +706,14 @@ extern "C" int tlie_attention_prefix(const void* q, const void* cache, int dtype
                                      int num_items, const int* positions, const int* part_first, float* part_o, float* part_ml,
                                      const float* sink, void* out, int tokens, int nq, int nkv, int d, int page_size, float scale,
                                      float softcap, void* stream) {
-  if (tokens <= 0 || num_items <= 0 || nq <= 0 || nkv <= 0 || nq % nkv != 0 || d <= 0 || d > 256 || d % 16 != 0 || page_size < 16 ||
+  // (a grid has fewer than 2^32 threads; the kernels read and write 16 bytes at a time)
+  if (tokens <= 0 || num_items <= 0 || nq <= 0 || nkv <= 0 || nq % nkv != 0 || d <= 0 || d > 256 || d % 16 != 0 || page_size < 16 || page_size > 65536 ||
       (page_size & (page_size - 1)) != 0 || max_blocks <= 0 || !(scale > 0.f) || !(softcap >= 0.f) || (dtype != kF32 && dtype != kBF16) ||
-      static_cast<long long>(num_items) * nkv > 0x7fffffffll || static_cast<long long>(tokens) * nq > 0x7ffffffcll)
+      static_cast<long long>(num_items) * nkv >= 1ll << 24 || static_cast<long long>(tokens) * nq >= 1ll << 26 ||
+      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(part_o)) & 15) != 0)
     return kBadArgument;
   const float scale_log2 = (softcap > 0.f ? softcap : scale) * 1.4426950408889634f, cap_pre = softcap > 0.f ? scale / softcap : 0.f;
+  if (!(scale_log2 < INFINITY) || !(cap_pre < INFINITY) || (softcap > 0.f && !(cap_pre > 0.f))) return kBadArgument;
   const int page_shift = 31 - __builtin_clz(page_size);
   hipStream_t s = (hipStream_t)stream;
   int status = kBadArgument;

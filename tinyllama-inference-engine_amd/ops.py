@@ -2806,7 +2806,8 @@ def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads
         if ((seq_len[members] - counts[members] < prefix) & (counts[members] > 0)).any():
             raise invalid_argument("shared_prefix_plan: a group's tokens stand behind its prefix")
         if prefix > 0 and seq_start[first + count] > seq_start[first]:
-            shared.append((first, count, prefix))
+            # (a sequence that brings no tokens may be shorter than the prefix: the first that brings some holds it)
+            shared.append((first, count, prefix, first + int(np.nonzero(counts[members])[0][0])))
             prefix_of[members] = prefix
 
     def tiles(tokens: int):
@@ -2820,11 +2821,11 @@ def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads
 
     # (sequence, first token, tokens, first column, first key, end of the keys, own, width)
     rows = []
-    for first, count, prefix in shared:
+    for first, count, prefix, reader in shared:
         begin, total = int(seq_start[first]), int(seq_start[first + count] - seq_start[first])
         col0, width = tiles(total)
         block = np.zeros((col0.shape[0], 8), dtype=np.int64)
-        block[:, 0], block[:, 1], block[:, 2], block[:, 3], block[:, 5], block[:, 7] = first, begin, total, col0, prefix, width
+        block[:, 0], block[:, 1], block[:, 2], block[:, 3], block[:, 5], block[:, 7] = reader, begin, total, col0, prefix, width
         rows.append(block)
     for seq in np.nonzero(counts > 0)[0]:
         total = int(counts[seq])
@@ -2857,8 +2858,8 @@ def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads
     items[:, 5] = np.minimum(rows[index, 5], items[:, 4] + part[index])
     # parts of a token: its group's, then its own
     ahead, own_part = np.zeros(sequences, dtype=np.int64), np.ones(sequences, dtype=np.int64)
-    for first, count, prefix in shared:
-        ahead[first:first + count] = cuts[np.nonzero((rows[:, 6] == 0) & (rows[:, 0] == first))[0][0]]
+    for first, count, _, reader in shared:
+        ahead[first:first + count] = cuts[np.nonzero((rows[:, 6] == 0) & (rows[:, 0] == reader))[0][0]]
     is_own = rows[:, 6] == 1
     own_part[rows[is_own, 0]] = part[is_own]
     items[:, 7] = place + np.where(items[:, 6] == 1, ahead[items[:, 0]], 0)
@@ -2880,9 +2881,10 @@ def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads:
     device = torch.device(device)
     items, part_first = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype,
                                             _compute_units(device) if device.type == "cuda" else 256)
-    if int(part_first[-1]) * num_heads >= 1 << 31 or items.shape[0] * num_kv_heads >= 1 << 31:
-        raise invalid_shape("shared_prefix_plan: the step is beyond what one launch takes")
     longest = max((int(length) for length in seq_len), default=0)
+    if (int(part_first[-1]) * num_heads >= 1 << 31 or items.shape[0] * num_kv_heads >= 1 << 24 or (part_first.shape[0] - 1) * num_heads >= 1 << 26
+            or longest > 1 << 30):
+        raise invalid_shape("shared_prefix_plan: the step is beyond what one launch takes")
     return SharedPrefixPlan(torch.from_numpy(items).to(device), torch.from_numpy(part_first).to(device), part_first.shape[0] - 1, int(part_first[-1]),
                             len(seq_len), longest, (num_heads, num_kv_heads, head_dim, dtype))
 
@@ -2947,8 +2949,11 @@ def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: t
 
     q [tokens, nq * d], cache [pages, 2, nkv, page_size * d] and block_table [sequences, max_blocks] as for `attention_mfma`, which gives
     the same result (up to rounding) from the same arguments.  plan: from `shared_prefix_plan` for this step and these sizes; a group's shared
-    positions are read through its first sequence's row of the table, all others through their own sequence's.  The pages of whole blocks
-    are usually the same ones in all rows of the group, but need not be.  positions: int32 [tokens], the tokens' positions, as the plan has them.
+    positions are read through the table's row of its first sequence that brings tokens, all others through their own sequence's.  The pages of whole blocks
+    are usually the same ones in all rows of the group, but need not be; entries of the table that none of these positions lie on may hold anything.
+    positions: int32 [tokens], the tokens' positions, as the plan has them.  q and the cache start at multiples of 16 bytes.
+    A key or value row that a token does not see reaches it only where several tokens of one sequence run together and a later one's value is
+    infinite or a NaN.
     softcap: a scaled score s enters the softmax as softcap * tanh(s / softcap).  sink: float32 [nq], a number per head whose exponential
     joins the softmax's denominator.  Rows of q that no sequence brings give zeros."""
     if (num_heads, num_kv_heads, head_dim, q.dtype) != plan.sizes:
@@ -2957,7 +2962,7 @@ def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: t
     _device_tensor(cache, "cache", q.dtype)
     _device_tensor(block_table, "block_table", torch.int32)
     _device_tensor(positions, "positions", torch.int32)
-    if softcap is not None and not float(softcap) > 0.0:
+    if softcap is not None and not ctypes.c_float(softcap).value > 0.0:
         raise invalid_argument("attention_shared_prefix: a cap of the scores must be positive")
     if sink is not None:
         _device_tensor(sink, "sink", torch.float32)
@@ -2969,8 +2974,8 @@ def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: t
     if q.dim() != 2 or q.shape[1] != num_heads * head_dim or tokens != plan.tokens or positions.shape != (tokens,):
         raise invalid_shape(f"attention_shared_prefix: q {list(q.shape)} and positions {list(positions.shape)} are not [{plan.tokens}, nq * d] and [{plan.tokens}]")
     page_size = _check_cache(cache, num_kv_heads, head_dim, "attention_shared_prefix")
-    if head_dim % 16 != 0 or not 0 < head_dim <= ATTENTION_MAX_HEAD_DIM or page_size < 16 or page_size & (page_size - 1):
-        raise invalid_argument("attention_shared_prefix takes head sizes in steps of 16 up to 256, pages of a power of two of rows (at least 16)")
+    if head_dim % 16 != 0 or not 0 < head_dim <= ATTENTION_MAX_HEAD_DIM or not 16 <= page_size <= 65536 or page_size & (page_size - 1):
+        raise invalid_argument("attention_shared_prefix takes head sizes in steps of 16 up to 256, pages of a power of two of rows (16 to 65536)")
     if block_table.dim() != 2 or block_table.shape[0] < plan.sequences or block_table.shape[1] * page_size < plan.longest:
         raise invalid_shape(f"attention_shared_prefix: block_table {list(block_table.shape)} does not hold {plan.sequences} sequences of up to {plan.longest} positions")
     _one_device("attention_shared_prefix", q, cache, block_table, positions, plan.items, plan.part_first, sink)
