@@ -16,6 +16,8 @@
 // relative error 2^-9 is that of a value; sums, maxima and o are float); float on 16x16x4, 16 keys a block, nothing rounded.
 #include "common.h"
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace tlie {
@@ -694,6 +696,42 @@ static int launch_items(const void* q, const void* cache, const int* block_table
   return launch_status();
 }
 
+// ---- the host's half: which items a step has ----
+
+// Columns of the tile that has so many of its item before it, itself included (prefix_items_kernel takes them so).
+static int tile_columns(long long columns, int d, bool is_float) {
+  if (columns <= 16) return 16;
+  if (is_float) return d <= 128 ? 32 : 16;
+  return columns > 64 && d <= 128 ? 128 : 64;
+}
+// A tile of 64 columns costs three times what one of 16 does a key, one of 128 five times (their products and softmax, not the keys' reading).
+static double tile_cost(int columns) { return columns <= 32 ? 1.0 : columns <= 64 ? 3.0 : 5.0; }
+
+constexpr int kLeastKeys = 128;      // that a part has, if the whole has as many
+
+// Parts of about equal cost: a workgroup a compute unit, two where they are long (a part more is a result more to write and to join; 64 sequences
+// behind 6000 positions, 32 heads of 128 on 8: 35.6 us in 12 parts, 45 in 23; 2 behind 8000 15.8 in 32, 21 in 64; eight questions behind
+// 4000 51 in 6 parts, 56 in 4).
+static double part_cost(double total, int compute_units) { return std::max(total / (2.0 * compute_units), std::min(total / compute_units, 2600.0)); }
+
+struct Cut {
+  long long part, count;             // keys a part, and parts of the longest tile
+};
+// How `keys` positions, read by tiles the widest of which has `columns`, are cut.
+static Cut cut_keys(long long keys, int columns, double budget, int most_parts) {
+  const long long by_cost = std::llrint(static_cast<double>(keys) * tile_cost(columns) / std::max(budget, 1.0));
+  const long long count = std::max(1ll, std::min({(keys + kLeastKeys - 1) / kLeastKeys, by_cost, static_cast<long long>(most_parts)}));
+  const long long part = ((keys + count - 1) / count + 31) / 32 * 32;
+  return Cut{part, (keys + part - 1) / part};
+}
+
+// f(first column, columns of the tile) for the tiles of so many columns: of one width but the last, which has what is left.
+template <typename F>
+static void each_tile(long long columns, int d, bool is_float, F f) {
+  const int step = tile_columns(columns, d, is_float);
+  for (long long col0 = 0; col0 < columns; col0 += step) f(col0, columns - col0 > step ? step : tile_columns(columns - col0, d, is_float));
+}
+
 }  // namespace tlie
 
 using namespace tlie;
@@ -736,4 +774,104 @@ extern "C" int tlie_attention_prefix(const void* q, const void* cache, int dtype
   else
     hipLaunchKernelGGL((prefix_join_kernel<false>), dim3((rows + 3) / 4), dim3(256), 0, s, part_o, part_ml, part_first, sink, out, rows, nq, d);
   return launch_status();
+}
+
+// The items of a step, on the host: seq_start [sequences + 1] and seq_len [sequences] are its cumulative token counts and its sequences' lengths
+// after it; groups [num_groups][3] (first sequence, sequences, prefix), in ascending order, have the keys 0 .. prefix - 1 in common.
+// items: int32 [.][8], of which max_items fit; part_first: int32 [tokens + 1].  Returns the number of items, and writes nothing when they do
+// not fit; or -1: sequences that do not count up, or are shorter than what they bring; -2: groups that are not runs of the step's
+// sequences, apart from one another; -3: a token inside its group's prefix; -4: sizes; -5: a step beyond one launch.
+extern "C" int tlie_prefix_plan(const long long* seq_start, const long long* seq_len, int sequences, const long long* groups, int num_groups, int nq,
+                                int nkv, int d, int dtype, int compute_units, int most_parts, int* items, int max_items, int* part_first) {
+  constexpr long long kLongest = 1ll << 30;
+  const bool is_float = dtype == kF32;
+  if (sequences < 0 || num_groups < 0 || nq <= 0 || nkv <= 0 || nq % nkv != 0 || d <= 0 || compute_units <= 0 || most_parts <= 0) return -4;
+  const long long G = nq / nkv;
+  if (seq_start[0] != 0) return -1;
+  for (int s = 0; s < sequences; ++s) {
+    const long long count = seq_start[s + 1] - seq_start[s];
+    if (count < 0 || seq_len[s] < count) return -1;
+    if (seq_len[s] > kLongest || seq_start[s + 1] >= (1ll << 26) / nq) return -5;
+  }
+  const long long tokens = seq_start[sequences];
+  // ---- the groups, checked, and what the step costs ----
+  double cost = 0.0;
+  long long after = 0;
+  for (int g = 0; g < num_groups; ++g) {
+    const long long first = groups[3 * g], count = groups[3 * g + 1], prefix = groups[3 * g + 2];
+    if (count < 1 || prefix < 0 || first < after || count > sequences || first > sequences - count) return -2;
+    after = first + count;
+    for (long long s = first; s < after; ++s)
+      if (seq_start[s + 1] > seq_start[s] && seq_len[s] - (seq_start[s + 1] - seq_start[s]) < prefix) return -3;
+    each_tile((seq_start[after] - seq_start[first]) * G, d, is_float, [&](long long, int width) { cost += static_cast<double>(prefix) * tile_cost(width); });
+  }
+  // f(sequence, its tokens, its own first key), for those that bring tokens, and of its group's place (or -1)
+  auto each_sequence = [&](auto f) {
+    int g = 0;
+    for (int s = 0; s < sequences; ++s) {
+      while (g < num_groups && groups[3 * g] + groups[3 * g + 1] <= s) ++g;
+      const bool grouped = g < num_groups && groups[3 * g] <= s;
+      if (seq_start[s + 1] > seq_start[s]) f(s, seq_start[s + 1] - seq_start[s], grouped ? groups[3 * g + 2] : 0ll, grouped ? g : -1);
+    }
+  };
+  // a tile's keys end with the last token that it has columns of
+  auto own_end = [&](int s, long long count, long long col0, int width) { return seq_len[s] - count + std::min(count - 1, (col0 + width - 1) / G) + 1; };
+  each_sequence([&](int s, long long count, long long from, int) {
+    each_tile(count * G, d, is_float, [&](long long col0, int width) { cost += static_cast<double>(own_end(s, count, col0, width) - from) * tile_cost(width); });
+  });
+  const double budget = part_cost(cost * nkv, compute_units);
+  // All tiles of a group's prefix, and all of a sequence's own keys, are cut alike: as their widest and longest are.
+  auto cut_of_group = [&](int g) {
+    const long long columns = (seq_start[groups[3 * g] + groups[3 * g + 1]] - seq_start[groups[3 * g]]) * G;
+    return groups[3 * g + 2] > 0 && columns > 0 ? cut_keys(groups[3 * g + 2], tile_columns(columns, d, is_float), budget, most_parts) : Cut{1, 0};
+  };
+  auto cut_of_own = [&](int s, long long count, long long from) { return cut_keys(seq_len[s] - from, tile_columns(count * G, d, is_float), budget, most_parts); };
+
+  // ---- twice over the tiles: how many items, then the items ----
+  long long total = 0;
+  auto walk = [&](auto put) {                        // put(table row, tile's tokens from, tokens, first column, first key, end, own, keys a part, first part)
+    for (int g = 0; g < num_groups; ++g) {
+      const long long first = groups[3 * g], last = first + groups[3 * g + 1];
+      const Cut cut = cut_of_group(g);
+      if (cut.count == 0) continue;
+      long long reader = first;                      // a sequence that brings no tokens may be shorter than the prefix: the first that does holds it
+      while (seq_start[reader + 1] == seq_start[reader]) ++reader;
+      each_tile((seq_start[last] - seq_start[first]) * G, d, is_float, [&](long long col0, int) {
+        put(reader, seq_start[first], seq_start[last] - seq_start[first], col0, 0ll, groups[3 * g + 2], 0, cut.part, 0ll);
+      });
+    }
+    int group = -1;
+    long long ahead = 0;
+    each_sequence([&](int s, long long count, long long from, int g) {
+      if (g != group) group = g, ahead = g >= 0 ? cut_of_group(g).count : 0;
+      const Cut cut = cut_of_own(s, count, from);
+      each_tile(count * G, d, is_float, [&](long long col0, int width) {
+        put(s, seq_start[s], count, col0, from, own_end(s, count, col0, width), 1, cut.part, ahead);
+      });
+    });
+  };
+  walk([&](long long, long long, long long, long long, long long lo, long long hi, int, long long part, long long) { total += (hi - lo + part - 1) / part; });
+  if (total * nkv >= 1ll << 24) return -5;
+  if (total > max_items) return static_cast<int>(total);
+  int* word = items;
+  walk([&](long long table, long long tok0, long long ntok, long long col0, long long lo, long long hi, int own, long long part, long long place) {
+    for (long long key = lo; key < hi; key += part, ++place, word += 8) {
+      const long long values[8] = {table, tok0, ntok, col0, key, std::min(hi, key + part), own, place};
+      for (int i = 0; i < 8; ++i) word[i] = static_cast<int>(values[i]);
+    }
+  });
+  // a token's parts: its group's, then those of its own keys that begin at or before it
+  long long parts = 0, token = 0;
+  int group = -1;
+  long long ahead = 0;
+  each_sequence([&](int s, long long count, long long from, int g) {
+    if (g != group) group = g, ahead = g >= 0 ? cut_of_group(g).count : 0;
+    const Cut cut = cut_of_own(s, count, from);
+    for (long long i = 0; i < count; ++i, ++token) {
+      part_first[token] = static_cast<int>(std::min(parts, 0x7fffffffll));
+      parts += ahead + (seq_len[s] - count + i - from) / cut.part + 1;
+    }
+  });
+  part_first[tokens] = static_cast<int>(std::min(parts, 0x7fffffffll));
+  return parts * nq > 0x7fffffffll ? -5 : static_cast<int>(total);
 }

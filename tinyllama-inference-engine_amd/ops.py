@@ -2771,104 +2771,41 @@ def prefix_tile_columns(columns: int, head_dim: int, dtype: torch.dtype) -> int:
     return 128 if columns > 64 and head_dim <= 128 else 64
 
 
-PREFIX_COST = {16: 1.0, 32: 1.0, 64: 3.0, 128: 5.0}    # of a key, by the tile's columns
-PREFIX_LEAST, PREFIX_PARTS = 128, 64                    # keys that a part has at least, and parts that a token's keys are cut into at most
-
-
-def prefix_part_cost(total: float, compute_units: int) -> float:
-    """What a part of a step of this cost should cost: a workgroup a compute unit, two where they are long (a part more is a result more to
-    write and to join; 64 sequences behind 6000 positions, 32 heads of 128 on 8: 35.6 us in 12 parts, 45 in 23; 2 behind 8000 15.8 in 32, 21 in
-    64; eight questions behind 4000 51 in 6 parts, 56 in 4)."""
-    return max(total / (2 * compute_units), min(total / compute_units, 2600.0))
+PREFIX_PARTS = 64                      # parts that a prefix, and a sequence's own keys, are cut into at most
+_PLAN_ERRORS = {-1: (invalid_argument, "seq_start must count up from 0, and a sequence be as long as the tokens it brings"),
+                -2: (invalid_argument, "groups are runs of sequences of the step, apart from one another, with prefixes of 0 positions or more"),
+                -3: (invalid_argument, "a group's tokens stand behind its prefix"),
+                -4: (invalid_shape, "the number of heads must be a multiple of the number of kv heads"),
+                -5: (invalid_shape, "the step is beyond what one launch takes")}
 
 
 def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, compute_units: int = 256,
-                        most_parts: int = PREFIX_PARTS):
+                        most_parts: int = PREFIX_PARTS, items=None, part_first=None):
     """The host's half of `shared_prefix_plan`: (items [n, 8], part_first [tokens + 1]), int32 arrays of numpy.  most_parts: a limit to
-    the parts that a prefix, and a sequence's own keys, are cut into."""
+    the parts that a prefix, and a sequence's own keys, are cut into.  items, part_first: arrays to write into; with items' rows too few
+    None is returned.  (csrc/attention_prefix.hip forms them: in numpy a step of 64 sequences took half a millisecond of the host.)"""
     import numpy as np
-    seq_start, seq_len = np.asarray(seq_start, dtype=np.int64), np.asarray(seq_len, dtype=np.int64)
+    seq_start, seq_len = np.ascontiguousarray(seq_start, dtype=np.int64), np.ascontiguousarray(seq_len, dtype=np.int64)
     if seq_start.ndim != 1 or seq_len.ndim != 1 or seq_start.shape[0] != seq_len.shape[0] + 1:
         raise invalid_shape("shared_prefix_plan takes seq_start [sequences + 1] and seq_len [sequences]")
-    counts = seq_start[1:] - seq_start[:-1]
-    if seq_start[0] != 0 or (counts < 0).any() or (seq_len < counts).any():
-        raise invalid_argument("shared_prefix_plan: seq_start must count up from 0, and a sequence be as long as the tokens it brings")
-    if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads != 0:
-        raise invalid_shape("shared_prefix_plan: the number of heads must be a multiple of the number of kv heads")
-    group, sequences = num_heads // num_kv_heads, seq_len.shape[0]
-    prefix_of = np.zeros(sequences, dtype=np.int64)
-    seen, shared = 0, []
-    for first, count, prefix in sorted((int(a), int(b), int(c)) for a, b, c in groups):
-        if count < 1 or prefix < 0 or first < seen or first + count > sequences:
-            raise invalid_argument("shared_prefix_plan: groups are runs of sequences of the step, apart from one another, with prefixes of 0 positions or more")
-        seen = first + count
-        members = slice(first, first + count)
-        if ((seq_len[members] - counts[members] < prefix) & (counts[members] > 0)).any():
-            raise invalid_argument("shared_prefix_plan: a group's tokens stand behind its prefix")
-        if prefix > 0 and seq_start[first + count] > seq_start[first]:
-            # (a sequence that brings no tokens may be shorter than the prefix: the first that brings some holds it)
-            shared.append((first, count, prefix, first + int(np.nonzero(counts[members])[0][0])))
-            prefix_of[members] = prefix
-
-    def tiles(tokens: int):
-        """First columns and widths of an item's tiles: of one width but the last, which has what is left."""
-        columns = tokens * group
-        step = prefix_tile_columns(columns, head_dim, dtype)
-        col0 = np.arange(0, columns, step, dtype=np.int64)
-        width = np.full(col0.shape[0], step, dtype=np.int64)
-        width[-1] = prefix_tile_columns(columns - int(col0[-1]), head_dim, dtype)
-        return col0, width
-
-    # (sequence, first token, tokens, first column, first key, end of the keys, own, width)
-    rows = []
-    for first, count, prefix, reader in shared:
-        begin, total = int(seq_start[first]), int(seq_start[first + count] - seq_start[first])
-        col0, width = tiles(total)
-        block = np.zeros((col0.shape[0], 8), dtype=np.int64)
-        block[:, 0], block[:, 1], block[:, 2], block[:, 3], block[:, 5], block[:, 7] = reader, begin, total, col0, prefix, width
-        rows.append(block)
-    for seq in np.nonzero(counts > 0)[0]:
-        total = int(counts[seq])
-        col0, width = tiles(total)
-        block = np.zeros((col0.shape[0], 8), dtype=np.int64)
-        block[:, 0], block[:, 1], block[:, 2], block[:, 3], block[:, 4], block[:, 6], block[:, 7] = seq, seq_start[seq], total, col0, prefix_of[seq], 1, width
-        block[:, 5] = seq_len[seq] - total + np.minimum(total - 1, (col0 + width - 1) // group) + 1
-        rows.append(block)
-    tokens = int(seq_start[-1])
-    if not rows:
-        return np.zeros((0, 8), dtype=np.int32), np.zeros(tokens + 1, dtype=np.int32)
-    rows = np.concatenate(rows)
-    lengths = rows[:, 5] - rows[:, 4]
-    cost = np.array([PREFIX_COST[int(width)] for width in rows[:, 7]])
-    # Parts of about equal cost.  All tiles of a group's prefix, and all of a sequence's own keys, are cut alike: at the parts of their widest.
-    budget = prefix_part_cost(float((lengths * cost).sum()) * num_kv_heads, compute_units)
-    key = rows[:, 0] * 2 + rows[:, 6]
-    part = np.zeros(rows.shape[0], dtype=np.int64)
-    for which in np.unique(key):
-        mine = key == which
-        width, longest = int(rows[mine, 7].max()), int(lengths[mine].max())
-        count = max(1, min(-(-longest // PREFIX_LEAST), int(round(longest * PREFIX_COST[width] / max(budget, 1.0))), most_parts))
-        part[mine] = -(-(-(-longest // count)) // 32) * 32
-    cuts = -(-lengths // part)
-    index = np.repeat(np.arange(rows.shape[0]), cuts)
-    place = np.arange(index.shape[0]) - np.repeat(np.cumsum(cuts) - cuts, cuts)
-    items = np.empty((index.shape[0], 8), dtype=np.int32)
-    items[:, :7] = rows[index, :7]
-    items[:, 4] = rows[index, 4] + place * part[index]
-    items[:, 5] = np.minimum(rows[index, 5], items[:, 4] + part[index])
-    # parts of a token: its group's, then its own
-    ahead, own_part = np.zeros(sequences, dtype=np.int64), np.ones(sequences, dtype=np.int64)
-    for first, count, _, reader in shared:
-        ahead[first:first + count] = cuts[np.nonzero((rows[:, 6] == 0) & (rows[:, 0] == reader))[0][0]]
-    is_own = rows[:, 6] == 1
-    own_part[rows[is_own, 0]] = part[is_own]
-    items[:, 7] = place + np.where(items[:, 6] == 1, ahead[items[:, 0]], 0)
-    owner = np.repeat(np.arange(sequences), counts)
-    position = seq_len[owner] - counts[owner] + np.arange(tokens) - seq_start[owner]
-    parts = ahead[owner] + -(-(position + 1 - prefix_of[owner]) // own_part[owner])
-    part_first = np.zeros(tokens + 1, dtype=np.int32)
-    part_first[1:] = np.cumsum(parts)
-    return items, part_first
+    groups = np.array(sorted(groups), dtype=np.int64).reshape(-1, 3)
+    given = items is not None
+    if not given:
+        items = np.empty((256, 8), dtype=np.int32)
+    if part_first is None:
+        part_first = np.empty(max(0, int(seq_start[-1])) + 1, dtype=np.int32)
+    while True:
+        count = _entry("tlie_prefix_plan", "ppipiiiiiiipip")(seq_start.ctypes.data, seq_len.ctypes.data, seq_len.shape[0], groups.ctypes.data, groups.shape[0], num_heads,
+                                                            num_kv_heads, head_dim, dtype_code(dtype), compute_units, most_parts, items.ctypes.data,
+                                                            items.shape[0], part_first.ctypes.data)
+        if count < 0:
+            error, text = _PLAN_ERRORS[count]
+            raise error(f"shared_prefix_plan: {text}")
+        if count <= items.shape[0]:
+            return items[:count], part_first
+        if given:
+            return None
+        items = np.empty((count, 8), dtype=np.int32)
 
 
 def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device) -> SharedPrefixPlan:
@@ -2877,16 +2814,14 @@ def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads:
     seq_start: the step's cumulative token counts [sequences + 1]; seq_len: the sequences' lengths after the step [sequences]
     (arrays on the host).  groups: (first sequence, sequences, prefix) each, runs of sequences that hold the same keys and values at the
     positions 0 .. prefix - 1; all their tokens stand behind it.  Sequences in no group share nothing."""
-    dtype_code(dtype)
+    import numpy as np
     device = torch.device(device)
     items, part_first = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype,
                                             _compute_units(device) if device.type == "cuda" else 256)
     longest = max((int(length) for length in seq_len), default=0)
-    if (int(part_first[-1]) * num_heads >= 1 << 31 or items.shape[0] * num_kv_heads >= 1 << 24 or (part_first.shape[0] - 1) * num_heads >= 1 << 26
-            or longest > 1 << 30):
-        raise invalid_shape("shared_prefix_plan: the step is beyond what one launch takes")
-    return SharedPrefixPlan(torch.from_numpy(items).to(device), torch.from_numpy(part_first).to(device), part_first.shape[0] - 1, int(part_first[-1]),
-                            len(seq_len), longest, (num_heads, num_kv_heads, head_dim, dtype))
+    count, parts, tokens = items.shape[0], int(part_first[-1]), part_first.shape[0] - 1
+    both = torch.from_numpy(np.concatenate([items.ravel(), part_first])).to(device)             # (one transfer)
+    return SharedPrefixPlan(both[:count * 8].view(count, 8), both[count * 8:], tokens, parts, len(seq_len), longest, (num_heads, num_kv_heads, head_dim, dtype))
 
 
 def shared_prefix_pays(groups, num_kv_heads: int, head_dim: int) -> bool:
@@ -2907,25 +2842,26 @@ class RecordedPrefixPlan:
         self.parts = tokens * 24 + 256
         self._host = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, pin_memory=True)
         self._device = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, device=device)
+        self._units = _compute_units(self._device.device)
         self.plan = SharedPrefixPlan(self._device[:self.items * 8].view(self.items, 8), self._device[self.items * 8:], tokens, self.parts, tokens,
                                      longest, (num_heads, num_kv_heads, head_dim, dtype))
 
     def fill(self, seq_start, seq_len, groups) -> None:
         num_heads, num_kv_heads, head_dim, dtype = self.plan.sizes
-        most = PREFIX_PARTS
+        host, begin, most = self._host.numpy(), self.items * 8, PREFIX_PARTS
+        tokens = int(seq_start[-1])
+        if tokens > self.plan.tokens:
+            raise invalid_shape(f"a recorded plan for {self.plan.tokens} tokens does not hold {tokens}")
+        items, part_first = host[:begin].reshape(self.items, 8), host[begin:]
         while True:
-            items, part_first = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype,
-                                                    _compute_units(self._device.device), most)
-            if items.shape[0] <= self.items and int(part_first[-1]) <= self.parts:
+            made = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype, self._units, most, items, part_first)
+            if made is not None and int(part_first[tokens]) <= self.parts:
                 break
             if most == 1:
                 raise invalid_shape("a recorded step's shared prefixes do not fit its plan")
             most //= 2
-        host, begin = self._host.numpy(), self.items * 8
-        host[:items.size] = items.ravel()
-        host[items.size:begin] = 0
-        host[begin:begin + part_first.shape[0]] = part_first
-        host[begin + part_first.shape[0]:] = part_first[-1]
+        items[made[0].shape[0]:] = 0
+        part_first[tokens + 1:] = part_first[tokens]
         self._device.copy_(self._host, non_blocking=True)
 
 
