@@ -181,6 +181,12 @@ __device__ __forceinline__ void each_of(int index, const float4& v, F f) {
   f(index, v.x), f(index + 1, v.y), f(index + 2, v.z), f(index + 3, v.w);
 }
 
+// The parts' kernels have a workgroup a part, the parts of row r on the die r % 8 (workgroups go to the dies in turn), in all of them: what one kernel
+// leaves of a row, and the row itself, is in that die's L2 for the next, and the last kernel has row r there by itself.
+constexpr int kDies = 8;
+__device__ __forceinline__ int row_of(int parts) { return static_cast<int>(blockIdx.x / kDies) / parts * kDies + static_cast<int>(blockIdx.x % kDies); }
+__device__ __forceinline__ int part_of(int parts) { return static_cast<int>(blockIdx.x / kDies) % parts; }
+
 struct PartStat {
   uint64_t best;        // place_key of the part's first token in the order; 0: the part has none; all ones: a NaN or +inf
   float min;            // the smallest finite logit, +inf: none
@@ -190,10 +196,11 @@ constexpr uint64_t kBadPart = ~0ull;
 constexpr uint32_t kNotListed = ~0u;
 
 __global__ void __launch_bounds__(kPartThreads)
-draw_best_kernel(const float* __restrict__ logits, int vocab, int part_len, int parts, PartStat* __restrict__ stats) {
+draw_best_kernel(const float* __restrict__ logits, int rows, int vocab, int part_len, int parts, PartStat* __restrict__ stats) {
   __shared__ uint64_t best_of[kPartThreads / kWave];
   __shared__ float min_of[kPartThreads / kWave];
-  const int row = blockIdx.y, part = blockIdx.x, begin = part * part_len, end = min(vocab, begin + part_len);
+  const int row = row_of(parts), part = part_of(parts), begin = part * part_len, end = min(vocab, begin + part_len);
+  if (row >= rows) return;
   float most = -INFINITY, least = INFINITY;
   int at = 0;
   bool bad = false;
@@ -251,14 +258,15 @@ __device__ __forceinline__ double plain_weights(float max, const float4& v) {
 }
 
 __global__ void __launch_bounds__(kPartThreads)
-draw_weigh_kernel(const float* __restrict__ logits, int vocab, int part_len, int parts, const PartStat* __restrict__ stats,
+draw_weigh_kernel(const float* __restrict__ logits, int rows, int vocab, int part_len, int parts, const PartStat* __restrict__ stats,
                   const float* __restrict__ temperature, int shift, int want_sum, uint64_t* __restrict__ class_mass,
                   uint32_t* __restrict__ class_count, double* __restrict__ sums) {
   __shared__ unsigned long long mass[kClasses];
   __shared__ uint32_t count[kClasses];
   __shared__ double sum_of[kPartThreads / kWave];
   __shared__ double powers[kPowers];
-  const int row = blockIdx.y, part = blockIdx.x, begin = part * part_len, end = min(vocab, begin + part_len);
+  const int row = row_of(parts), part = part_of(parts), begin = part * part_len, end = min(vocab, begin + part_len);
+  if (row >= rows) return;
   uint64_t best;
   float least;
   join_stats(stats + static_cast<size_t>(row) * parts, parts, best, least);
@@ -681,13 +689,14 @@ __device__ uint64_t cross_without_list(CrossShared<THREADS>& s, const float* __r
 }
 
 __global__ void __launch_bounds__(kGatherThreads)
-draw_gather_kernel(const float* __restrict__ logits, int vocab, int part_len, int parts, const PartStat* __restrict__ stats,
+draw_gather_kernel(const float* __restrict__ logits, int rows, int vocab, int part_len, int parts, const PartStat* __restrict__ stats,
                    const float* __restrict__ uniform, const float* __restrict__ temperature, const int* __restrict__ top_k,
                    const float* __restrict__ top_p, const float* __restrict__ min_p, int shift, const uint64_t* __restrict__ class_mass,
                    const uint32_t* __restrict__ class_count, RowState* __restrict__ states, Listed* __restrict__ lists) {
   __shared__ ClassShared<kGatherThreads> s;
   __shared__ double powers[kPowers];
-  const int r = blockIdx.y, part = blockIdx.x, tid = threadIdx.x;
+  const int r = row_of(parts), part = part_of(parts), tid = threadIdx.x;
+  if (r >= rows) return;
   const Ask ask = ask_of(r, uniform, temperature, top_k, top_p, min_p);
   if (!(ask.t > 0.f)) return;
   uint64_t best;
@@ -909,11 +918,12 @@ extern "C" int tlie_draw(const float* logits, int rows, int vocab, const float* 
   double* sums = reinterpret_cast<double*>(stats + places);
   uint64_t* class_mass = reinterpret_cast<uint64_t*>(sums + places);
   uint32_t* class_count = reinterpret_cast<uint32_t*>(class_mass + places * kClasses);
-  hipLaunchKernelGGL(draw_best_kernel, dim3(parts, rows), dim3(kPartThreads), 0, s, logits, vocab, part_len, parts, stats);
-  hipLaunchKernelGGL(draw_weigh_kernel, dim3(parts, rows), dim3(kPartThreads), 0, s, logits, vocab, part_len, parts, stats, temperature, shift,
+  const dim3 grid((rows + kDies - 1) / kDies * kDies * parts);
+  hipLaunchKernelGGL(draw_best_kernel, grid, dim3(kPartThreads), 0, s, logits, rows, vocab, part_len, parts, stats);
+  hipLaunchKernelGGL(draw_weigh_kernel, grid, dim3(kPartThreads), 0, s, logits, rows, vocab, part_len, parts, stats, temperature, shift,
                      logprob != nullptr ? 1 : 0, class_mass, class_count, sums);
   if (temperature != nullptr)
-    hipLaunchKernelGGL(draw_gather_kernel, dim3(parts, rows), dim3(kGatherThreads), 0, s, logits, vocab, part_len, parts, stats, uniform, temperature,
+    hipLaunchKernelGGL(draw_gather_kernel, grid, dim3(kGatherThreads), 0, s, logits, rows, vocab, part_len, parts, stats, uniform, temperature,
                      top_k, top_p, min_p, shift, class_mass, class_count, states, lists);
   hipLaunchKernelGGL(draw_pick_kernel, dim3(rows), dim3(kPickThreads), 0, s, logits, vocab, parts, stats, uniform, temperature, top_k, top_p, min_p,
                      shift, states, lists, sums, out, logprob);
