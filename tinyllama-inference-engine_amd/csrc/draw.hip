@@ -22,41 +22,26 @@ namespace tlie {
 
 constexpr int kClasses = 1024, kPartThreads = 512, kGatherThreads = 256, kPickThreads = 512, kRowThreads = 1024, kListMost = 2048, kPartsMost = 8;
 
-// 2^(j / 128)
-constexpr int kPowers = 128;
-__constant__ double powers_of_two[kPowers] = {
-    1.0, 1.0054299011128027, 1.0108892860517005, 1.016378314910953,
-    1.0218971486541166, 1.0274459491187637, 1.0330248790212284, 1.0386341019613787,
-    1.0442737824274138, 1.0499440858006872, 1.0556451783605572, 1.061377227289262,
-    1.0671404006768237, 1.0729348675259756, 1.0787607977571199, 1.0846183622133092,
-    1.0905077326652577, 1.0964290818163769, 1.102382583307841, 1.1083684117236787,
-    1.1143867425958924, 1.1204377524096067, 1.1265216186082418, 1.1326385195987192,
-    1.1387886347566916, 1.1449721444318042, 1.1511892299529827, 1.1574400736337511,
-    1.1637248587775775, 1.1700437696832502, 1.1763969916502812, 1.182784710984341,
-    1.189207115002721, 1.1956643920398273, 1.202156731452703, 1.2086843236265816,
-    1.215247359980469, 1.2218460329727576, 1.22848053610687, 1.2351510639369334,
-    1.241857812073484, 1.2486009771892048, 1.255380757024691, 1.2621973503942507,
-    1.2690509571917332, 1.275941778396392, 1.2828700160787783, 1.2898358734066657,
-    1.2968395546510096, 1.3038812651919358, 1.3109612115247644, 1.318079601266064,
-    1.3252366431597413, 1.3324325470831615, 1.339667524053303, 1.3469417862329458,
-    1.3542555469368927, 1.3616090206382248, 1.3690024229745905, 1.3764359707545302,
-    1.383909881963832, 1.3914243757719262, 1.3989796725383112, 1.4065759938190154,
-    1.4142135623730951, 1.4218926021691656, 1.42961333839197, 1.4373759974489824,
-    1.4451808069770467, 1.4530279958490526, 1.460917794180647, 1.4688504333369818,
-    1.4768261459394993, 1.4848451658727524, 1.4929077282912648, 1.5010140696264256,
-    1.5091644275934228, 1.5173590411982147, 1.5255981507445384, 1.533881997840956,
-    1.5422108254079407, 1.550584877685, 1.559004400237837, 1.567469639965553,
-    1.5759808451078865, 1.5845382652524937, 1.593142151342267, 1.6017927556826934,
-    1.6104903319492543, 1.6192351351948637, 1.6280274218573478, 1.6368674497669644,
-    1.645755478153965, 1.6546917676561943, 1.6636765803267364, 1.6727101796415966,
-    1.681792830507429, 1.6909247992693053, 1.7001063537185235, 1.709337763100463,
-    1.718619298122478, 1.7279512309618377, 1.7373338352737062, 1.746767386199169,
-    1.7562521603732995, 1.7657884359332727, 1.7753764925265212, 1.785016611318935,
-    1.7947090750031072, 1.804454167806624, 1.8142521755003989, 1.8241033854070534,
-    1.8340080864093424, 1.843966568958626, 1.8539791250833855, 1.864046048397789,
-    1.8741676341103, 1.8843441790323345, 1.8945759815869656, 1.9048633418176741,
-    1.9152065613971474, 1.925605943636125, 1.9360617934922943, 1.9465744175792332,
-    1.9571441241754002, 1.9677712232331759, 1.978456026387951, 1.9891988469672663};
+// 2^(i / 32) and 2^(j / 1024): 2^(k / 1024) is the product of one of each
+constexpr int kPowers = 1024;
+__constant__ double powers_whole[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+__constant__ double powers_fine[32] = {
+    1.0, 1.0006771306930664, 1.0013547198921082, 1.002032767907594,
+    1.0027112750502025, 1.0033902416308227, 1.004069667960554, 1.0047495543507072,
+    1.0054299011128027, 1.006110708558573, 1.0067919769999607, 1.0074737067491204,
+    1.0081558981184175, 1.0088385514204294, 1.0095216669679448, 1.0102052450739643,
+    1.0108892860517005, 1.011573790214578, 1.0122587578762337, 1.0129441893505169,
+    1.0136300849514894, 1.0143164449934257, 1.0150032697908125, 1.0156905596583505,
+    1.016378314910953, 1.0170665358637463, 1.0177552228320703, 1.0184443761314785,
+    1.019133996077738, 1.0198240829868295, 1.0205146371749483, 1.0212056589585028};
 
 // larger for what stands earlier: the float's order, then the lower index (-0 and +0 are equal)
 __device__ __forceinline__ uint64_t place_key(float v, int index) {
@@ -73,23 +58,43 @@ __device__ __forceinline__ int place_index(uint64_t key) { return static_cast<in
 // What is the same for all tokens of a row.
 struct RowScale {
   float max, class_scale;
-  double max_wide, steps, one;       // one: the weight 1
-  const double* powers;              // in LDS: 2^(j / 128) times the weight 1
+  double max_wide, steps, least, one;       // least: the gap from which on nothing weighs; one: the weight 1
 };
+// With the powers 2^(j / 1024) in LDS, times the weight 1: ALL of them, for kernels that weigh every token, or 32 by 32 as they stand above, for
+// those that weigh the tokens in question (their products are the same numbers: the weight 1 is a power of two).
+template <bool ALL>
+struct PoweredScale : RowScale {
+  const double* powers;
+  __device__ __forceinline__ double power(int n) const {
+#pragma clang fp contract(off)
+    if constexpr (ALL) return powers[n & (kPowers - 1)];
+    else return powers[(n >> 5) & 31] * powers[32 + (n & 31)];
+  }
+};
+template <bool ALL>
+constexpr int kPowersHeld = ALL ? kPowers : 64;
 
 // Every thread of the workgroup: the powers into LDS (to be read after the next barrier).
-template <int THREADS>
+template <bool ALL, int THREADS>
 __device__ __forceinline__ void bring_powers(double* powers, int shift) {
+#pragma clang fp contract(off)
   const double one = __longlong_as_double((1023ll + shift) << 52);
-  for (int j = threadIdx.x; j < kPowers; j += THREADS) powers[j] = powers_of_two[j] * one;
+  if constexpr (ALL) {
+    for (int j = threadIdx.x; j < kPowers; j += THREADS) powers[j] = powers_whole[j >> 5] * powers_fine[j & 31] * one;
+  } else {
+    if (threadIdx.x < 64) powers[threadIdx.x] = threadIdx.x < 32 ? powers_whole[threadIdx.x] * one : powers_fine[threadIdx.x & 31];
+  }
 }
 
 // The classes share the gaps from 0 to 32 T (what is lighter than e^-32 rounds to no weight), or to the smallest logit if that is nearer.
-__device__ __forceinline__ RowScale row_scale(float max, float min, float temperature, int shift, const double* powers) {
+template <bool ALL>
+__device__ __forceinline__ PoweredScale<ALL> row_scale(float max, float min, float temperature, int shift, const double* powers) {
   const float span = fminf(32.f * temperature, max - min);
-  RowScale row;
+  PoweredScale<ALL> row;
   row.max = max, row.class_scale = span > 0.f ? kClasses / span : 0.f;
-  row.max_wide = max, row.steps = 184.6649652337873 / static_cast<double>(temperature), row.one = __longlong_as_double((1023ll + shift) << 52);
+  // (an infinite temperature as a finite one at which every finite gap is none)
+  const double wide = fmin(static_cast<double>(temperature), 1e300);
+  row.max_wide = max, row.steps = 1477.3197218702985 / wide, row.least = -34.0 * wide, row.one = __longlong_as_double((1023ll + shift) << 52);
   row.powers = powers;
   return row;
 }
@@ -97,24 +102,23 @@ __device__ __forceinline__ int gap_class(const RowScale& row, float v) {
   return static_cast<int>(fminf((row.max - v) * row.class_scale, static_cast<float>(kClasses - 1)));
 }
 
-// exp((v - max) / T) in units of 2^-shift; one function, each operation written out, for every kernel that forms it.  The exponent in steps
-// of ln 2 / 128 is a whole number n and a rest f of half a step at most: 2^(n / 128) from the table and its exponent, exp of the rest by its
-// series to the fourth power (1.3e-15 of it is left).  12 operations on 64-bit floats; by the series alone, to the eleventh power
-// of |r| <= 0.347, 23: the weights of 256 rows of 128256 tokens took 57 us that way.
-__device__ __forceinline__ double weight_wide(const RowScale& row, float v) {
+// exp((v - max) / T) in units of 2^-shift; one function, each operation written out, for every kernel that forms it.  The
+// exponent in steps of ln 2 / 1024 is a whole number n and a rest f of half a step at most: 2^(n / 1024) from the table and its exponent, exp of
+// the rest by its series to the third power (5.5e-16 of it is left).  10 operations on 64-bit floats, and a conversion: the processor's time is
+// what the weights of many rows take (256 rows of 128256 tokens MEASURED).
+template <bool ALL>
+__device__ __forceinline__ double weight_wide(const PoweredScale<ALL>& row, float v) {
 #pragma clang fp contract(off)
-  const double y = fmax((static_cast<double>(v) - row.max_wide) * row.steps, -8192.0);
-  const double shifted = y + 6755399441055744.0;                        // 1.5 * 2^52: the nearest whole number in the low bits
+  const double gap = fmax(static_cast<double>(v) - row.max_wide, row.least);
+  const double shifted = fma(gap, row.steps, 6755399441055744.0);        // 1.5 * 2^52: the nearest whole number in the low bits
   const int n = static_cast<int>(__double_as_longlong(shifted));
-  const double f = y - (shifted - 6755399441055744.0);
+  const double f = fma(gap, row.steps, 6755399441055744.0 - shifted);
   constexpr double step = 0.6931471805599453 / kPowers;
-  double p = step * step * step * step / 24.0;
-  p = fma(p, f, step * step * step / 6.0);
-  p = fma(p, f, step * step / 2.0);
+  double p = fma(step * step * step / 6.0, f, step * step / 2.0);
   p = fma(p, f, step);
   p = p * f;
-  const double power = row.powers[n & (kPowers - 1)];
-  const double scaled = __hiloint2double(__double2hiint(power) + ((n >> 7) << 20), __double2loint(power));
+  const double power = row.power(n);
+  const double scaled = __hiloint2double(__double2hiint(power) + ((n >> 10) << 20), __double2loint(power));
   return fma(scaled, p, scaled);
 }
 // a weight below 2^52 to the nearest whole number: adding 2^52 leaves it in the low bits
@@ -243,13 +247,20 @@ __device__ __forceinline__ void join_stats(const PartStat* __restrict__ stats, i
   }
 }
 
-__device__ __forceinline__ void weigh_token(const RowScale& scale, float v, unsigned long long* mass, uint32_t* count) {
-  const uint64_t units = weight_units(weight_wide(scale, v));
-  if (units != 0) {
-    const int c = gap_class(scale, v);
-    atomicAdd(&mass[c], static_cast<unsigned long long>(units));
-    atomicAdd(&count[c], 1u);
-  }
+// (the four weights first: with each one's sums behind it, behind a branch, every wave waits for its power alone)
+template <bool ALL>
+__device__ __forceinline__ void weigh_group(const PoweredScale<ALL>& scale, const float4& four, unsigned long long* mass, uint32_t* count) {
+  const float v[4] = {four.x, four.y, four.z, four.w};
+  uint64_t units[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) units[j] = weight_units(weight_wide(scale, v[j]));
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (units[j] != 0) {
+      const int c = gap_class(scale, v[j]);
+      atomicAdd(&mass[c], static_cast<unsigned long long>(units[j]));
+      atomicAdd(&count[c], 1u);
+    }
 }
 // exp(v - max), for the log-probability: an exponential's rounding of 2^-23 each, a sum of four in 32 bits, the rest in 64
 __device__ __forceinline__ double plain_weights(float max, const float4& v) {
@@ -264,7 +275,7 @@ draw_weigh_kernel(const float* __restrict__ logits, int rows, int vocab, int par
   __shared__ unsigned long long mass[kClasses];
   __shared__ uint32_t count[kClasses];
   __shared__ double sum_of[kPartThreads / kWave];
-  __shared__ double powers[kPowers];
+  __shared__ double powers[kPowersHeld<true>];
   const int row = row_of(parts), part = part_of(parts), begin = part * part_len, end = min(vocab, begin + part_len);
   if (row >= rows) return;
   uint64_t best;
@@ -274,13 +285,13 @@ draw_weigh_kernel(const float* __restrict__ logits, int rows, int vocab, int par
   const float t = temperature ? temperature[row] : 0.f;
   const bool drawn = t > 0.f;
   if (!drawn && !want_sum) return;
-  bring_powers<kPartThreads>(powers, shift);
+  bring_powers<true, kPartThreads>(powers, shift);
   for (int c = threadIdx.x; c < kClasses; c += kPartThreads) mass[c] = 0, count[c] = 0;
   __syncthreads();
-  const RowScale scale = row_scale(place_value(best), least, t, shift, powers);
+  const auto scale = row_scale<true>(place_value(best), least, t, shift, powers);
   double sum = 0.0;
-  scan_tokens<kPartThreads, 4>(logits + static_cast<size_t>(row) * vocab, begin, end, [&](int first, const float4& four) {
-    if (drawn) each_of(first, four, [&](int, float v) { weigh_token(scale, v, mass, count); });
+  scan_tokens<kPartThreads, 4>(logits + static_cast<size_t>(row) * vocab, begin, end, [&](int, const float4& four) {
+    if (drawn) weigh_group(scale, four, mass, count);
     if (want_sum) sum += plain_weights(scale.max, four);
   });
   const size_t place = static_cast<size_t>(row) * parts + part;
@@ -486,8 +497,8 @@ __device__ __forceinline__ bool any_between(const float4& v, float lower, float 
   return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= lower && fminf(fminf(v.x, v.y), fminf(v.z, v.w)) <= upper;
 }
 // found(place in the list, key, weight, class) for each token of a group that a wanted class holds
-template <int THREADS, typename F>
-__device__ __forceinline__ void list_group(ClassShared<THREADS>& s, const RowScale& scale, float lower, float upper, int first, const float4& four, F found) {
+template <int THREADS, bool ALL, typename F>
+__device__ __forceinline__ void list_group(ClassShared<THREADS>& s, const PoweredScale<ALL>& scale, float lower, float upper, int first, const float4& four, F found) {
   if (!any_between(four, lower, upper)) return;
   each_of(first, four, [&](int i, float v) {
     if (!(v >= lower && v <= upper)) return;
@@ -520,8 +531,8 @@ struct CrossShared {
 };
 
 // The chosen token, from the list: entry(i) is its i-th.
-template <int THREADS, typename F>
-__device__ uint64_t cross(CrossShared<THREADS>& s, const RowScale& scale, const Ask& ask, const RowState& state, uint64_t best, F entry) {
+template <int THREADS, bool ALL, typename F>
+__device__ uint64_t cross(CrossShared<THREADS>& s, const PoweredScale<ALL>& scale, const Ask& ask, const RowState& state, uint64_t best, F entry) {
   constexpr int kEach = kListMost / THREADS;
   const int tid = threadIdx.x, size = static_cast<int>(state.size);
   // A token's running mass and rank: up to the class before, and of its own class what stands no later.  The list's tokens go into
@@ -624,8 +635,8 @@ __device__ uint64_t cross(CrossShared<THREADS>& s, const RowScale& scale, const 
 
 // Without a list (more tokens than it holds share the classes in question): the place in the order where the running mass
 // (or count) reaches target, found digit by digit of the place keys, eight passes over the row.  Returns the running mass there.
-template <int THREADS>
-__device__ __forceinline__ uint64_t descend(CrossShared<THREADS>& s, const float* __restrict__ row, int vocab, const RowScale& scale, uint64_t target, bool by_count,
+template <int THREADS, bool ALL>
+__device__ __forceinline__ uint64_t descend(CrossShared<THREADS>& s, const float* __restrict__ row, int vocab, const PoweredScale<ALL>& scale, uint64_t target, bool by_count,
                                          uint64_t* key) {
   uint64_t prefix = 0, mass_before = 0, count_before = 0, mass = 0;
   for (int digit = 7; digit >= 0; --digit) {
@@ -661,8 +672,8 @@ __device__ __forceinline__ uint64_t descend(CrossShared<THREADS>& s, const float
   *key = prefix;
   return mass;
 }
-template <int THREADS>
-__device__ uint64_t cross_without_list(CrossShared<THREADS>& s, const float* __restrict__ row, int vocab, const RowScale& scale, uint64_t one, const Ask& ask,
+template <int THREADS, bool ALL>
+__device__ uint64_t cross_without_list(CrossShared<THREADS>& s, const float* __restrict__ row, int vocab, const PoweredScale<ALL>& scale, uint64_t one, const Ask& ask,
                                        const RowState& state) {
   uint64_t place = 0, kept = state.total_lo;
   __syncthreads();
@@ -694,7 +705,7 @@ draw_gather_kernel(const float* __restrict__ logits, int rows, int vocab, int pa
                    const float* __restrict__ top_p, const float* __restrict__ min_p, int shift, const uint64_t* __restrict__ class_mass,
                    const uint32_t* __restrict__ class_count, RowState* __restrict__ states, Listed* __restrict__ lists) {
   __shared__ ClassShared<kGatherThreads> s;
-  __shared__ double powers[kPowers];
+  __shared__ double powers[kPowersHeld<false>];
   const int r = row_of(parts), part = part_of(parts), tid = threadIdx.x;
   if (r >= rows) return;
   const Ask ask = ask_of(r, uniform, temperature, top_k, top_p, min_p);
@@ -703,8 +714,8 @@ draw_gather_kernel(const float* __restrict__ logits, int rows, int vocab, int pa
   float least;
   join_stats(stats + static_cast<size_t>(r) * parts, parts, best, least);
   if (best == kBadPart || best == 0) return;
-  bring_powers<kGatherThreads>(powers, shift);
-  const RowScale scale = row_scale(place_value(best), least, ask.t, shift, powers);
+  bring_powers<false, kGatherThreads>(powers, shift);
+  const auto scale = row_scale<false>(place_value(best), least, ask.t, shift, powers);
   // the row's classes, four neighbours a thread; all parts are asked for together.  (Four waves: with a class a thread, sixteen
   // waves do what is the same for all of the row, and 64 rows in 8 parts took 20 us)
   constexpr int kOwn = kClasses / kGatherThreads;
@@ -745,7 +756,7 @@ draw_pick_kernel(const float* __restrict__ logits, int vocab, int parts, const P
                  const float* __restrict__ min_p, int shift, const RowState* __restrict__ states, const Listed* __restrict__ lists,
                  const double* __restrict__ sums, int* __restrict__ out, float* __restrict__ logprob) {
   __shared__ CrossShared<kPickThreads> s;
-  __shared__ double powers[kPowers];
+  __shared__ double powers[kPowersHeld<false>];
   const int r = blockIdx.x, tid = threadIdx.x;
   const Ask ask = ask_of(r, uniform, temperature, top_k, top_p, min_p);
   const Listed* list = lists + static_cast<size_t>(r) * kListMost;
@@ -768,8 +779,8 @@ draw_pick_kernel(const float* __restrict__ logits, int vocab, int parts, const P
   }
   uint64_t chosen = best;
   if (ask.t > 0.f) {
-    bring_powers<kPickThreads>(powers, shift);
-    const RowScale scale = row_scale(place_value(best), least, ask.t, shift, powers);
+    bring_powers<false, kPickThreads>(powers, shift);
+    const auto scale = row_scale<false>(place_value(best), least, ask.t, shift, powers);
     if (state.size <= kListMost)
       chosen = cross(s, scale, ask, state, best, [&](int i) { return list[i]; });
     else
@@ -784,7 +795,7 @@ draw_pick_kernel(const float* __restrict__ logits, int vocab, int parts, const P
 struct RowShared {
   ClassShared<kRowThreads> classes;
   CrossShared<kRowThreads> cross;
-  double powers[kPowers];
+  double powers[kPowersHeld<true>];
   uint64_t wave_best[kRowThreads / kWave];
   float wave_least[kRowThreads / kWave];
   double wave_sum[kRowThreads / kWave];
@@ -821,7 +832,7 @@ draw_row_kernel(const float* __restrict__ logits, int vocab, const float* __rest
     least = fminf(least, __shfl_xor(least, offset, 64));
   }
   if (lane == 0) s.wave_best[wave] = best, s.wave_least[wave] = least;
-  bring_powers<kRowThreads>(s.powers, shift);
+  bring_powers<true, kRowThreads>(s.powers, shift);
   unsigned long long* mass_of = reinterpret_cast<unsigned long long*>(s.classes.running_mass);       // the histogram, until it is summed up
   uint32_t* count_of = s.classes.running_count;
   for (int c = tid; c < kClasses; c += kRowThreads) mass_of[c] = 0, count_of[c] = 0;
@@ -838,11 +849,11 @@ draw_row_kernel(const float* __restrict__ logits, int vocab, const float* __rest
     }
     return;
   }
-  const RowScale scale = row_scale(place_value(best), least, ask.t, shift, s.powers);
+  const auto scale = row_scale<true>(place_value(best), least, ask.t, shift, s.powers);
   // ---- the weights, and the sum of the log-probability's ----
   double sum = 0.0;
-  scan_tokens<kRowThreads, 2>(row, 0, vocab, [&](int first, const float4& four) {
-    if (ask.t > 0.f) each_of(first, four, [&](int, float v) { weigh_token(scale, v, mass_of, count_of); });
+  scan_tokens<kRowThreads, 2>(row, 0, vocab, [&](int, const float4& four) {
+    if (ask.t > 0.f) weigh_group(scale, four, mass_of, count_of);
     if (logprob) sum += plain_weights(scale.max, four);
   });
   if (logprob) {
