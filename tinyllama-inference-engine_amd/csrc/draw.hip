@@ -373,6 +373,7 @@ struct ClassShared {
   uint64_t wave_mass[THREADS / kWave];
   uint32_t wave_count[THREADS / kWave], listed_count[THREADS / kWave];
   int found[7];                             // classes, a place for each question
+  uint32_t held_count;                      // of list_tokens
 };
 
 // From the masses and counts of a thread's own classes (kClasses / THREADS neighbours): which classes the crossings lie in, and
@@ -394,6 +395,7 @@ __device__ RowState find_classes(ClassShared<THREADS>& s, const RowScale& scale,
     const uint64_t own = all;
     const uint32_t own_n = all_n;
     if (tid < 7) s.found[tid] = kClasses;
+    if (tid == 0) s.held_count = 0;
     running_sums<THREADS>(s.wave_mass, s.wave_count, all, all_n);
     all -= own, all_n -= own_n;
 #pragma unroll
@@ -496,17 +498,35 @@ __device__ __forceinline__ void value_bounds(const ClassShared<THREADS>& s, cons
 __device__ __forceinline__ bool any_between(const float4& v, float lower, float upper) {
   return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= lower && fminf(fminf(v.x, v.y), fminf(v.z, v.w)) <= upper;
 }
-// found(place in the list, key, weight, class) for each token of a group that a wanted class holds
-template <int THREADS, bool ALL, typename F>
-__device__ __forceinline__ void list_group(ClassShared<THREADS>& s, const PoweredScale<ALL>& scale, float lower, float upper, int first, const float4& four, F found) {
-  if (!any_between(four, lower, upper)) return;
-  each_of(first, four, [&](int i, float v) {
-    if (!(v >= lower && v <= upper)) return;
-    const int c = gap_class(scale, v);
-    if (s.begin[c] == kNotListed) return;
+// A token that a wanted class holds, until its weight is formed.
+struct Held {
+  float v;
+  int index;
+};
+// found(place in the list, key, weight, class) for each token of begin .. end - 1 that a wanted class holds, by the whole workgroup.  They are
+// few: with their weights formed where they are met, nearly every wave's step waits for one lane's; held back, they are formed side by side.
+// held: kListMost places (more tokens than that, of no weight then, are looked at where they are met).  Ends before a barrier that the
+// caller needs for what it does with `held` or what `found` wrote.
+template <int THREADS, int TOGETHER, bool ALL, typename F>
+__device__ __forceinline__ void list_tokens(ClassShared<THREADS>& s, const PoweredScale<ALL>& scale, float lower, float upper, const float* __restrict__ row,
+                                            int begin, int end, Held* held, F found) {
+  auto list = [&](float v, int i) {
     const uint64_t units = weight_units(weight_wide(scale, v));
+    const int c = gap_class(scale, v);
     if (units != 0) found(atomicAdd(&s.place[c], 1u), place_key(v, i), units, c);
+  };
+  scan_tokens<THREADS, TOGETHER>(row, begin, end, [&](int first, const float4& four) {
+    if (!any_between(four, lower, upper)) return;
+    each_of(first, four, [&](int i, float v) {
+      if (!(v >= lower && v <= upper) || s.begin[gap_class(scale, v)] == kNotListed) return;
+      const uint32_t place = atomicAdd(&s.held_count, 1u);
+      if (place < kListMost) held[place] = Held{v, i};
+      else list(v, i);
+    });
   });
+  __syncthreads();
+  const uint32_t count = min(s.held_count, static_cast<uint32_t>(kListMost));
+  for (uint32_t j = threadIdx.x; j < count; j += THREADS) list(held[j].v, held[j].index);
 }
 template <int THREADS>
 __device__ __forceinline__ Listed listed_of(const ClassShared<THREADS>& s, uint64_t key, uint64_t units, int c) {
@@ -705,6 +725,7 @@ draw_gather_kernel(const float* __restrict__ logits, int rows, int vocab, int pa
                    const float* __restrict__ top_p, const float* __restrict__ min_p, int shift, const uint64_t* __restrict__ class_mass,
                    const uint32_t* __restrict__ class_count, RowState* __restrict__ states, Listed* __restrict__ lists) {
   __shared__ ClassShared<kGatherThreads> s;
+  __shared__ Held held[kListMost];
   __shared__ double powers[kPowersHeld<false>];
   const int r = row_of(parts), part = part_of(parts), tid = threadIdx.x;
   if (r >= rows) return;
@@ -745,9 +766,8 @@ draw_gather_kernel(const float* __restrict__ logits, int rows, int vocab, int pa
   value_bounds(s, scale, least, lower, upper);
   const int begin = part * part_len, end = min(vocab, begin + part_len);
   Listed* list = lists + static_cast<size_t>(r) * kListMost;
-  scan_tokens<kGatherThreads, 8>(logits + static_cast<size_t>(r) * vocab, begin, end, [&](int first, const float4& four) {
-    list_group(s, scale, lower, upper, first, four, [&](uint32_t place, uint64_t key, uint64_t units, int c) { list[place] = listed_of(s, key, units, c); });
-  });
+  list_tokens<kGatherThreads, 8>(s, scale, lower, upper, logits + static_cast<size_t>(r) * vocab, begin, end, held,
+                                 [&](uint32_t place, uint64_t key, uint64_t units, int c) { list[place] = listed_of(s, key, units, c); });
 }
 
 __global__ void __launch_bounds__(kPickThreads)
@@ -871,10 +891,10 @@ draw_row_kernel(const float* __restrict__ logits, int vocab, const float* __rest
     if (state.size <= kListMost) {
       float lower, upper;
       value_bounds(s.classes, scale, least, lower, upper);
-      scan_tokens<kRowThreads, 4>(row, 0, vocab, [&](int first, const float4& four) {
-        list_group(s.classes, scale, lower, upper, first, four,
-                   [&](uint32_t place, uint64_t key, uint64_t units, int) { s.cross.list[place] = Entry{key, units}; });
-      });
+      static_assert(sizeof(s.cross.bucket_mass) >= kListMost * sizeof(Held), "free until the crossings are looked for");
+      list_tokens<kRowThreads, 4>(s.classes, scale, lower, upper, row, 0, vocab, reinterpret_cast<Held*>(s.cross.bucket_mass),
+                                  [&](uint32_t place, uint64_t key, uint64_t units, int) { s.cross.list[place] = Entry{key, units}; });
+      __syncthreads();
       // (the crossings read an entry before they write the list again, with barriers in between)
       chosen = cross(s.cross, scale, ask, state, best, [&](int i) {
         const Entry entry = s.cross.list[i];
