@@ -13,9 +13,14 @@
 // of them are exact in any order, so atomics leave the result the same from call to call, class sums and token sums agree to the
 // unit, and a crossing is found in exactly one place.
 //
-// Four launches.  The first three take every row in parts: its maximum; weights into the parts' histograms; the classes in question (each
-// part's workgroup finds them again, which costs less than another launch) and their tokens into the row's list.  The fourth, a workgroup
-// a row, finds the crossings.
+// Two forms.  A row in parts, four launches: its maximum; weights into the parts' histograms; the classes in question (each part's workgroup finds
+// them again, which costs less than another launch) and their tokens into the row's list; and, a workgroup a row, the crossings.  Or all of
+// it by one workgroup a row.
+//
+// What bounds them.  Few rows: reads and sums that wait for one another (1 row of 32000 tokens 20 us, its four kernels 2.5, 4.4, 7.5 and 5.1).
+// Many: three readings of the row, the first from memory (64 rows of 128256, 33 MB: 5.4 us, 6.1 TB/s), and the 64-bit arithmetic of the
+// weights (13.9 us, of which 9.4 without it); then 17.5 us for the tokens in question and 7.4 for the crossings, 44 in all.  256 such rows by a
+// workgroup each: 21, 35, 19 (with the classes) and 3 us, 88 in all with what the slowest row takes longer.
 #include "common.h"
 
 namespace tlie {
@@ -105,7 +110,7 @@ __device__ __forceinline__ int gap_class(const RowScale& row, float v) {
 // exp((v - max) / T) in units of 2^-shift; one function, each operation written out, for every kernel that forms it.  The
 // exponent in steps of ln 2 / 1024 is a whole number n and a rest f of half a step at most: 2^(n / 1024) from the table and its exponent, exp of
 // the rest by its series to the third power (5.5e-16 of it is left).  10 operations on 64-bit floats, and a conversion: the processor's time is
-// what the weights of many rows take (256 rows of 128256 tokens MEASURED).
+// what the weights of many rows take (35 of 88 us for 256 rows of 128256 tokens; with 12 such operations 39).
 template <bool ALL>
 __device__ __forceinline__ double weight_wide(const PoweredScale<ALL>& row, float v) {
 #pragma clang fp contract(off)
@@ -191,13 +196,35 @@ constexpr int kDies = 8;
 __device__ __forceinline__ int row_of(int parts) { return static_cast<int>(blockIdx.x / kDies) / parts * kDies + static_cast<int>(blockIdx.x % kDies); }
 __device__ __forceinline__ int part_of(int parts) { return static_cast<int>(blockIdx.x / kDies) % parts; }
 
+// What a thread has seen of a row: its first largest token's group, the smallest logit (-inf too), and whether one is a NaN or +inf.  A group of
+// four is compared as one and kept whole, so that which of its tokens it is is asked once, at the end.
+struct Seen {
+  float most = -INFINITY, least = INFINITY;
+  float4 group = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  int first = 0;
+  bool bad = false;
+  __device__ __forceinline__ void take(int index, const float4& v) {
+    bad = bad || !(v.x < INFINITY) || !(v.y < INFINITY) || !(v.z < INFINITY) || !(v.w < INFINITY);
+    const float here = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+    least = fminf(fminf(least, fminf(v.x, v.y)), fminf(v.z, v.w));
+    const bool more = here > most;                                // (a thread meets its groups in the order of their tokens)
+    most = more ? here : most, first = more ? index : first;
+    group.x = more ? v.x : group.x, group.y = more ? v.y : group.y, group.z = more ? v.z : group.z;
+  }
+  __device__ __forceinline__ uint64_t best() const;
+};
+
 struct PartStat {
   uint64_t best;        // place_key of the part's first token in the order; 0: the part has none; all ones: a NaN or +inf
-  float min;            // the smallest finite logit, +inf: none
+  float min;            // the smallest logit, +inf: none
   uint32_t unused;
 };
 constexpr uint64_t kBadPart = ~0ull;
 constexpr uint32_t kNotListed = ~0u;
+__device__ __forceinline__ uint64_t Seen::best() const {
+  if (bad) return kBadPart;
+  return most > -INFINITY ? place_key(most, first + (group.x == most ? 0 : group.y == most ? 1 : group.z == most ? 2 : 3)) : 0;
+}
 
 __global__ void __launch_bounds__(kPartThreads)
 draw_best_kernel(const float* __restrict__ logits, int rows, int vocab, int part_len, int parts, PartStat* __restrict__ stats) {
@@ -205,18 +232,10 @@ draw_best_kernel(const float* __restrict__ logits, int rows, int vocab, int part
   __shared__ float min_of[kPartThreads / kWave];
   const int row = row_of(parts), part = part_of(parts), begin = part * part_len, end = min(vocab, begin + part_len);
   if (row >= rows) return;
-  float most = -INFINITY, least = INFINITY;
-  int at = 0;
-  bool bad = false;
-  scan_tokens<kPartThreads, 4>(logits + static_cast<size_t>(row) * vocab, begin, end, [&](int first, const float4& four) {
-    each_of(first, four, [&](int i, float v) {
-      bad = bad || !(v < INFINITY);
-      if (v > most) most = v, at = i;                             // (a thread meets its tokens in the order of their index)
-      least = v > -INFINITY ? fminf(least, v) : least;
-    });
-  });
-  uint64_t best = most > -INFINITY ? place_key(most, at) : 0;
-  if (bad) best = kBadPart;
+  Seen seen;
+  scan_tokens<kPartThreads, 4>(logits + static_cast<size_t>(row) * vocab, begin, end, [&](int first, const float4& four) { seen.take(first, four); });
+  uint64_t best = seen.best();
+  float least = seen.least;
   for (int offset = 32; offset > 0; offset >>= 1) {
     const uint64_t other = __shfl_xor(best, offset, 64);
     best = other > best ? other : best;
@@ -490,7 +509,8 @@ __device__ __forceinline__ void value_bounds(const ClassShared<THREADS>& s, cons
   const int c_first = s.found[5], c_last = kClasses - 1 - s.found[6];
   lower = -3.4028235e38f, upper = INFINITY;
   if (scale.class_scale > 0.f) {                                  // (else every token is of the first class)
-    const float room = fmaxf(fabsf(scale.max), fabsf(least)) * 2.4e-7f;
+    // (tokens that weigh lie within 34 T of the first; the smallest logit may be the least there is, or -inf)
+    const float room = (fabsf(scale.max) + fminf(scale.max - least, static_cast<float>(-scale.least))) * 2.4e-7f;
     upper = scale.max - static_cast<float>(c_first) * 0.99999f / scale.class_scale + room;
     if (c_last < kClasses - 1) lower = scale.max - static_cast<float>(c_last + 1) * 1.00001f / scale.class_scale - room;
   }
@@ -834,18 +854,10 @@ draw_row_kernel(const float* __restrict__ logits, int vocab, const float* __rest
   const float* row = logits + static_cast<size_t>(r) * vocab;
   const Ask ask = ask_of(r, uniform, temperature, top_k, top_p, min_p);
   // ---- the first token, the least logit, and whether the row can be drawn from ----
-  float most = -INFINITY, least = INFINITY;
-  int at = 0;
-  bool bad = false;
-  scan_tokens<kRowThreads, 4>(row, 0, vocab, [&](int first, const float4& four) {
-    each_of(first, four, [&](int i, float v) {
-      bad = bad || !(v < INFINITY);
-      if (v > most) most = v, at = i;
-      least = v > -INFINITY ? fminf(least, v) : least;
-    });
-  });
-  uint64_t best = most > -INFINITY ? place_key(most, at) : 0;
-  if (bad) best = kBadPart;
+  Seen seen;
+  scan_tokens<kRowThreads, 4>(row, 0, vocab, [&](int first, const float4& four) { seen.take(first, four); });
+  uint64_t best = seen.best();
+  float least = seen.least;
   for (int offset = 32; offset > 0; offset >>= 1) {
     const uint64_t other = __shfl_xor(best, offset, 64);
     best = other > best ? other : best;

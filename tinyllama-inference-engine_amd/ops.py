@@ -2122,13 +2122,14 @@ DRAW_ROW_BYTES, DRAW_PART_BYTES = 32 + 2048 * 40, 24 + 1024 * 12      # of scrat
 def draw_parts(rows: int, vocab: int) -> int:
     """Into how many parts `sample_filtered` cuts each row; 0: a row by one workgroup, in one launch instead of four.
 
-    One workgroup a row where the rows fill the chip or are short (1 row of 16000 tokens 19.2 us, in parts 20.6, of 32000 24.7 and 20.8; 64 of
-    32000 32.8 and 34.2, of 128256 85 and 53; 256 of 128256 94 and 112).  Else at most 8 parts, each brings a histogram to write and, by all
-    of them, to read: of 4096 tokens up to 16 rows, of 8192 beyond, a thousand workgroups at most (7 rows of 50261 in 8 parts 25 us, in 4 28;
-    64 rows of 128256 in 8 parts 53, in 4 61; 256 rows in 4 parts 112, in 8 128)."""
-    if vocab <= 512 * (rows + 40):
+    One workgroup a row where rows are short, or so many that parts find no idle compute units: 1 row of 16000 tokens 19.5 us either way, of 24000
+    23.3 and in parts 20.3; 64 of 24000 29.0 and 29.0, of 32000 32.0 and 30.3; 128 of 64000 44.4 and 45.4, of 128256 77 and 72; 192 of 128256 81
+    and 90, 256 88 and 112.  Else at most 8 parts, each brings a histogram to write and, by all of them, to read: of 4096 tokens up to 32
+    rows, of 8192 beyond, a thousand workgroups at most (32 rows of 32000 in 8 parts 27 us, in 4 30; 64 of 24000 in 4 29.0, in 8 29.4, of 128256
+    in 8 45, in 4 54)."""
+    if vocab <= 16000 + 7 * rows * rows // 2:
         return 0
-    return max(1, min(8, 1024 // max(rows, 1), -(-vocab // (4096 if rows <= 16 else 8192))))
+    return max(1, min(8, 1024 // max(rows, 1), -(-vocab // (4096 if rows <= 32 else 8192))))
 
 
 def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
