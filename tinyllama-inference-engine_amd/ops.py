@@ -2107,12 +2107,17 @@ def _address(tensor: torch.Tensor | None):
     return None if tensor is None else tensor.data_ptr()
 
 
-def _one_device(what: str, *tensors) -> None:
-    """All tensors (None: absent) lie on the current device, whose current stream the kernels go to."""
-    current = torch._C._cuda_getDevice()
-    for tensor in tensors:
-        if tensor is not None and tensor.device.index != current:
-            raise invalid_argument(f"{what}: a tensor lies on {tensor.device}, the current device is cuda:{current}")
+def _expect(what: str, inputs: tuple, optional: tuple = ()) -> int:
+    """Each of (tensor, name, dtype) is a contiguous tensor of the dtype on the current device, whose current stream the kernels go to (or, of the
+    optional ones, None); returns the device's index.  (One pass and no calls where all is well: a small call's time is the host's.)"""
+    current = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else None
+    for tensor, name, dtype in inputs + optional if optional else inputs:
+        if (isinstance(tensor, torch.Tensor) and tensor.is_cuda and tensor.dtype is dtype and tensor.is_contiguous() and tensor.get_device() == current
+                or tensor is None and any(entry[1] == name for entry in optional)):
+            continue
+        _device_tensor(tensor, name, dtype)
+        raise invalid_argument(f"{what}: {name} lies on {tensor.device}, the current device is cuda:{current}")
+    return current
 
 
 DRAW_MAX_VOCAB = (1 << 24) - 1
@@ -2147,24 +2152,20 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: to
     262144): what is lighter than half of that is never drawn, and the same inputs give the same token in any batch.
     logprobs: also returns float32 [rows], log softmax(logits)[token] of the logits as they are, without temperature and filters.
     out (int32 [rows]), out_logprobs (float32 [rows]): to write into, else new tensors."""
-    _device_tensor(logits, "logits", torch.float32)
+    current = _expect("sample_filtered", ((logits, "logits", torch.float32), (uniform, "uniform", torch.float32)),
+                      ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                       (min_p, "min_p", torch.float32), (out, "out", torch.int32), (out_logprobs, "out_logprobs", torch.float32)))
     if logits.dim() != 2:
         raise invalid_shape("sample_filtered takes logits [rows, vocab]")
     rows, vocab = logits.shape
     if not 0 < vocab <= DRAW_MAX_VOCAB or rows > 65535:
         raise invalid_shape(f"sample_filtered takes 1 to {DRAW_MAX_VOCAB} tokens and up to 65535 rows, not {list(logits.shape)}")
-    if uniform is None:
-        raise invalid_argument("sample_filtered needs a random number per row")
-    for name, tensor, dtype in (("uniform", uniform, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                                ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("out", out, torch.int32),
-                                ("out_logprobs", out_logprobs, torch.float32)):
-        if tensor is not None:
-            _device_tensor(tensor, name, dtype)
-            if tensor.shape != (rows,):
-                raise invalid_shape(f"sample_filtered: {name} needs one entry per row")
+    for name, tensor in (("uniform", uniform), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p), ("out", out),
+                         ("out_logprobs", out_logprobs)):
+        if tensor is not None and (tensor.dim() != 1 or tensor.shape[0] != rows):
+            raise invalid_shape(f"sample_filtered: {name} needs one entry per row")
     if out_logprobs is not None and not logprobs:
         raise invalid_argument("sample_filtered: out_logprobs goes with logprobs")
-    _one_device("sample_filtered", logits, uniform, temperature, top_k, top_p, min_p, out, out_logprobs)
     if out is None:
         out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
     if logprobs and out_logprobs is None:
@@ -2173,7 +2174,8 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: to
         parts = draw_parts(rows, vocab)
         scratch = torch.empty((rows * (DRAW_ROW_BYTES + parts * DRAW_PART_BYTES),), dtype=torch.uint8, device=logits.device) if parts else None
         _check(_entry("tlie_draw", "piipppppipppp")(logits.data_ptr(), rows, vocab, uniform.data_ptr(), _address(temperature), _address(top_k), _address(top_p),
-                                                    _address(min_p), parts, _address(scratch), out.data_ptr(), _address(out_logprobs), _stream()),
+                                                    _address(min_p), parts, _address(scratch), out.data_ptr(), _address(out_logprobs),
+                                                    torch._C._cuda_getCurrentRawStream(current)),
                "sample_filtered")
     return (out, out_logprobs) if logprobs else out
 
@@ -2895,27 +2897,24 @@ def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: t
     joins the softmax's denominator.  Rows of q that no sequence brings give zeros."""
     if (num_heads, num_kv_heads, head_dim, q.dtype) != plan.sizes:
         raise invalid_argument(f"attention_shared_prefix: the plan is for {plan.sizes}, not for {(num_heads, num_kv_heads, head_dim, q.dtype)}")
-    _device_tensor(q, "q", (torch.float32, torch.bfloat16))
-    _device_tensor(cache, "cache", q.dtype)
-    _device_tensor(block_table, "block_table", torch.int32)
-    _device_tensor(positions, "positions", torch.int32)
+    dtype = q.dtype
+    current = _expect("attention_shared_prefix", ((q, "q", dtype), (cache, "cache", dtype), (block_table, "block_table", torch.int32),
+                                                  (positions, "positions", torch.int32), (plan.items, "the plan", torch.int32)),
+                      ((sink, "sink", torch.float32),) if sink is not None else ())
     if softcap is not None and not ctypes.c_float(softcap).value > 0.0:
         raise invalid_argument("attention_shared_prefix: a cap of the scores must be positive")
-    if sink is not None:
-        _device_tensor(sink, "sink", torch.float32)
-        if sink.shape != (num_heads,):
-            raise invalid_shape("attention_shared_prefix: the sink needs one entry per query head")
+    if sink is not None and sink.shape != (num_heads,):
+        raise invalid_shape("attention_shared_prefix: the sink needs one entry per query head")
     if not scale > 0:
         raise invalid_argument(f"attention_shared_prefix: the scale {scale} of the scores is not positive")
-    tokens = q.shape[0]
-    if q.dim() != 2 or q.shape[1] != num_heads * head_dim or tokens != plan.tokens or positions.shape != (tokens,):
-        raise invalid_shape(f"attention_shared_prefix: q {list(q.shape)} and positions {list(positions.shape)} are not [{plan.tokens}, nq * d] and [{plan.tokens}]")
+    tokens = plan.tokens
+    if q.shape != (tokens, num_heads * head_dim) or positions.shape != (tokens,):
+        raise invalid_shape(f"attention_shared_prefix: q {list(q.shape)} and positions {list(positions.shape)} are not [{tokens}, nq * d] and [{tokens}]")
     page_size = _check_cache(cache, num_kv_heads, head_dim, "attention_shared_prefix")
     if head_dim % 16 != 0 or not 0 < head_dim <= ATTENTION_MAX_HEAD_DIM or not 16 <= page_size <= 65536 or page_size & (page_size - 1):
         raise invalid_argument("attention_shared_prefix takes head sizes in steps of 16 up to 256, pages of a power of two of rows (16 to 65536)")
     if block_table.dim() != 2 or block_table.shape[0] < plan.sequences or block_table.shape[1] * page_size < plan.longest:
         raise invalid_shape(f"attention_shared_prefix: block_table {list(block_table.shape)} does not hold {plan.sequences} sequences of up to {plan.longest} positions")
-    _one_device("attention_shared_prefix", q, cache, block_table, positions, plan.items, plan.part_first, sink)
     out = torch.empty_like(q)
     if tokens == 0:
         return out
@@ -2923,12 +2922,12 @@ def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: t
         return out.zero_()
     # the parts' results: their values (a part and head's at a multiple of 64 bytes), then their maxima and sums
     rows = plan.parts * num_heads
-    parts = torch.empty((rows * (head_dim + 2),), dtype=torch.float32, device=q.device)
+    parts = q.new_empty(rows * (head_dim + 2), dtype=torch.float32)
     address = parts.data_ptr()
     _check(_entry("tlie_attention_prefix", "ppipipippppppiiiiiffp")(
-        q.data_ptr(), cache.data_ptr(), dtype_code(q.dtype), block_table.data_ptr(), block_table.shape[1], plan.items.data_ptr(), plan.items.shape[0],
+        q.data_ptr(), cache.data_ptr(), dtype_code(dtype), block_table.data_ptr(), block_table.shape[1], plan.items.data_ptr(), plan.items.shape[0],
         positions.data_ptr(), plan.part_first.data_ptr(), address, address + rows * head_dim * 4, _address(sink), out.data_ptr(), tokens, num_heads,
-        num_kv_heads, head_dim, page_size, scale, softcap or 0.0, _stream()), "attention_shared_prefix")
+        num_kv_heads, head_dim, page_size, scale, softcap or 0.0, torch._C._cuda_getCurrentRawStream(current)), "attention_shared_prefix")
     return out
 
 
