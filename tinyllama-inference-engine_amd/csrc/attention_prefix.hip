@@ -38,26 +38,16 @@ constexpr int kPrefixWaves = 4;
 // heads: 70 us against 66).
 constexpr float kSlack = 6.f;
 
-// 128 neighbouring entries of a sequence's block table, two a lane: a block's page numbers come from registers, so that its keys and
-// values are asked for without waiting for a page number from memory first (3 us a block in the middle of a walk).
-struct TableWindow {
-  int first, low, high;
-  __device__ __forceinline__ void load(const int* __restrict__ pages, int max_blocks, int from) {
-    const int lane = threadIdx.x & 63;
-    first = from;
-    low = pages[min(from + lane, max_blocks - 1)];
-    high = pages[min(from + 64 + lane, max_blocks - 1)];
-  }
-  __device__ __forceinline__ int page(int index) const {          // index: the same for every lane, within the window
-    const int place = __builtin_amdgcn_readfirstlane(index - first);
-    const int a = __builtin_amdgcn_readlane(low, place & 63), b = __builtin_amdgcn_readlane(high, place & 63);
-    return place < 64 ? a : b;
-  }
-};
+// The page that position `key` lies on, of an item with keys on the pages page_lo .. page_hi; key is the same for every lane, so that the
+// number comes through the scalar cache, whose lines hold sixteen.  Rows of a page outside the item's keys are read with the others and
+// masked; pages that hold none of them are not: the first or last page of the keys is read again in their place, whatever the table says there.
+__device__ __forceinline__ int page_of(const int* __restrict__ pages, int key, int page_shift, int page_lo, int page_hi) {
+  return pages[__builtin_amdgcn_readfirstlane(min(max(key >> page_shift, page_lo), page_hi))];
+}
 
 template <int DT, bool FLOAT, int CT>
 __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, const void* __restrict__ q_any, const void* __restrict__ cache_any,
-                                            const int* __restrict__ pages, int max_blocks, const int* __restrict__ positions,
+                                            const int* __restrict__ pages, const int* __restrict__ positions,
                                             const int* __restrict__ part_first, float* __restrict__ part_o, float* __restrict__ part_ml,
                                             int nq, int nkv, int page_shift, float scale_log2, float cap_pre, float* lds) {
   using Elem = std::conditional_t<FLOAT, float, uint16_t>;
@@ -104,15 +94,12 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
     Piece k[TILES][KS];
     Values v[DT][TILES];
   };
-  // Rows of a page outside the item's keys are read with the others and masked; pages that hold none of them are not: the first or
-  // last page of the keys is read again in their place, whatever the table says there.
-  TableWindow window;
   const int page_lo = item.key_lo >> page_shift, page_hi = (item.key_hi - 1) >> page_shift;
   auto load = [&](int kb, Block& block) {
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
       const int first = kb + t * 16;
-      const int page = window.page(min(max(first >> page_shift, page_lo), page_hi));
+      const int page = page_of(pages, first, page_shift, page_lo, page_hi);
       const Elem* keys = k_base + (static_cast<size_t>(page) * page_stride + (first & page_mask)) * D;
       const Elem* values = v_base + static_cast<size_t>(page) * page_stride * D + (first & page_mask);
 #pragma unroll
@@ -261,21 +248,16 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
   // two blocks in registers: while one is worked on the other is on its way
   constexpr int kStride = BLOCK * kPrefixWaves;
   Block ring[2];
-  for (int begin = item.key_lo & ~31; begin < item.key_hi;) {
-    window.load(pages, max_blocks, begin >> page_shift);
-    const int end = min(item.key_hi, (window.first + 128) << page_shift);        // (a multiple of 32, or the item's)
-    const int mine_first = begin + BLOCK * wave, last = (end - 1) & ~(BLOCK - 1);
-    load(min(mine_first, last), ring[0]);
-    load(min(mine_first + kStride, last), ring[1]);
-    for (int kb = mine_first; kb < end; kb += 2 * kStride) {
+  const int mine_first = (item.key_lo & ~31) + BLOCK * wave, last = (item.key_hi - 1) & ~(BLOCK - 1);
+  load(min(mine_first, last), ring[0]);
+  load(min(mine_first + kStride, last), ring[1]);
+  for (int kb = mine_first; kb < item.key_hi; kb += 2 * kStride) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int mine = kb + r * kStride;
-        if (mine < end) work(mine, ring[r]);
-        load(min(mine + 2 * kStride, last), ring[r]);              // (past the last block the last again: as many loads on every path)
-      }
+    for (int r = 0; r < 2; ++r) {
+      const int mine = kb + r * kStride;
+      if (mine < item.key_hi) work(mine, ring[r]);
+      load(min(mine + 2 * kStride, last), ring[r]);                // (past the last block the last again: as many loads on every path)
     }
-    begin = end;
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -335,7 +317,7 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
 // are spread over the banks; values as [half of 16 keys][16 dims][4 keys][dim], of which a read takes 512 bytes in the order of the lanes.
 template <int DT, int CT>
 __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh, const uint16_t* __restrict__ q, const uint16_t* __restrict__ cache,
-                                                 const int* __restrict__ pages, int max_blocks, const int* __restrict__ positions,
+                                                 const int* __restrict__ pages, const int* __restrict__ positions,
                                                  const int* __restrict__ part_first, float* __restrict__ part_o, float* __restrict__ part_ml,
                                                  int nq, int nkv, int page_shift, float scale_log2, float cap_pre, unsigned char* lds) {
   constexpr int D = DT * 16, KS = (DT + 1) / 2, kPieces = 2 * DT;           // pieces of a key
@@ -398,11 +380,10 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
   auto is_values = [&](int i) { return kAlike ? i >= 2 : min(wave + 4 * i, 2 * DT - 1) >= DT; };       // (the same for the whole wave)
   auto to_of = [&](int i) { return kAlike ? to[i >> 1] + (i & 1) * (kBytes / 2) : to[i]; };
   Piece staged[2][kCalls];
-  TableWindow window;
-  const int page_lo = item.key_lo >> page_shift, page_hi = (item.key_hi - 1) >> page_shift;       // (as above: other entries of the table are not followed)
+  const int page_lo = item.key_lo >> page_shift, page_hi = (item.key_hi - 1) >> page_shift;
   auto bring = [&](int kb, Piece (&into)[kCalls]) {
-    const size_t at_a = static_cast<size_t>(window.page(max(kb >> page_shift, page_lo))) * page_stride * D;
-    const size_t at_b = static_cast<size_t>(window.page(min(max((kb + 16) >> page_shift, page_lo), page_hi))) * page_stride * D;
+    const size_t at_a = static_cast<size_t>(page_of(pages, kb, page_shift, page_lo, page_hi)) * page_stride * D;
+    const size_t at_b = static_cast<size_t>(page_of(pages, kb + 16, page_shift, page_lo, page_hi)) * page_stride * D;
     const int row_a = kb & page_mask, row_b = (kb + 16) & page_mask;
     const uint16_t *keys_a = k_base + at_a + row_a * D, *keys_b = k_base + at_b + row_b * D;
     const uint16_t *values_a = v_base + at_a + row_a, *values_b = v_base + at_b + row_b;
@@ -549,24 +530,20 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
     }
   };
   int buffer = 0;
-  for (int begin = item.key_lo & ~31; begin < item.key_hi;) {
-    window.load(pages, max_blocks, begin >> page_shift);
-    const int end = min(item.key_hi, (window.first + 128) << page_shift), last = (end - 1) & ~31;
-    bring(begin, staged[0]);
-    bring(min(begin + 32, last), staged[1]);
-    for (int kb = begin; kb <= last; kb += 64) {
-      unsigned char* place = lds + buffer * 4 * kBytes;
-      put(place, staged[0]);
-      put(place + 2 * kBytes, staged[1]);
-      lds_barrier();
-      bring(min(kb + 64, last), staged[0]);                    // (past the last block the last again: as many loads on every path)
-      bring(min(kb + 96, last), staged[1]);
+  const int begin = item.key_lo & ~31, last = (item.key_hi - 1) & ~31;
+  bring(begin, staged[0]);
+  bring(min(begin + 32, last), staged[1]);
+  for (int kb = begin; kb <= last; kb += 64) {
+    unsigned char* place = lds + buffer * 4 * kBytes;
+    put(place, staged[0]);
+    put(place + 2 * kBytes, staged[1]);
+    lds_barrier();
+    bring(min(kb + 64, last), staged[0]);                      // (past the last block the last again: as many loads on every path)
+    bring(min(kb + 96, last), staged[1]);
 #pragma unroll 1
-      for (int u = 0; u < 2; ++u)
-        if (kb + 32 * u <= last && kb + 32 * u < high) work(kb + 32 * u, place + u * 2 * kBytes);
-      buffer ^= 1;
-    }
-    begin = end;
+    for (int u = 0; u < 2; ++u)
+      if (kb + 32 * u <= last && kb + 32 * u < high) work(kb + 32 * u, place + u * 2 * kBytes);
+    buffer ^= 1;
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -612,7 +589,7 @@ prefix_items_kernel(const void* __restrict__ q, const void* __restrict__ cache, 
   if (item.ntok <= 0) return;                                  // a list of fixed size ends in items without tokens
   const int* pages = block_table + static_cast<size_t>(item.table) * max_blocks;
   const int columns = item.ntok * (nq / nkv) - item.col0;      // (of the tile and those behind it)
-#define TLIE_ARGS max_blocks, positions, part_first, part_o, part_ml, nq, nkv, page_shift, scale_log2, cap_pre
+#define TLIE_ARGS positions, part_first, part_o, part_ml, nq, nkv, page_shift, scale_log2, cap_pre
   if constexpr (FLOAT) {
     if (kFloatWide > 1 && columns > 16)
       prefix_item<DT, true, kFloatWide>(item, kvh, q, cache, pages, TLIE_ARGS, reinterpret_cast<float*>(lds));
