@@ -34,8 +34,8 @@ struct PrefixItem {
 
 constexpr int kPrefixWaves = 4;
 // Powers may grow to 2^6 before what they are relative to moves: sums and values are float, and the rounding of a probability to
-// bfloat16 is relative.  Without slack a wave of 32 columns rescales in almost every block of an item (30000 keys, 128 columns on 8 key
-// heads: 70 us against 66).
+// bfloat16 is relative.  Without slack a wave of 32 columns rescales in almost every block of an item (eight
+// questions behind 4000 positions 59 us against 56, three documents with capped scores 15.0 against 14.0).
 constexpr float kSlack = 6.f;
 
 // The page that position `key` lies on, of an item with keys on the pages page_lo .. page_hi; key is the same for every lane, so that the
@@ -315,6 +315,13 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
 // that one barrier a turn is enough (a wave writes a buffer again only behind the barrier that every wave reaches after it has read it).
 // Keys lie as [key][piece of 16 bytes], a key's pieces rotated by key / kPeriod so that the 16 keys that a read takes the same piece of
 // are spread over the banks; values as [half of 16 keys][16 dims][4 keys][dim], of which a read takes 512 bytes in the order of the lanes.
+//
+// What bounds it.  128 columns of 128 dims: no one thing; of 43 us (8 questions of some 46 tokens behind 4000 positions, 24.5 GFLOP, 20 us at the
+// rate of a large product) bringing the keys takes 18 by itself, and without the scores' products, the values', or the exponentials 5, 7
+// and 2 us are saved.  32 sequences behind 30000 positions, keys from memory: bringing them 37 of 40 us (3.4 TB/s: two workgroups a
+// compute unit have 64 KB on their way, and wait for a turn's last piece before they ask for the next).  The parts' results cost 5 us to
+// write and 7 to join in both.  Eight waves a workgroup that leave one result between them halve
+// that but take longer: one workgroup a unit, all its waves at the same barriers (56 against 51 us, 49 against 46, 64 sequences behind 6000 43 against 35).
 template <int DT, int CT>
 __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh, const uint16_t* __restrict__ q, const uint16_t* __restrict__ cache,
                                                  const int* __restrict__ pages, const int* __restrict__ positions,
@@ -686,14 +693,13 @@ static double tile_cost(int columns) { return columns <= 32 ? 1.0 : columns <= 6
 
 constexpr int kLeastKeys = 128;      // that a part has, if the whole has as many
 
-// Parts of about equal cost: a workgroup a compute unit, two where they are long (a part more is a result more to write and to join; 64 sequences
-// behind 6000 positions, 32 heads of 128 on 8: 35.6 us in 12 parts, 45 in 23; 2 behind 8000 15.8 in 32, 21 in 64; eight questions behind
-// 4000 51 in 6 parts, 56 in 4).
-// A sixteenth of the units stays free for what the cuts leave over: 2 behind 8000 in one part more than there are units for 15.9 us, in two
-// fewer 13.2.
+// Parts of about equal cost: a workgroup a compute unit, two where they are long.  A part more is a result more to write and to join, and
+// memory's time where a prefix is long: 32 sequences behind 30000 positions, 32 heads of 128 on 8, their keys not in any cache, 46.9 us in 47 parts,
+// 52.8 in 53, 50.6 in 40; eight questions behind 4000 51 in 5 parts, 57 in 4, 66 in 6.  A sixteenth of the units stays free for what the
+// cuts leave over: 2 behind 8000 in one part more than there are units for 15.9 us, in two fewer 13.2.
 static double part_cost(double total, int compute_units) {
   const double units = 0.9375 * compute_units;
-  return std::max(total / (2.0 * units), std::min(total / units, 2600.0));
+  return std::max(total / (2.0 * units), std::min(total / units, 3200.0));
 }
 
 struct Cut {
@@ -703,7 +709,7 @@ struct Cut {
 static Cut cut_keys(long long keys, int columns, double budget, int most_parts) {
   const long long by_cost = std::llrint(static_cast<double>(keys) * tile_cost(columns) / std::max(budget, 1.0));
   const long long count = std::max(1ll, std::min({(keys + kLeastKeys - 1) / kLeastKeys, by_cost, static_cast<long long>(most_parts)}));
-  // whole turns of a workgroup: wide tiles take two blocks of 32 keys each (32 sequences behind 30000 positions in parts of 544 keys 45.7 us, of 576 42.7)
+  // whole turns of a workgroup: wide tiles take two blocks of 32 keys each (32 sequences behind 30000 positions, keys in the caches: in parts of 544 keys 45.7 us, of 576 42.7)
   const long long turn = columns > 32 ? 64 : 32, part = ((keys + count - 1) / count + turn - 1) / turn * turn;
   return Cut{part, (keys + part - 1) / part};
 }
