@@ -2829,8 +2829,8 @@ def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads:
 
 def shared_prefix_pays(groups, num_kv_heads: int, head_dim: int) -> bool:
     """Whether a decode step of these groups is faster through `attention_shared_prefix` than through `attention_mfma`: from four million
-    elements of keys on that are not read again (32 heads of 64 on 4, 64 sequences behind 1024 positions 13.4 us against 12.5, behind 2048 16.1 against 18.4;
-    of 128 on 8, 2 behind 1024 10.5 and 10.4, 8 behind 1024 10.0 against 13.6, 64 behind 2048 20.6 against 56.7; on 32, 4 behind 256 10.5 and 10.3)."""
+    elements of keys on that are not read again (32 heads of 64 on 4, 64 sequences behind 1024 positions 13.6 us against 12.5, behind 2048 15.9 against 18.8;
+    of 128 on 8, 2 behind 1024 10.4 and 10.2, 8 behind 1024 10.0 against 13.8, 64 behind 2048 19.7 against 56.9; on 32, 4 behind 256 10.6 and 10.3)."""
     return sum((count - 1) * prefix for _, count, prefix in groups) * num_kv_heads * head_dim >= 4_000_000
 
 
