@@ -260,3 +260,20 @@ def test_more_logits_than_32_bits_count():
     got = ops.sample_filtered(logits, numbers, **spread)
     assert torch.equal(got[-8:], ops.sample_filtered(few.to(DEV), uniform.to(DEV), **filters))
     assert not got[:-8].any()
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 1001), (3, 1002), (2, 60001), (2, 60003)])
+def test_the_first_of_equal_maxima_wherever_they_stand(rows, vocab):
+    """The largest logit at two places, one of them in the last, cut group of four tokens, the other at every place of the first
+    groups; also with rows that start past a multiple of 16 bytes (every row but the first of an odd vocabulary)."""
+    places = list(range(12)) + [511 * 4, 512 * 4, vocab // 2, vocab - 2]
+    for place in places:
+        if place >= vocab - 1:
+            continue
+        logits = torch.zeros((rows, vocab))
+        logits[:, place], logits[:, vocab - 1] = 3.0, 3.0
+        zero = torch.zeros(rows, device=DEV)
+        got = ops.sample_filtered(logits.to(DEV), zero)
+        assert got.tolist() == [place] * rows, place
+        got = ops.sample_filtered(logits.to(DEV), zero, torch.full((rows,), 0.1, device=DEV), top_k=torch.ones(rows, dtype=torch.int32, device=DEV))
+        assert got.tolist() == [place] * rows, place

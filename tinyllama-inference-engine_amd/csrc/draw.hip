@@ -207,7 +207,7 @@ struct Seen {
     bad = bad || !(v.x < INFINITY) || !(v.y < INFINITY) || !(v.z < INFINITY) || !(v.w < INFINITY);
     const float here = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
     least = fminf(fminf(least, fminf(v.x, v.y)), fminf(v.z, v.w));
-    const bool more = here > most;                                // (a thread meets its groups in the order of their tokens)
+    const bool more = here > most || (here == most && index < first);      // (a thread may meet the range's last, cut group before others)
     most = more ? here : most, first = more ? index : first;
     group.x = more ? v.x : group.x, group.y = more ? v.y : group.y, group.z = more ? v.z : group.z;
   }
