@@ -196,7 +196,7 @@ constexpr int kDies = 8;
 __device__ __forceinline__ int row_of(int parts) { return static_cast<int>(blockIdx.x / kDies) / parts * kDies + static_cast<int>(blockIdx.x % kDies); }
 __device__ __forceinline__ int part_of(int parts) { return static_cast<int>(blockIdx.x / kDies) % parts; }
 
-// What a thread has seen of a row: its first largest token's group, the smallest logit (-inf too), and whether one is a NaN or +inf.  A group of
+// What a thread has seen of a row: its first largest token's group, the smallest finite logit, and whether one is a NaN or +inf.  A group of
 // four is compared as one and kept whole, so that which of its tokens it is is asked once, at the end.
 struct Seen {
   float most = -INFINITY, least = INFINITY;
@@ -206,7 +206,12 @@ struct Seen {
   __device__ __forceinline__ void take(int index, const float4& v) {
     bad = bad || !(v.x < INFINITY) || !(v.y < INFINITY) || !(v.z < INFINITY) || !(v.w < INFINITY);
     const float here = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-    least = fminf(fminf(least, fminf(v.x, v.y)), fminf(v.z, v.w));
+    float low = fminf(fminf(v.x, v.y), fminf(v.z, v.w));
+    if (low == -INFINITY) {                                       // (a token that cannot be drawn, or none: of the others)
+      const float none = INFINITY;
+      low = fminf(fminf(v.x > -INFINITY ? v.x : none, v.y > -INFINITY ? v.y : none), fminf(v.z > -INFINITY ? v.z : none, v.w > -INFINITY ? v.w : none));
+    }
+    least = fminf(least, low);
     const bool more = here > most || (here == most && index < first);      // (a thread may meet the range's last, cut group before others)
     most = more ? here : most, first = more ? index : first;
     group.x = more ? v.x : group.x, group.y = more ? v.y : group.y, group.z = more ? v.z : group.z;
@@ -216,7 +221,7 @@ struct Seen {
 
 struct PartStat {
   uint64_t best;        // place_key of the part's first token in the order; 0: the part has none; all ones: a NaN or +inf
-  float min;            // the smallest logit, +inf: none
+  float min;            // the smallest finite logit, +inf: none
   uint32_t unused;
 };
 constexpr uint64_t kBadPart = ~0ull;
@@ -509,7 +514,7 @@ __device__ __forceinline__ void value_bounds(const ClassShared<THREADS>& s, cons
   const int c_first = s.found[5], c_last = kClasses - 1 - s.found[6];
   lower = -3.4028235e38f, upper = INFINITY;
   if (scale.class_scale > 0.f) {                                  // (else every token is of the first class)
-    // (tokens that weigh lie within 34 T of the first; the smallest logit may be the least there is, or -inf)
+    // (tokens that weigh lie within 34 T of the first; the smallest logit may be the least there is)
     const float room = (fabsf(scale.max) + fminf(scale.max - least, static_cast<float>(-scale.least))) * 2.4e-7f;
     upper = scale.max - static_cast<float>(c_first) * 0.99999f / scale.class_scale + room;
     if (c_last < kClasses - 1) lower = scale.max - static_cast<float>(c_last + 1) * 1.00001f / scale.class_scale - room;
