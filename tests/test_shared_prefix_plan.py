@@ -84,6 +84,25 @@ def test_a_prefix_is_read_through_a_sequence_that_holds_it():
     assert items[items[:, 6] == 0][:, 0].tolist() == [1] and part_first.tolist() == [0, 2, 4]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 4, 64), (32, 8, 128), (8, 8, 256), (40, 1, 64), (150, 1, 128), (12, 4, 48)])
+def test_a_recorded_plan_holds_any_step_of_single_tokens(heads, kv_heads, dim, dtype):
+    """Cut into one part each, which is what it comes down to when more do not fit."""
+    rng = random.Random(dim)
+    for tokens in (1, 2, 3, 8, 16, 33, 64, 256):
+        items_held, parts_held = ops.RecordedPrefixPlan.room(tokens, heads, kv_heads, dim, dtype)
+        for largest in (2, 3, tokens):
+            groups, at, lengths = [], 0, []
+            while at < tokens:
+                count = min(tokens - at, rng.randint(2, max(2, largest)))
+                prefix = rng.choice([1, 100, 20000])
+                groups.append((at, count, prefix))
+                lengths += [prefix + rng.choice([1, 700, 9000]) for _ in range(count)]
+                at += count
+            items, part_first = ops.shared_prefix_items(range(tokens + 1), lengths, groups, heads, kv_heads, dim, dtype, 256, 1)
+            assert items.shape[0] <= items_held and part_first[-1] <= parts_held
+
+
 def test_other_types_are_refused():
     with pytest.raises(EngineError):
         ops.shared_prefix_plan([0, 1], [4], [], 8, 4, 64, torch.float16, "cpu")

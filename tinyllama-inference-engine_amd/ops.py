@@ -2791,7 +2791,10 @@ def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads
     seq_start, seq_len = np.ascontiguousarray(seq_start, dtype=np.int64), np.ascontiguousarray(seq_len, dtype=np.int64)
     if seq_start.ndim != 1 or seq_len.ndim != 1 or seq_start.shape[0] != seq_len.shape[0] + 1:
         raise invalid_shape("shared_prefix_plan takes seq_start [sequences + 1] and seq_len [sequences]")
-    groups = np.array(sorted(groups), dtype=np.int64).reshape(-1, 3)
+    groups = sorted(tuple(group) for group in groups)
+    if any(len(group) != 3 for group in groups):
+        raise invalid_shape("shared_prefix_plan: a group is (first sequence, sequences, prefix)")
+    groups = np.array(groups, dtype=np.int64).reshape(-1, 3)
     given = items is not None
     if not given:
         items = np.empty((256, 8), dtype=np.int32)
@@ -2838,11 +2841,15 @@ class RecordedPrefixPlan:
     """A `SharedPrefixPlan` at fixed addresses and of fixed size, for a recorded step of up to `tokens` single tokens: `fill` writes a
     step's work into it.  Items and parts beyond the step's have no tokens."""
 
-    def __init__(self, tokens: int, longest: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device):
+    @staticmethod
+    def room(tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype) -> tuple[int, int]:
+        """(items, parts) that it holds.  With one part each, a token has ceil(G / step) items of its own and the groups ceil(columns / step) each;
+        room for parts beside."""
         group, step = num_heads // num_kv_heads, prefix_tile_columns(17, head_dim, dtype)
-        # with one part each, a token has ceil(G / step) items of its own and the groups ceil(columns / step) each; room for parts beside
-        self.items = tokens * -(-group // step) + -(-tokens * group // step) + tokens // 2 + 64
-        self.parts = tokens * 24 + 256
+        return tokens * -(-group // step) + -(-tokens * group // step) + tokens // 2 + 64, tokens * 24 + 256
+
+    def __init__(self, tokens: int, longest: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device):
+        self.items, self.parts = self.room(tokens, num_heads, num_kv_heads, head_dim, dtype)
         self._host = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, pin_memory=True)
         self._device = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, device=device)
         self._units = _compute_units(self._device.device)
