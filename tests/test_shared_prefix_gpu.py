@@ -18,6 +18,13 @@ DEV = "cuda:0"
 BF16, F32 = torch.bfloat16, torch.float32
 
 
+@pytest.fixture(autouse=True, params=["as it comes", "cut into parts"])
+def form(request, monkeypatch):
+    """Short steps run in one launch; every step also runs cut into parts."""
+    if request.param == "cut into parts":
+        monkeypatch.setattr(ops, "direct_prefix_items", lambda *step: None)
+
+
 def make_step(seed, dtype, heads, kv_heads, dim, page, sequences, groups, fill=1.0):
     """sequences: (length after the step, tokens it brings).  Sequences of a group have the pages of whole blocks of their prefix in
     common, and a copy of the prefix's rows on the page where it ends."""

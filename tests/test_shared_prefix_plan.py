@@ -116,3 +116,32 @@ def test_arguments_on_the_host_are_refused():
     with pytest.raises(EngineError):
         ops.attention_shared_prefix(torch.zeros(1, 32), torch.zeros(1, 2, 1, 256), torch.zeros(1, 1, dtype=torch.int32),
                                     torch.zeros(1, dtype=torch.int32), plan, 2, 1, 16, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 4, 64), (4, 2, 16), (40, 1, 64), (12, 4, 48)])
+def test_the_items_of_short_steps_cover_every_column_once(heads, kv_heads, dim, dtype):
+    rng, group, short = random.Random(dim), heads // kv_heads, 0
+    for _ in range(60):
+        start, lengths, groups, prefix = drawn_step(rng)
+        items = ops.direct_prefix_items(start, lengths, groups, heads, kv_heads, dim, dtype, 256)
+        if items is None:
+            continue
+        short += 1
+        assert items.shape[0] * kv_heads <= 256
+        seen = set()
+        for sequence, tok0, tokens, col0, shared, end, own, reader in items.tolist():
+            assert own == 1 and tok0 == start[sequence] and tokens == start[sequence + 1] - start[sequence] and shared == prefix[sequence]
+            assert lengths[reader] >= shared and (reader == sequence or any(a <= reader <= sequence < a + b for a, b, _ in groups))
+            for column in range(col0, min(col0 + 16, tokens * group)):
+                seen.add((sequence, column))
+                assert end > lengths[sequence] - tokens + column // group        # the token's own key is among them
+        assert len(seen) == int(start[-1]) * group
+    assert short > 0
+
+
+def test_long_steps_and_wide_heads_are_cut():
+    plan = lambda length, dim, dtype=torch.bfloat16, count=4: ops.direct_prefix_items(range(count + 1), [length] * count, [(0, count, length - 1)], 32, 4, dim, dtype, 256)
+    assert plan(700, 64) is not None and plan(1000, 64) is None
+    assert plan(300, 64, torch.float32) is not None and plan(700, 64, torch.float32) is None
+    assert plan(100, 128) is None and plan(100, 64, count=65) is None

@@ -32,7 +32,7 @@ struct PrefixItem {
   int table, tok0, ntok, col0, key_lo, key_hi, own, part;
 };
 
-constexpr int kPrefixWaves = 4;
+constexpr int kPrefixWaves = 4, kDirectWaves = 8;
 // Powers may grow to 2^6 before what they are relative to moves: sums and values are float, and the rounding of a probability to
 // bfloat16 is relative.  Without slack a wave of 32 columns rescales in almost every block of an item (eight
 // questions behind 4000 positions 59 us against 56, three documents with capped scores 15.0 against 14.0).
@@ -45,8 +45,16 @@ __device__ __forceinline__ int page_of(const int* __restrict__ pages, int key, i
   return pages[__builtin_amdgcn_readfirstlane(min(max(key >> page_shift, page_lo), page_hi))];
 }
 
-template <int DT, bool FLOAT, int CT>
-__device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, const void* __restrict__ q_any, const void* __restrict__ cache_any,
+// Where an item that leaves its columns' results themselves has them go, and the keys 0 .. shared - 1 that it reads through another row.
+struct Direct {
+  const int* pages;
+  int shared;
+  const float* sink;
+  void* out;
+};
+
+template <int DT, bool FLOAT, int CT, int WAVES, bool DIRECT>
+__device__ __forceinline__ void prefix_item(const PrefixItem& item, const Direct& direct, int kvh, const void* __restrict__ q_any, const void* __restrict__ cache_any,
                                             const int* __restrict__ pages, const int* __restrict__ positions,
                                             const int* __restrict__ part_first, float* __restrict__ part_o, float* __restrict__ part_ml,
                                             int nq, int nkv, int page_shift, float scale_log2, float cap_pre, float* lds) {
@@ -82,8 +90,8 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
         query[ct][ks] = *reinterpret_cast<const Piece*>(q + (static_cast<size_t>(tok[ct]) * nq + head[ct]) * D + (ks * 4 + grp) * kPiece);
     }
   }
-  // keys that every column of the item sees are [open_lo, open_hi): blocks inside need no mask
-  const int open_lo = item.key_lo, open_hi = item.own ? min(item.key_hi, pos0 + item.col0 / G + 1) : item.key_hi;
+  // keys that every column of the item sees end at open_hi: blocks inside need no mask
+  const int open_hi = item.own ? min(item.key_hi, pos0 + item.col0 / G + 1) : item.key_hi;
 
   const size_t page_stride = static_cast<size_t>(2 * nkv) << page_shift;    // in rows of D
   const Elem* k_base = cache + (static_cast<size_t>(kvh) << page_shift) * D;
@@ -94,12 +102,18 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
     Piece k[TILES][KS];
     Values v[DT][TILES];
   };
-  const int page_lo = item.key_lo >> page_shift, page_hi = (item.key_hi - 1) >> page_shift;
-  auto load = [&](int kb, Block& block) {
+  // the item's blocks: those of the keys that it reads through another row first
+  const int shared_keys = DIRECT ? direct.shared : 0, shared_blocks = (shared_keys + BLOCK - 1) / BLOCK, begin = item.key_lo & ~31;
+  auto is_shared = [&](int index) { return DIRECT && index < shared_blocks; };
+  auto key_of = [&](int index) { return is_shared(index) ? index * BLOCK : begin + (index - shared_blocks) * BLOCK; };
+  auto load = [&](int index, Block& block) {
+    const int kb = key_of(index);
+    const int* from = is_shared(index) ? direct.pages : pages;
+    const int page_lo = (is_shared(index) ? 0 : item.key_lo) >> page_shift, page_hi = ((is_shared(index) ? shared_keys : item.key_hi) - 1) >> page_shift;
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
       const int first = kb + t * 16;
-      const int page = page_of(pages, first, page_shift, page_lo, page_hi);
+      const int page = page_of(from, first, page_shift, page_lo, page_hi);
       const Elem* keys = k_base + (static_cast<size_t>(page) * page_stride + (first & page_mask)) * D;
       const Elem* values = v_base + static_cast<size_t>(page) * page_stride * D + (first & page_mask);
 #pragma unroll
@@ -120,8 +134,9 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
     for (int dt = 0; dt < DT; ++dt) o[ct][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto work = [&](int kb, Block& block) {
-    const bool ragged = kb < open_lo || kb + BLOCK > open_hi;     // (the same for the whole wave)
+  auto work = [&](int index, Block& block) {
+    const int kb = key_of(index), key_lo = is_shared(index) ? 0 : item.key_lo, key_hi = is_shared(index) ? shared_keys : item.key_hi;
+    const bool ragged = kb < key_lo || kb + BLOCK > (is_shared(index) ? shared_keys : open_hi);     // (the same for the whole wave)
     if (ragged) {
       // rows that are not the item's may hold anything: 0 * NaN must not arise
 #pragma unroll
@@ -131,7 +146,7 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = kb + t * 16 + grp * 4 + j;
-            const bool out = key < item.key_lo || key >= item.key_hi;
+            const bool out = key < key_lo || key >= key_hi;
             if constexpr (FLOAT) block.v[dt][t][j] = out ? 0u : block.v[dt][t][j];
             else block.v[dt][t][j >> 1] &= out ? ((j & 1) ? 0x0000ffffu : 0xffff0000u) : 0xffffffffu;
           }
@@ -175,7 +190,7 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = kb + t * 16 + grp * 4 + j;
-            s[ct][t][j] = key >= item.key_lo && key < item.key_hi && key <= last_key[ct] ? s[ct][t][j] : -INFINITY;
+            s[ct][t][j] = key >= key_lo && key < key_hi && key <= last_key[ct] ? s[ct][t][j] : -INFINITY;
           }
     }
     float lane_top[CT];
@@ -246,17 +261,16 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
   };
 
   // two blocks in registers: while one is worked on the other is on its way
-  constexpr int kStride = BLOCK * kPrefixWaves;
   Block ring[2];
-  const int mine_first = (item.key_lo & ~31) + BLOCK * wave, last = (item.key_hi - 1) & ~(BLOCK - 1);
-  load(min(mine_first, last), ring[0]);
-  load(min(mine_first + kStride, last), ring[1]);
-  for (int kb = mine_first; kb < item.key_hi; kb += 2 * kStride) {
+  const int blocks = shared_blocks + (item.key_hi - begin + BLOCK - 1) / BLOCK;
+  load(min(wave, blocks - 1), ring[0]);
+  load(min(wave + WAVES, blocks - 1), ring[1]);
+  for (int index = wave; index < blocks; index += 2 * WAVES) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int mine = kb + r * kStride;
-      if (mine < item.key_hi) work(mine, ring[r]);
-      load(min(mine + 2 * kStride, last), ring[r]);                // (past the last block the last again: as many loads on every path)
+      const int mine = index + r * WAVES;
+      if (mine < blocks) work(mine, ring[r]);
+      load(min(mine + 2 * WAVES, blocks - 1), ring[r]);            // (past the last block the last again: as many loads on every path)
     }
   }
 #pragma unroll
@@ -269,7 +283,7 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
   // The waves' results into one: every wave brings its own onto the common maximum; then, one column group after the other, the
   // values meet in LDS and each wave adds up a quarter of the dims, in the order of the waves.
   float* stats = lds;                                          // [waves][CT][16][2]
-  float* slots = lds + kPrefixWaves * CT * 32;                 // [waves][DT][64][4]
+  float* slots = lds + WAVES * CT * 32;                 // [waves][DT][64][4]
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct)
     if (grp == 0) {
@@ -281,10 +295,10 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
   for (int ct = 0; ct < CT; ++ct) {
     float most = -INFINITY, total = 0.f;
 #pragma unroll
-    for (int w = 0; w < kPrefixWaves; ++w) most = fmaxf(most, stats[((w * CT + ct) * 16 + col) * 2]);
+    for (int w = 0; w < WAVES; ++w) most = fmaxf(most, stats[((w * CT + ct) * 16 + col) * 2]);
     const float below = most == -INFINITY ? 0.f : most;
 #pragma unroll
-    for (int w = 0; w < kPrefixWaves; ++w)
+    for (int w = 0; w < WAVES; ++w)
       total += __builtin_amdgcn_exp2f(stats[((w * CT + ct) * 16 + col) * 2] - below) * stats[((w * CT + ct) * 16 + col) * 2 + 1];
     const float down = __builtin_amdgcn_exp2f(top[ct] - below);
     if (ct > 0) __syncthreads();                               // (the slots have been read)
@@ -293,20 +307,37 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, int kvh, con
       *reinterpret_cast<float4*>(slots + ((wave * DT + dt) * 64 + lane) * 4) =
           make_float4(o[ct][dt][0] * down, o[ct][dt][1] * down, o[ct][dt][2] * down, o[ct][dt][3] * down);
     __syncthreads();
-    // (a token that stands before the others of its tile may have fewer parts than they)
-    const int first_part = part_first[tok[ct]];
-    if (!valid[ct] || item.part >= part_first[tok[ct] + 1] - first_part) continue;
-    const size_t slot = static_cast<size_t>(first_part + item.part) * nq + head[ct];
-    for (int dt = wave; dt < DT; dt += kPrefixWaves) {
+    size_t slot = static_cast<size_t>(tok[ct]) * nq + head[ct];
+    float scale_out = 1.f;
+    if constexpr (DIRECT) {
+      if (!valid[ct]) continue;
+      const float own = direct.sink != nullptr ? direct.sink[head[ct]] * 1.4426950408889634f : -INFINITY;
+      const float end = fmaxf(most, own), under = end == -INFINITY ? 0.f : end, weight = __builtin_amdgcn_exp2f(most - under);
+      const float whole = total * weight + (direct.sink != nullptr ? __builtin_amdgcn_exp2f(own - under) : 0.f);
+      scale_out = whole > 0.f ? weight / whole : 0.f;
+    } else {
+      // (a token that stands before the others of its tile may have fewer parts than they)
+      const int first_part = part_first[tok[ct]];
+      if (!valid[ct] || item.part >= part_first[tok[ct] + 1] - first_part) continue;
+      slot = static_cast<size_t>(first_part + item.part) * nq + head[ct];
+    }
+    for (int dt = wave; dt < DT; dt += WAVES) {
       float4 all = *reinterpret_cast<const float4*>(slots + (dt * 64 + lane) * 4);
 #pragma unroll
-      for (int w = 1; w < kPrefixWaves; ++w) {
+      for (int w = 1; w < WAVES; ++w) {
         const float4 more = *reinterpret_cast<const float4*>(slots + ((w * DT + dt) * 64 + lane) * 4);
         all.x += more.x, all.y += more.y, all.z += more.z, all.w += more.w;
       }
-      *reinterpret_cast<float4*>(part_o + slot * D + dt * 16 + grp * 4) = all;
+      if constexpr (DIRECT) {
+        all.x *= scale_out, all.y *= scale_out, all.z *= scale_out, all.w *= scale_out;
+        const size_t place = slot * D + dt * 16 + grp * 4;
+        if constexpr (FLOAT) *reinterpret_cast<float4*>(static_cast<float*>(direct.out) + place) = all;
+        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(direct.out) + place) = make_uint2(pack_bf16(all.x, all.y), pack_bf16(all.z, all.w));
+      } else {
+        *reinterpret_cast<float4*>(part_o + slot * D + dt * 16 + grp * 4) = all;
+      }
     }
-    if (wave == 0 && grp == 0) part_ml[slot * 2] = most, part_ml[slot * 2 + 1] = total;
+    if (!DIRECT && wave == 0 && grp == 0) part_ml[slot * 2] = most, part_ml[slot * 2 + 1] = total;
   }
 }
 
@@ -599,20 +630,38 @@ prefix_items_kernel(const void* __restrict__ q, const void* __restrict__ cache, 
 #define TLIE_ARGS positions, part_first, part_o, part_ml, nq, nkv, page_shift, scale_log2, cap_pre
   if constexpr (FLOAT) {
     if (kFloatWide > 1 && columns > 16)
-      prefix_item<DT, true, kFloatWide>(item, kvh, q, cache, pages, TLIE_ARGS, reinterpret_cast<float*>(lds));
+      prefix_item<DT, true, kFloatWide, kPrefixWaves, false>(item, {}, kvh, q, cache, pages, TLIE_ARGS, reinterpret_cast<float*>(lds));
     else
-      prefix_item<DT, true, 1>(item, kvh, q, cache, pages, TLIE_ARGS, reinterpret_cast<float*>(lds));
+      prefix_item<DT, true, 1, kPrefixWaves, false>(item, {}, kvh, q, cache, pages, TLIE_ARGS, reinterpret_cast<float*>(lds));
   } else {
     const uint16_t* q16 = static_cast<const uint16_t*>(q);
     const uint16_t* cache16 = static_cast<const uint16_t*>(cache);
     if (columns <= 16)
-      prefix_item<DT, false, 1>(item, kvh, q, cache, pages, TLIE_ARGS, reinterpret_cast<float*>(lds));
+      prefix_item<DT, false, 1, kPrefixWaves, false>(item, {}, kvh, q, cache, pages, TLIE_ARGS, reinterpret_cast<float*>(lds));
     else if (DT > 8 || columns <= 64)
       prefix_wide_item<DT, 1>(item, kvh, q16, cache16, pages, TLIE_ARGS, lds);
     else
       prefix_wide_item<DT, (DT <= 8 ? 2 : 1)>(item, kvh, q16, cache16, pages, TLIE_ARGS, lds);
   }
 #undef TLIE_ARGS
+}
+
+// Short steps in one launch: a workgroup of eight waves (sixteen take longer: 10.2 us in place of 7.3 for 340 keys of 64 dims) for up to 16
+// columns of a sequence and all of their keys, the shared ones through another row of the table and read by every sequence for itself,
+// from the second on out of a cache.  What bounds it is latency, and then the 16 addresses a clock of a compute unit's loads: 5 us per 1000 keys.
+template <int DT, bool FLOAT>
+__global__ void __launch_bounds__(64 * kDirectWaves, 2)
+prefix_direct_kernel(const void* __restrict__ q, const void* __restrict__ cache, const int* __restrict__ block_table, int max_blocks,
+                     const int* __restrict__ items, const int* __restrict__ positions, const float* __restrict__ sink, void* __restrict__ out, int nq,
+                     int nkv, int page_shift, float scale_log2, float cap_pre) {
+  __shared__ __attribute__((aligned(16))) float lds[kDirectWaves * (32 + DT * 256)];
+  const int kvh = blockIdx.x % nkv;
+  const int* words = items + static_cast<size_t>(blockIdx.x / nkv) * 8;
+  auto word = [&](int i) { return __builtin_amdgcn_readfirstlane(words[i]); };
+  const PrefixItem item{word(0), word(1), word(2), word(3), word(4), word(5), 1, 0};
+  const Direct direct{block_table + static_cast<size_t>(word(7)) * max_blocks, item.key_lo, sink, out};
+  prefix_item<DT, FLOAT, 1, kDirectWaves, true>(item, direct, kvh, q, cache, block_table + static_cast<size_t>(item.table) * max_blocks, positions, nullptr,
+                                                nullptr, nullptr, nq, nkv, page_shift, scale_log2, cap_pre, lds);
 }
 
 // out[t][h] = sum_i w_i o_i / (sum_i w_i l_i + w_sink) over the token's parts.  A wave a (token, head): the lanes have a part's weight
@@ -680,6 +729,14 @@ static int launch_items(const void* q, const void* cache, const int* block_table
   return launch_status();
 }
 
+template <bool FLOAT, int DT>
+static int launch_direct(const void* q, const void* cache, const int* block_table, int max_blocks, const int* items, int num_items, const int* positions,
+                         const float* sink, void* out, int nq, int nkv, int page_shift, float scale_log2, float cap_pre, hipStream_t stream) {
+  hipLaunchKernelGGL((prefix_direct_kernel<DT, FLOAT>), dim3(num_items * nkv), dim3(64 * kDirectWaves), 0, stream, q, cache, block_table, max_blocks, items,
+                     positions, sink, out, nq, nkv, page_shift, scale_log2, cap_pre);
+  return launch_status();
+}
+
 // ---- the host's half: which items a step has ----
 
 // Columns of the tile that has so many of its item before it, itself included (prefix_items_kernel takes them so).
@@ -728,7 +785,7 @@ using namespace tlie;
 // q, out: [tokens, nq, d]; cache: [pages, 2, nkv, page_size * d] (keys [row][dim], values [dim][row]); both of `dtype`.
 // items: int32 [num_items, 8] (see PrefixItem; tiles of columns as prefix_items_kernel has them); part_first: int32 [tokens + 1], the first part of
 // each token, so that part_first[tokens] is their number; part_o: float [parts, nq, d], part_ml: float [parts, nq, 2].
-// sink: float [nq] or null.  softcap: 0, or the cap of the scaled scores.
+// sink: float [nq] or null.  softcap: 0, or the cap of the scaled scores.  part_o null: the items are those of tlie_prefix_direct.
 extern "C" int tlie_attention_prefix(const void* q, const void* cache, int dtype, const int* block_table, int max_blocks, const int* items,
                                      int num_items, const int* positions, const int* part_first, float* part_o, float* part_ml,
                                      const float* sink, void* out, int tokens, int nq, int nkv, int d, int page_size, float scale,
@@ -739,11 +796,27 @@ extern "C" int tlie_attention_prefix(const void* q, const void* cache, int dtype
       static_cast<long long>(num_items) * nkv >= 1ll << 24 || static_cast<long long>(tokens) * nq >= 1ll << 26 ||
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(part_o)) & 15) != 0)
     return kBadArgument;
+  const bool is_direct = part_o == nullptr;
   const float scale_log2 = (softcap > 0.f ? softcap : scale) * 1.4426950408889634f, cap_pre = softcap > 0.f ? scale / softcap : 0.f;
   if (!(scale_log2 < INFINITY) || !(cap_pre < INFINITY) || (softcap > 0.f && !(cap_pre > 0.f))) return kBadArgument;
   const int page_shift = 31 - __builtin_clz(page_size);
   hipStream_t s = (hipStream_t)stream;
   int status = kBadArgument;
+  if (is_direct) {
+#define TLIE_CASE(DT)                                                                                                                              \
+  case DT:                                                                                                                                         \
+    return launch_direct<false, DT>(q, cache, block_table, max_blocks, items, num_items, positions, sink, out, nq, nkv, page_shift, scale_log2,    \
+                                    cap_pre, s);
+#define TLIE_FLOAT(DT)                                                                                                                             \
+  case DT:                                                                                                                                         \
+    return launch_direct<true, DT>(q, cache, block_table, max_blocks, items, num_items, positions, sink, out, nq, nkv, page_shift, scale_log2,     \
+                                   cap_pre, s);
+    if (dtype == kF32) switch (d / 16) { TLIE_FLOAT(1) TLIE_FLOAT(2) TLIE_FLOAT(3) TLIE_FLOAT(4) }
+    else switch (d / 16) { TLIE_CASE(1) TLIE_CASE(2) TLIE_CASE(3) TLIE_CASE(4) TLIE_CASE(5) TLIE_CASE(6) }
+#undef TLIE_FLOAT
+#undef TLIE_CASE
+    return kBadArgument;
+  }
 #define TLIE_CASE(DT)                                                                                                                              \
   case DT:                                                                                                                                         \
     status = dtype == kF32 ? launch_items<true, DT>(q, cache, block_table, max_blocks, items, num_items, positions, part_first, part_o,      \
@@ -863,4 +936,38 @@ extern "C" int tlie_prefix_plan(const long long* seq_start, const long long* seq
   });
   part_first[tokens] = static_cast<int>(std::min(parts, 0x7fffffffll));
   return parts * nq > 0x7fffffffll ? -5 : static_cast<int>(total);
+}
+
+// The items of a short step that one launch takes (part_o null in tlie_attention_prefix), for a step that tlie_prefix_plan has a plan for: [.][8]
+// (sequence, first token, tokens, first column, shared keys, end of the keys, 1, the row that the shared keys are read through).  Returns
+// their number; 0: such a step takes longer this way.
+extern "C" int tlie_prefix_direct(const long long* seq_start, const long long* seq_len, int sequences, const long long* groups, int num_groups, int nq,
+                                  int nkv, int d, int dtype, int compute_units, int* items, int max_items) {
+  const long long G = nq / nkv;
+  // bytes of a plane of keys, and head sizes, up to which one launch is no slower in a recording either (16 sequences, 32 heads of 64 on 4, 440
+  // keys 7.4 us, in parts 10.4; 12 heads of 32 on 4, 940 keys 6.6 and 8.2; 16 heads of 96, 540 keys 9.3 and 10.4; of 128 on 8, 160 keys
+  // 10.1 and 9.9, 300 11.9 and 9.7); from eager calls 9.8 us and 14.1.  More workgroups than units run one after the other (48
+  // sequences, 24 heads of 80 on 8: 13.9 and 11.9).
+  constexpr long long kMostBytes = 98304;
+  if (d > (dtype == kF32 ? 64 : 96)) return 0;
+  long long count = 0;
+  int g = 0;
+  for (int s = 0; s < sequences; ++s) {
+    const long long tokens = seq_start[s + 1] - seq_start[s];
+    while (g < num_groups && groups[3 * g] + groups[3 * g + 1] <= s) ++g;
+    if (tokens == 0) continue;
+    const bool grouped = g < num_groups && groups[3 * g] <= s;
+    long long reader = s;
+    if (grouped) {
+      reader = groups[3 * g];
+      while (seq_start[reader + 1] == seq_start[reader]) ++reader;
+    }
+    for (long long col0 = 0; col0 < tokens * G; col0 += 16, ++count) {
+      const long long end = seq_len[s] - tokens + std::min(tokens - 1, (col0 + 15) / G) + 1;
+      if (end * d * (dtype == kF32 ? 4 : 2) > kMostBytes || count >= max_items) return 0;
+      const long long values[8] = {s, seq_start[s], tokens, col0, grouped ? groups[3 * g + 2] : 0, end, 1, reader};
+      for (int i = 0; i < 8; ++i) items[count * 8 + i] = static_cast<int>(values[i]);
+    }
+  }
+  return count * nkv <= compute_units ? static_cast<int>(count) : 0;
 }

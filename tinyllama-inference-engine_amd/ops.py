@@ -2763,6 +2763,8 @@ class SharedPrefixPlan:
     sequences: int
     longest: int
     sizes: tuple                   # (num_heads, num_kv_heads, head_dim, dtype)
+    # a short step in one launch: its tokens (else 0); items are then (sequence, first token, tokens, first column, shared keys, end, 1, their row)
+    direct: int = 0
 
 
 def prefix_tile_columns(columns: int, head_dim: int, dtype: torch.dtype) -> int:
@@ -2814,6 +2816,18 @@ def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads
         items = np.empty((count, 8), dtype=np.int32)
 
 
+def direct_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, compute_units: int):
+    """The items of a step that one launch takes, an int32 array [n, 8] of numpy; None: a step that is better cut (csrc/attention_prefix.hip has
+    the rule).  For arguments that `shared_prefix_items` takes."""
+    import numpy as np
+    seq_start, seq_len = np.ascontiguousarray(seq_start, dtype=np.int64), np.ascontiguousarray(seq_len, dtype=np.int64)
+    groups = np.array(sorted(groups), dtype=np.int64).reshape(-1, 3)
+    items = np.empty((compute_units, 8), dtype=np.int32)
+    count = _entry("tlie_prefix_direct", "ppipiiiiiipi")(seq_start.ctypes.data, seq_len.ctypes.data, seq_len.shape[0], groups.ctypes.data, groups.shape[0], num_heads,
+                                                        num_kv_heads, head_dim, dtype_code(dtype), compute_units, items.ctypes.data, items.shape[0])
+    return items[:count].copy() if count > 0 else None
+
+
 def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device) -> SharedPrefixPlan:
     """What `attention_shared_prefix` does in a step, for all of its layers.
 
@@ -2822,12 +2836,17 @@ def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads:
     positions 0 .. prefix - 1; all their tokens stand behind it.  Sequences in no group share nothing."""
     import numpy as np
     device = torch.device(device)
-    items, part_first = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype,
-                                            _compute_units(device) if device.type == "cuda" else 256)
+    units = _compute_units(device) if device.type == "cuda" else 256
+    items, part_first = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype, units)
     longest = max((int(length) for length in seq_len), default=0)
+    sizes = (num_heads, num_kv_heads, head_dim, dtype)
+    direct = direct_prefix_items(seq_start, seq_len, groups, *sizes, units)
+    if direct is not None:
+        items, tokens = torch.from_numpy(direct).to(device), part_first.shape[0] - 1
+        return SharedPrefixPlan(items, items[:0], tokens, 0, len(seq_len), longest, sizes, tokens)
     count, parts, tokens = items.shape[0], int(part_first[-1]), part_first.shape[0] - 1
     both = torch.from_numpy(np.concatenate([items.ravel(), part_first])).to(device)             # (one transfer)
-    return SharedPrefixPlan(both[:count * 8].view(count, 8), both[count * 8:], tokens, parts, len(seq_len), longest, (num_heads, num_kv_heads, head_dim, dtype))
+    return SharedPrefixPlan(both[:count * 8].view(count, 8), both[count * 8:], tokens, parts, len(seq_len), longest, sizes)
 
 
 def shared_prefix_pays(groups, num_kv_heads: int, head_dim: int) -> bool:
@@ -2922,11 +2941,17 @@ def attention_shared_prefix(q: torch.Tensor, cache: torch.Tensor, block_table: t
         raise invalid_argument("attention_shared_prefix takes head sizes in steps of 16 up to 256, pages of a power of two of rows (16 to 65536)")
     if block_table.dim() != 2 or block_table.shape[0] < plan.sequences or block_table.shape[1] * page_size < plan.longest:
         raise invalid_shape(f"attention_shared_prefix: block_table {list(block_table.shape)} does not hold {plan.sequences} sequences of up to {plan.longest} positions")
-    out = torch.empty_like(q)
+    out = torch.empty_like(q) if not plan.direct or plan.direct == tokens else torch.zeros_like(q)      # (rows that its items do not write)
     if tokens == 0:
         return out
     if plan.items.shape[0] == 0:
         return out.zero_()
+    if plan.direct:
+        _check(_entry("tlie_attention_prefix", "ppipipippppppiiiiiffp")(
+            q.data_ptr(), cache.data_ptr(), dtype_code(dtype), block_table.data_ptr(), block_table.shape[1], plan.items.data_ptr(), plan.items.shape[0],
+            positions.data_ptr(), None, None, None, _address(sink), out.data_ptr(), tokens, num_heads, num_kv_heads, head_dim, page_size, scale,
+            softcap or 0.0, torch._C._cuda_getCurrentRawStream(current)), "attention_shared_prefix")
+        return out
     # the parts' results: their values (a part and head's at a multiple of 64 bytes), then their maxima and sums
     rows = plan.parts * num_heads
     parts = q.new_empty(rows * (head_dim + 2), dtype=torch.float32)
