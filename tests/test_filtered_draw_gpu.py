@@ -277,3 +277,15 @@ def test_the_first_of_equal_maxima_wherever_they_stand(rows, vocab):
         assert got.tolist() == [place] * rows, place
         got = ops.sample_filtered(logits.to(DEV), zero, torch.full((rows,), 0.1, device=DEV), top_k=torch.ones(rows, dtype=torch.int32, device=DEV))
         assert got.tolist() == [place] * rows, place
+
+
+def test_the_largest_vocabulary():
+    """Tokens at both ends of 2^24 - 1, with weights of 2^-38 of the largest at the least."""
+    vocab = ops.DRAW_MAX_VOCAB
+    logits = torch.full((3, vocab), -60.0)
+    logits[:, 5], logits[:, vocab - 1], logits[:, vocab // 2] = 2.0, 1.0, 0.0
+    logits[2, vocab - 2] = 3.0
+    uniform = torch.tensor([0.1, 0.7, 0.99])
+    check(logits, uniform, temperature=torch.ones(3), top_k=torch.tensor([0, 2, 3], dtype=torch.int32), min_p=torch.full((3,), 0.01))
+    with pytest.raises(EngineError):
+        ops.sample_filtered(torch.zeros((1, vocab + 1), device=DEV), torch.zeros(1, device=DEV))

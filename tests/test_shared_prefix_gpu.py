@@ -296,3 +296,16 @@ def test_a_longer_table_of_small_pages_than_a_window_holds():
     check(make_step(16, BF16, 4, 1, 64, 16, [(4500, 1), (4490, 1)], [(0, 2, 4400)]))
     check(make_step(17, BF16, 24, 1, 64, 16, [(4500, 1), (4490, 1)], [(0, 2, 4400)]))
     check(make_step(18, F32, 4, 1, 32, 16, [(4500, 1)], []))
+
+
+@pytest.mark.parametrize("heads,sequences,groups", [(16, [(300, 1), (310, 1), (290, 1)], [(0, 3, 280)]), (64, [(300, 1), (310, 9), (290, 1)], [(0, 3, 280)])])
+def test_pages_past_32_bits(heads, sequences, groups):
+    """The step's pages at the end of a cache of more than 2^32 bytes and 2^31 elements: the results of the same pages at its beginning."""
+    step = make_step(19, BF16, heads, 8, 64, 32, sequences, groups)
+    want = call(step)
+    pages, last = step["cache"].shape[0], (1 << 32) // step["cache"][0].numel() + 7
+    cache = torch.empty((last + pages, *step["cache"].shape[1:]), dtype=BF16, device=DEV)
+    assert cache.numel() > 1 << 32
+    cache[last:] = step["cache"].to(DEV)
+    step["cache"], step["table"] = cache, step["table"] + last
+    assert torch.equal(call(step), want)
