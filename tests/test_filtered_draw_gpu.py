@@ -289,3 +289,11 @@ def test_the_largest_vocabulary():
     check(logits, uniform, temperature=torch.ones(3), top_k=torch.tensor([0, 2, 3], dtype=torch.int32), min_p=torch.full((3,), 0.01))
     with pytest.raises(EngineError):
         ops.sample_filtered(torch.zeros((1, vocab + 1), device=DEV), torch.zeros(1, device=DEV))
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 20000), (1, 28000), (3, 20480), (35, 24576)])
+def test_odd_numbers_of_rows_times_parts(rows, vocab):
+    assert rows * ops.draw_parts(rows, vocab) % 2 == 1
+    logits, uniform, gen = rows_of(vocab + rows, rows, vocab)
+    check(logits, uniform, **filters_of(gen, rows))
+    check(logits, uniform, temperature=torch.full((rows,), 0.8), top_p=torch.full((rows,), 0.9))

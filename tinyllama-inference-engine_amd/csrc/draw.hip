@@ -938,9 +938,34 @@ draw_row_kernel(const float* __restrict__ logits, int vocab, const float* __rest
 
 using namespace tlie;
 
-// The entry's scratch, for `parts` parts a row: the rows' lists and states, the parts' statistics, sums, masses and counts of classes.
+// The entry's scratch, for `parts` parts a row: the rows' lists and states, the parts' statistics, masses and counts of classes, and sums.
 constexpr long long kRowBytes = sizeof(RowState) + kListMost * sizeof(Listed), kPartBytes = sizeof(PartStat) + 8 + kClasses * 12;
 static_assert(sizeof(RowState) == 32 && sizeof(Listed) == 40 && sizeof(PartStat) == 16, "the host's face counts them so");
+
+// Where each begins, in bytes.  Classes are read 16 bytes at a time, so what stands before them has a multiple of 16 whatever the number of rows
+// and parts (a row's list 80 KB); the sums, of 8 bytes each, stand last.
+struct Scratch {
+  long long lists, states, stats, class_mass, class_count, sums, end;
+};
+static Scratch scratch_of(long long rows, long long parts) {
+  static_assert(kListMost * sizeof(Listed) % 16 == 0 && sizeof(RowState) % 16 == 0 && sizeof(PartStat) % 16 == 0 && kClasses % 4 == 0, "read in pieces of 16 bytes");
+  const long long places = rows * parts;
+  Scratch s{};
+  s.states = s.lists + rows * kListMost * static_cast<long long>(sizeof(Listed));
+  s.stats = s.states + rows * static_cast<long long>(sizeof(RowState));
+  s.class_mass = s.stats + places * static_cast<long long>(sizeof(PartStat));
+  s.class_count = s.class_mass + places * kClasses * 8;
+  s.sums = s.class_count + places * kClasses * 4;
+  s.end = s.sums + places * 8;
+  return s;
+}
+
+// The starts of a scratch's seven pieces (the last: its end), for rows in `parts` parts each.
+extern "C" void tlie_draw_scratch(int rows, int parts, long long* starts) {
+  const Scratch s = scratch_of(rows, parts);
+  const long long values[7] = {s.lists, s.states, s.stats, s.class_mass, s.class_count, s.sums, s.end};
+  for (int i = 0; i < 7; ++i) starts[i] = values[i];
+}
 
 // logits: float [rows, vocab], vocab < 2^24; uniform: float [rows]; temperature, top_k, top_p, min_p: [rows] or null; parts: 1 to 8, or 0: a row by
 // one workgroup (scratch is then null);
@@ -948,7 +973,7 @@ static_assert(sizeof(RowState) == 32 && sizeof(Listed) == 40 && sizeof(PartStat)
 extern "C" int tlie_draw(const float* logits, int rows, int vocab, const float* uniform, const float* temperature, const int* top_k,
                          const float* top_p, const float* min_p, int parts, void* scratch, int* out, float* logprob, void* stream) {
   if (rows <= 0 || vocab <= 0 || vocab >= (1 << 24) || parts < 0 || parts > kPartsMost || rows > 65535 ||
-      uniform == nullptr || (parts > 0 && scratch == nullptr))
+      uniform == nullptr || (parts > 0 && (scratch == nullptr || reinterpret_cast<uintptr_t>(scratch) % 16 != 0)))
     return kBadArgument;
   hipStream_t s = (hipStream_t)stream;
   int shift = 44;                                   // the weights' sum stays below 2^62
@@ -959,13 +984,14 @@ extern "C" int tlie_draw(const float* logits, int rows, int vocab, const float* 
     return launch_status();
   }
   const int part_len = (vocab + parts - 1) / parts;
-  const size_t places = static_cast<size_t>(rows) * parts;
-  Listed* lists = static_cast<Listed*>(scratch);
-  RowState* states = reinterpret_cast<RowState*>(lists + static_cast<size_t>(rows) * kListMost);
-  PartStat* stats = reinterpret_cast<PartStat*>(states + rows);
-  double* sums = reinterpret_cast<double*>(stats + places);
-  uint64_t* class_mass = reinterpret_cast<uint64_t*>(sums + places);
-  uint32_t* class_count = reinterpret_cast<uint32_t*>(class_mass + places * kClasses);
+  const Scratch at = scratch_of(rows, parts);
+  unsigned char* base = static_cast<unsigned char*>(scratch);
+  Listed* lists = reinterpret_cast<Listed*>(base + at.lists);
+  RowState* states = reinterpret_cast<RowState*>(base + at.states);
+  PartStat* stats = reinterpret_cast<PartStat*>(base + at.stats);
+  uint64_t* class_mass = reinterpret_cast<uint64_t*>(base + at.class_mass);
+  uint32_t* class_count = reinterpret_cast<uint32_t*>(base + at.class_count);
+  double* sums = reinterpret_cast<double*>(base + at.sums);
   const dim3 grid((rows + kDies - 1) / kDies * kDies * parts);
   hipLaunchKernelGGL(draw_best_kernel, grid, dim3(kPartThreads), 0, s, logits, rows, vocab, part_len, parts, stats);
   hipLaunchKernelGGL(draw_weigh_kernel, grid, dim3(kPartThreads), 0, s, logits, rows, vocab, part_len, parts, stats, temperature, shift,
