@@ -145,3 +145,24 @@ def test_long_steps_and_wide_heads_are_cut():
     assert plan(700, 64) is not None and plan(1000, 64) is None
     assert plan(300, 64, torch.float32) is not None and plan(700, 64, torch.float32) is None
     assert plan(100, 128) is None and plan(100, 64, count=65) is None
+
+
+@pytest.mark.parametrize("start,lengths,fits", [
+    ([0, 1, 2], [64, 64], True), ([0, 1, 2, 3, 4], [10, 20, 64, 3], True),
+    ([0, 1, 2], [64, 65], False),                     # longer than the tables that the plan goes with
+    ([0, 1, 1], [3, 1000], False),                    # the same, of a sequence that brings nothing
+    ([0, 1, 1, 1, 1, 2], [9, 9, 9, 9, 9], False),     # more sequences than such tables have rows
+    ([0, 1, 2, 3, 4, 5], [9] * 5, False),             # more tokens
+])
+def test_steps_beyond_a_recorded_plan_are_refused(start, lengths, fits):
+    """A recorded step's block table is checked against what its plan may hold, once; so `fill` keeps every step within that."""
+    plan = ops.RecordedPrefixPlan(4, 64, 8, 4, 64, torch.bfloat16, "cpu")
+    if fits:
+        plan.fill(start, lengths, [])
+        items, _ = ops.shared_prefix_items(start, lengths, [], 8, 4, 64, torch.bfloat16)
+        assert plan.plan.items[:len(items)].tolist() == items.tolist() and not plan.plan.items[len(items):].any()
+    else:
+        before = plan.plan.items.clone()
+        with pytest.raises(EngineError):
+            plan.fill(start, lengths, [])
+        assert torch.equal(plan.plan.items, before)

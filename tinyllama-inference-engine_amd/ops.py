@@ -2857,8 +2857,8 @@ def shared_prefix_pays(groups, num_kv_heads: int, head_dim: int) -> bool:
 
 
 class RecordedPrefixPlan:
-    """A `SharedPrefixPlan` at fixed addresses and of fixed size, for a recorded step of up to `tokens` single tokens: `fill` writes a
-    step's work into it.  Items and parts beyond the step's have no tokens."""
+    """A `SharedPrefixPlan` at fixed addresses and of fixed size, for a recorded step of up to `tokens` single tokens in as many sequences of up
+    to `longest` positions: `fill` writes a step's work into it.  Items and parts beyond the step's have no tokens."""
 
     @staticmethod
     def room(tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype) -> tuple[int, int]:
@@ -2869,18 +2869,22 @@ class RecordedPrefixPlan:
 
     def __init__(self, tokens: int, longest: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device):
         self.items, self.parts = self.room(tokens, num_heads, num_kv_heads, head_dim, dtype)
-        self._host = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, pin_memory=True)
         self._device = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, device=device)
-        self._units = _compute_units(self._device.device)
+        self._host = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, pin_memory=self._device.is_cuda)
+        self._units = _compute_units(self._device.device) if self._device.is_cuda else 256
         self.plan = SharedPrefixPlan(self._device[:self.items * 8].view(self.items, 8), self._device[self.items * 8:], tokens, self.parts, tokens,
                                      longest, (num_heads, num_kv_heads, head_dim, dtype))
 
     def fill(self, seq_start, seq_len, groups) -> None:
+        import numpy as np
         num_heads, num_kv_heads, head_dim, dtype = self.plan.sizes
         host, begin, most = self._host.numpy(), self.items * 8, PREFIX_PARTS
         tokens = int(seq_start[-1])
-        if tokens > self.plan.tokens:
-            raise invalid_shape(f"a recorded plan for {self.plan.tokens} tokens does not hold {tokens}")
+        if tokens > self.plan.tokens or len(seq_len) > self.plan.sequences:
+            raise invalid_shape(f"a recorded plan for {self.plan.tokens} tokens does not hold {tokens} in {len(seq_len)} sequences")
+        longest = int(np.max(seq_len, initial=0))
+        if longest > self.plan.longest:
+            raise invalid_shape(f"a recorded plan for {self.plan.longest} positions does not hold a sequence of {longest}")
         items, part_first = host[:begin].reshape(self.items, 8), host[begin:]
         while True:
             made = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype, self._units, most, items, part_first)
