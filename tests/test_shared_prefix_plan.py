@@ -166,3 +166,21 @@ def test_steps_beyond_a_recorded_plan_are_refused(start, lengths, fits):
         with pytest.raises(EngineError):
             plan.fill(start, lengths, [])
         assert torch.equal(plan.plan.items, before)
+
+
+def test_a_recorded_plans_buffer_is_written_behind_its_last_transfer():
+    """`fill` again, with no step in between: the host's buffer is still being read until the event behind its transfer has been reached."""
+    log = []
+
+    class Event:
+        def synchronize(self):
+            log.append(("wait", plan._host.clone()))
+
+        def record(self):
+            log.append(("record", plan._host.clone()))
+    plan = ops.RecordedPrefixPlan(4, 64, 8, 4, 64, torch.bfloat16, "cpu")
+    plan._sent = Event()
+    plan.fill([0, 1, 2], [40, 41], [(0, 2, 39)])
+    plan.fill([0, 1], [17], [])
+    assert [name for name, _ in log] == ["wait", "record", "wait", "record"]
+    assert torch.equal(log[1][1], log[2][1]) and not torch.equal(log[2][1], log[3][1])

@@ -2858,7 +2858,7 @@ def shared_prefix_pays(groups, num_kv_heads: int, head_dim: int) -> bool:
 
 class RecordedPrefixPlan:
     """A `SharedPrefixPlan` at fixed addresses and of fixed size, for a recorded step of up to `tokens` single tokens in as many sequences of up
-    to `longest` positions: `fill` writes a step's work into it.  Items and parts beyond the step's have no tokens."""
+    to `longest` positions: `fill` writes a step's work into it, on the current stream.  Items and parts beyond the step's have no tokens."""
 
     @staticmethod
     def room(tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype) -> tuple[int, int]:
@@ -2872,6 +2872,7 @@ class RecordedPrefixPlan:
         self._device = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, device=device)
         self._host = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, pin_memory=self._device.is_cuda)
         self._units = _compute_units(self._device.device) if self._device.is_cuda else 256
+        self._sent = torch.cuda.Event() if self._device.is_cuda else None         # the last transfer has read the host's buffer
         self.plan = SharedPrefixPlan(self._device[:self.items * 8].view(self.items, 8), self._device[self.items * 8:], tokens, self.parts, tokens,
                                      longest, (num_heads, num_kv_heads, head_dim, dtype))
 
@@ -2886,6 +2887,8 @@ class RecordedPrefixPlan:
         if longest > self.plan.longest:
             raise invalid_shape(f"a recorded plan for {self.plan.longest} positions does not hold a sequence of {longest}")
         items, part_first = host[:begin].reshape(self.items, 8), host[begin:]
+        if self._sent is not None:
+            self._sent.synchronize()
         while True:
             made = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype, self._units, most, items, part_first)
             if made is not None and int(part_first[tokens]) <= self.parts:
@@ -2896,6 +2899,8 @@ class RecordedPrefixPlan:
         items[made[0].shape[0]:] = 0
         part_first[tokens + 1:] = part_first[tokens]
         self._device.copy_(self._host, non_blocking=True)
+        if self._sent is not None:
+            self._sent.record()
 
 
 def step_prefix_plan(ctx, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype) -> SharedPrefixPlan:
