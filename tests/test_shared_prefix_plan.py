@@ -184,3 +184,9 @@ def test_a_recorded_plans_buffer_is_written_behind_its_last_transfer():
     plan.fill([0, 1], [17], [])
     assert [name for name, _ in log] == ["wait", "record", "wait", "record"]
     assert torch.equal(log[1][1], log[2][1]) and not torch.equal(log[2][1], log[3][1])
+
+
+@pytest.mark.parametrize("start,lengths", [([0, 1 << 40], [1 << 40]), ([0, 1 << 62], [1 << 62]), ([0, 1 << 26], [1 << 27])])
+def test_more_tokens_than_a_launch_takes_are_refused_and_not_allocated(start, lengths):
+    with pytest.raises(EngineError):
+        ops.shared_prefix_plan(start, lengths, [], 8, 4, 64, torch.bfloat16, "cpu")

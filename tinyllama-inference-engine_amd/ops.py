@@ -2801,7 +2801,7 @@ def shared_prefix_items(seq_start, seq_len, groups, num_heads: int, num_kv_heads
     if not given:
         items = np.empty((256, 8), dtype=np.int32)
     if part_first is None:
-        part_first = np.empty(max(0, int(seq_start[-1])) + 1, dtype=np.int32)
+        part_first = np.empty(min(max(0, int(seq_start[-1])), 1 << 26) + 1, dtype=np.int32)      # (more tokens are refused before any is written)
     while True:
         count = _entry("tlie_prefix_plan", "ppipiiiiiiipip")(seq_start.ctypes.data, seq_len.ctypes.data, seq_len.shape[0], groups.ctypes.data, groups.shape[0], num_heads,
                                                             num_kv_heads, head_dim, dtype_code(dtype), compute_units, most_parts, items.ctypes.data,
