@@ -297,3 +297,17 @@ def test_odd_numbers_of_rows_times_parts(rows, vocab):
     logits, uniform, gen = rows_of(vocab + rows, rows, vocab)
     check(logits, uniform, **filters_of(gen, rows))
     check(logits, uniform, temperature=torch.full((rows,), 0.8), top_p=torch.full((rows,), 0.9))
+
+
+@pytest.mark.parametrize("rows,vocab", [(6, 3000), (2, 60000), (6, 20000)])
+def test_min_p_above_one_keeps_the_first_token_alone(rows, vocab):
+    """No weight reaches more than the largest's, so of several largest the first is kept; at 1 they all are.  Also where more tokens
+    are equal than are sorted."""
+    logits, _, gen = rows_of(vocab, rows, vocab)
+    logits[:, [40, 700, vocab - 1]] = 30.0
+    logits[1] = 2.0
+    ones = torch.ones(rows)
+    for min_p in (1.0, 1.0 + 2.0 ** -23, 1.5, 1e30, math.inf):
+        for u in (0.0, 0.4, 0.99):
+            got = check(logits, u * ones, temperature=0.8 * ones, min_p=min_p * ones)
+            assert min_p == 1.0 or got.tolist() == [40, 0] + [40] * (rows - 2)

@@ -662,7 +662,7 @@ __device__ uint64_t cross(CrossShared<THREADS>& s, const PoweredScale<ALL>& scal
     kept = s.answers[1];
   }
   if (ask.floor > 0.f) {
-    const double least_weight = static_cast<double>(fminf(ask.floor, 1.f)) * scale.one;
+    const double least_weight = static_cast<double>(ask.floor) * scale.one;
 #pragma unroll
     for (int j = 0; j < kEach; ++j)
       if (units[j] != 0 && weight_wide(scale, place_value(key[j])) >= least_weight)
@@ -725,7 +725,7 @@ __device__ uint64_t cross_without_list(CrossShared<THREADS>& s, const float* __r
   for (int step = 0; step < 3; ++step) {                          // top_k, top_p, the draw: a loop, so that the code is there once
     if ((step == 0 && !state.cut_k) || (step == 1 && !(ask.p < 1.f))) continue;
     if (step == 2 && ask.floor > 0.f) {
-      const double least_weight = static_cast<double>(fminf(ask.floor, 1.f)) * scale.one;
+      const double least_weight = static_cast<double>(ask.floor) * scale.one;
       if (threadIdx.x == 0) s.answers[3] = 0;
       __syncthreads();
       scan_tokens<THREADS, 4>(row, 0, vocab, [&](int first, const float4& four) {
