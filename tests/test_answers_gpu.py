@@ -186,3 +186,19 @@ def test_the_command_line(tmp_path, capsys):
     for wrong in (["--answers", "0"], ["--top-k", "-2"], ["--min-p", "1.5"]):
         assert main(["generate", folder, text, "6", "--dtype", "float32", "--temperature", "0.9", *wrong]) != 0
         capsys.readouterr()
+
+
+@pytest.mark.parametrize("filters", [dict(top_k=20), dict(min_p=0.05), dict(logprobs=True), dict(top_k=20, logprobs=True), dict()])
+def test_logits_that_are_not_finite_are_errors_whatever_the_draw(filters):
+    """An infinity of either sign or a NaN: `numerical_error`, for rows with filters as for rows without."""
+    from tlie_amd.errors import EngineError
+    from tlie_amd.sampling.sampler import Sampler
+    sampler = Sampler(DEV, capacity=4)
+    params = [SamplingParams(temperature=0.8, seed=index, **filters) for index in range(3)]
+    logits = torch.randn((3, 700), generator=torch.Generator().manual_seed(2)).to(DEV)
+    assert len(sampler.sample(logits, params, [0, 0, 0])) == 3
+    for value in (-math.inf, math.inf, math.nan):
+        bad = logits.clone()
+        bad[1, 33] = value
+        with pytest.raises(EngineError):
+            sampler.sample(bad, params, [0, 0, 0])

@@ -311,3 +311,22 @@ def test_min_p_above_one_keeps_the_first_token_alone(rows, vocab):
         for u in (0.0, 0.4, 0.99):
             got = check(logits, u * ones, temperature=0.8 * ones, min_p=min_p * ones)
             assert min_p == 1.0 or got.tolist() == [40, 0] + [40] * (rows - 2)
+
+
+@pytest.mark.parametrize("rows,vocab", [(7, 1001), (7, 4098), (2, 60003)])
+def test_rows_that_have_to_be_finite(rows, vocab):
+    """With finite=True one logit of -inf, at any place of the row, gives -1; the other rows draw what they draw without."""
+    logits, uniform, _ = rows_of(vocab, rows, vocab)
+    on = lambda value: value.to(DEV)
+    draw = lambda values, **named: ops.sample_filtered(on(values), on(uniform), torch.ones(rows, device=DEV), torch.full((rows,), 9, dtype=torch.int32, device=DEV),
+                                                       logprobs=True, **named)
+    want, want_logprobs = draw(logits)
+    got, logprobs = draw(logits, finite=True)
+    assert torch.equal(got, want) and torch.equal(logprobs, want_logprobs)
+    for place in (0, 1, 2, 3, 4, 500, vocab // 2, vocab - 4, vocab - 3, vocab - 2, vocab - 1):
+        masked = logits.clone()
+        masked[1, place] = -math.inf
+        assert draw(masked)[0][1] >= 0
+        got, logprobs = draw(masked, finite=True)
+        assert got[1] == -1 and math.isnan(logprobs[1]), place
+        assert torch.equal(got[[0] + list(range(2, rows))], want[[0] + list(range(2, rows))])

@@ -24,5 +24,5 @@ def test_pieces_begin_at_multiples_of_16_bytes(rows, vocab):
 
 
 def test_a_scratch_that_does_not_begin_so_is_refused():
-    draw = ops._entry("tlie_draw", "piipppppipppp")
-    assert draw(4096, 1, 32000, 4096, 4096, None, None, None, 8, 4096 + 8, 4096, None, None) == -1      # (refused before any launch: no GPU is needed)
+    draw = ops._entry("tlie_draw", "piipppppiipppp")
+    assert draw(4096, 1, 32000, 4096, 4096, None, None, None, 0, 8, 4096 + 8, 4096, None, None) == -1      # (refused before any launch: no GPU is needed)

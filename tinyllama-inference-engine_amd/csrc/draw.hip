@@ -196,9 +196,11 @@ constexpr int kDies = 8;
 __device__ __forceinline__ int row_of(int parts) { return static_cast<int>(blockIdx.x / kDies) / parts * kDies + static_cast<int>(blockIdx.x % kDies); }
 __device__ __forceinline__ int part_of(int parts) { return static_cast<int>(blockIdx.x / kDies) % parts; }
 
-// What a thread has seen of a row: its first largest token's group, the smallest finite logit, and whether one is a NaN or +inf.  A group of
-// four is compared as one and kept whole, so that which of its tokens it is is asked once, at the end.
+// What a thread has seen of the tokens begin .. end - 1: its first largest token's group, the smallest finite logit, and whether one is a NaN or
+// +inf (with `finite`, or -inf).  A group of four is compared as one and kept whole, so that which of its tokens it is is asked once, at the end.
 struct Seen {
+  const int begin, end;
+  const bool finite;
   float most = -INFINITY, least = INFINITY;
   float4 group = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
   int first = 0;
@@ -210,6 +212,8 @@ struct Seen {
     if (low == -INFINITY) {                                       // (a token that cannot be drawn, or none: of the others)
       const float none = INFINITY;
       low = fminf(fminf(v.x > -INFINITY ? v.x : none, v.y > -INFINITY ? v.y : none), fminf(v.z > -INFINITY ? v.z : none, v.w > -INFINITY ? v.w : none));
+      auto cannot = [&](int i, float x) { return x == -INFINITY && i >= begin && i < end; };
+      bad = bad || (finite && (cannot(index, v.x) || cannot(index + 1, v.y) || cannot(index + 2, v.z) || cannot(index + 3, v.w)));
     }
     least = fminf(least, low);
     const bool more = here > most || (here == most && index < first);      // (a thread may meet the range's last, cut group before others)
@@ -220,7 +224,7 @@ struct Seen {
 };
 
 struct PartStat {
-  uint64_t best;        // place_key of the part's first token in the order; 0: the part has none; all ones: a NaN or +inf
+  uint64_t best;        // place_key of the part's first token in the order; 0: the part has none; all ones: the row cannot be drawn from
   float min;            // the smallest finite logit, +inf: none
   uint32_t unused;
 };
@@ -232,12 +236,12 @@ __device__ __forceinline__ uint64_t Seen::best() const {
 }
 
 __global__ void __launch_bounds__(kPartThreads)
-draw_best_kernel(const float* __restrict__ logits, int rows, int vocab, int part_len, int parts, PartStat* __restrict__ stats) {
+draw_best_kernel(const float* __restrict__ logits, int rows, int vocab, int part_len, int parts, int finite, PartStat* __restrict__ stats) {
   __shared__ uint64_t best_of[kPartThreads / kWave];
   __shared__ float min_of[kPartThreads / kWave];
   const int row = row_of(parts), part = part_of(parts), begin = part * part_len, end = min(vocab, begin + part_len);
   if (row >= rows) return;
-  Seen seen;
+  Seen seen{begin, end, finite != 0};
   scan_tokens<kPartThreads, 4>(logits + static_cast<size_t>(row) * vocab, begin, end, [&](int first, const float4& four) { seen.take(first, four); });
   uint64_t best = seen.best();
   float least = seen.least;
@@ -851,7 +855,7 @@ struct RowShared {
 // runs, 28 us for a row of 32000 tokens.)
 __global__ void __launch_bounds__(kRowThreads)
 draw_row_kernel(const float* __restrict__ logits, int vocab, const float* __restrict__ uniform, const float* __restrict__ temperature,
-                const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p, int shift,
+                const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p, int shift, int finite,
                 int* __restrict__ out, float* __restrict__ logprob) {
   __shared__ RowShared s;
   constexpr int kWaves = kRowThreads / kWave, kOwn = kClasses / kRowThreads;
@@ -859,7 +863,7 @@ draw_row_kernel(const float* __restrict__ logits, int vocab, const float* __rest
   const float* row = logits + static_cast<size_t>(r) * vocab;
   const Ask ask = ask_of(r, uniform, temperature, top_k, top_p, min_p);
   // ---- the first token, the least logit, and whether the row can be drawn from ----
-  Seen seen;
+  Seen seen{0, vocab, finite != 0};
   scan_tokens<kRowThreads, 4>(row, 0, vocab, [&](int first, const float4& four) { seen.take(first, four); });
   uint64_t best = seen.best();
   float least = seen.least;
@@ -969,9 +973,9 @@ extern "C" void tlie_draw_scratch(int rows, int parts, long long* starts) {
 
 // logits: float [rows, vocab], vocab < 2^24; uniform: float [rows]; temperature, top_k, top_p, min_p: [rows] or null; parts: 1 to 8, or 0: a row by
 // one workgroup (scratch is then null);
-// out: int [rows]; logprob: float [rows] or null.  scratch: rows * (kRowBytes + parts * kPartBytes) bytes, at a multiple of 16.
+// finite: not 0, a row with a logit of -inf cannot be drawn from either; out: int [rows]; logprob: float [rows] or null.  scratch: rows * (kRowBytes + parts * kPartBytes) bytes, at a multiple of 16.
 extern "C" int tlie_draw(const float* logits, int rows, int vocab, const float* uniform, const float* temperature, const int* top_k,
-                         const float* top_p, const float* min_p, int parts, void* scratch, int* out, float* logprob, void* stream) {
+                         const float* top_p, const float* min_p, int finite, int parts, void* scratch, int* out, float* logprob, void* stream) {
   if (rows <= 0 || vocab <= 0 || vocab >= (1 << 24) || parts < 0 || parts > kPartsMost || rows > 65535 ||
       uniform == nullptr || (parts > 0 && (scratch == nullptr || reinterpret_cast<uintptr_t>(scratch) % 16 != 0)))
     return kBadArgument;
@@ -979,8 +983,8 @@ extern "C" int tlie_draw(const float* logits, int rows, int vocab, const float* 
   int shift = 44;                                   // the weights' sum stays below 2^62
   while ((static_cast<long long>(vocab) << shift) >= (1ll << 62)) --shift;
   if (parts == 0) {
-    hipLaunchKernelGGL(draw_row_kernel, dim3(rows), dim3(kRowThreads), 0, s, logits, vocab, uniform, temperature, top_k, top_p, min_p, shift, out,
-                       logprob);
+    hipLaunchKernelGGL(draw_row_kernel, dim3(rows), dim3(kRowThreads), 0, s, logits, vocab, uniform, temperature, top_k, top_p, min_p, shift,
+                       finite, out, logprob);
     return launch_status();
   }
   const int part_len = (vocab + parts - 1) / parts;
@@ -993,7 +997,7 @@ extern "C" int tlie_draw(const float* logits, int rows, int vocab, const float* 
   uint32_t* class_count = reinterpret_cast<uint32_t*>(base + at.class_count);
   double* sums = reinterpret_cast<double*>(base + at.sums);
   const dim3 grid((rows + kDies - 1) / kDies * kDies * parts);
-  hipLaunchKernelGGL(draw_best_kernel, grid, dim3(kPartThreads), 0, s, logits, rows, vocab, part_len, parts, stats);
+  hipLaunchKernelGGL(draw_best_kernel, grid, dim3(kPartThreads), 0, s, logits, rows, vocab, part_len, parts, finite, stats);
   hipLaunchKernelGGL(draw_weigh_kernel, grid, dim3(kPartThreads), 0, s, logits, rows, vocab, part_len, parts, stats, temperature, shift,
                      logprob != nullptr ? 1 : 0, class_mass, class_count, sums);
   if (temperature != nullptr)

@@ -2139,7 +2139,7 @@ def draw_parts(rows: int, vocab: int) -> int:
 
 def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
                     top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None, logprobs: bool = False,
-                    out: torch.Tensor | None = None, out_logprobs: torch.Tensor | None = None):
+                    out: torch.Tensor | None = None, out_logprobs: torch.Tensor | None = None, finite: bool = False):
     """One token per row of float32 logits [rows, vocab], from given random numbers `uniform` (float32 [rows], in [0, 1)).
 
     Tokens stand in descending order of their logits, equal ones by index, with weights exp((logit - max) / temperature).  Kept are
@@ -2150,6 +2150,7 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: to
     top_k, top_p and min_p holds one entry a row.  A logit of -inf is a token that cannot be drawn; a row with a NaN or +inf, or
     of -inf alone, gives -1 (and a NaN).  Weights are summed as whole numbers of 2^-44 of the largest (fewer bits beyond a vocabulary of
     262144): what is lighter than half of that is never drawn, and the same inputs give the same token in any batch.
+    finite: a row with a logit of -inf gives -1 (and a NaN) too, as in `sample`.
     logprobs: also returns float32 [rows], log softmax(logits)[token] of the logits as they are, without temperature and filters.
     out (int32 [rows]), out_logprobs (float32 [rows]): to write into, else new tensors."""
     current = _expect("sample_filtered", ((logits, "logits", torch.float32), (uniform, "uniform", torch.float32)),
@@ -2173,8 +2174,8 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, temperature: to
     if rows > 0:
         parts = draw_parts(rows, vocab)
         scratch = torch.empty((rows * (DRAW_ROW_BYTES + parts * DRAW_PART_BYTES),), dtype=torch.uint8, device=logits.device) if parts else None
-        _check(_entry("tlie_draw", "piipppppipppp")(logits.data_ptr(), rows, vocab, uniform.data_ptr(), _address(temperature), _address(top_k), _address(top_p),
-                                                    _address(min_p), parts, _address(scratch), out.data_ptr(), _address(out_logprobs),
+        _check(_entry("tlie_draw", "piipppppiipppp")(logits.data_ptr(), rows, vocab, uniform.data_ptr(), _address(temperature), _address(top_k), _address(top_p),
+                                                    _address(min_p), int(finite), parts, _address(scratch), out.data_ptr(), _address(out_logprobs),
                                                     torch._C._cuda_getCurrentRawStream(current)),
                "sample_filtered")
     return (out, out_logprobs) if logprobs else out

@@ -144,7 +144,7 @@ class Sampler:
         device = self._floats[:, :rows]
         logprobs = self._logprobs[:rows] if wants_logprobs else None
         ops.sample_filtered(logits, device[3], device[0], top_k=self._top_k[:rows], top_p=device[1], min_p=device[2], logprobs=wants_logprobs, out=out,
-                            out_logprobs=logprobs)
+                            out_logprobs=logprobs, finite=True)
         if all(filtered):
             return
         longs[0, :rows] = torch.tensor([_signed(int(p.seed)) for p in params], dtype=torch.int64)
