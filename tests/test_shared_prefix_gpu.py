@@ -309,3 +309,22 @@ def test_pages_past_32_bits(heads, sequences, groups):
     cache[last:] = step["cache"].to(DEV)
     step["cache"], step["table"] = cache, step["table"] + last
     assert torch.equal(call(step), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (24, 8, 80), (64, 1, 128), (40, 1, 32)])
+@pytest.mark.parametrize("softcap", [0.02, 1.0, 50.0, 1000.0, 1030.0, 3e4, 1e6, 1e12, 1e30])
+def test_caps_of_any_size(dtype, heads, kv_heads, dim, softcap):
+    """A cap far above the scores leaves them as they are: their tangent hyperbolic is then taken of very small numbers."""
+    check(make_step(20, dtype, heads, kv_heads, dim, 16, [(150, 1), (170, 3), (133, 1)], [(0, 2, 140)]), softcap)
+
+
+def test_caps_beyond_what_a_float_tells_apart_are_refused():
+    """scale / softcap below the smallest float of 24 bits."""
+    step = make_step(21, BF16, 8, 2, 64, 16, [(50, 1), (60, 1)], [(0, 2, 40)])
+    plan = ops.shared_prefix_plan(step["start"], step["lengths"], step["groups"], 8, 2, 64, BF16, DEV)
+    q, cache, table, positions = (step[name].to(DEV) for name in ("q", "cache", "table", "positions"))
+    for scale, softcap in ((1e-3, 2e38), (1e-20, 1e25), (0.125, 1.1e37)):
+        with pytest.raises(EngineError):
+            ops.attention_shared_prefix(q, cache, table, positions, plan, 8, 2, 64, scale, softcap=softcap)
+    ops.attention_shared_prefix(q, cache, table, positions, plan, 8, 2, 64, 0.125, softcap=1e37)

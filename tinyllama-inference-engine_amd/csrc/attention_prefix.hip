@@ -45,6 +45,34 @@ __device__ __forceinline__ int page_of(const int* __restrict__ pages, int key, i
   return pages[__builtin_amdgcn_readfirstlane(min(max(key >> page_shift, page_lo), page_hi))];
 }
 
+// tanh(t) of each score, t in units of the cap.  1 - 2 / (e^2t + 1) is off by up to 2^-22, however small t: a capped score by that share of the cap (a
+// cap of 10^6 left scores of 5 wrong by 0.06).  In bfloat16, up to a cap of 1024, it is an eighth of a probability's rounding of 2^-9.  Beyond, and in 32
+// bits, small t by their series to the seventh power (62 / 2835 t^8 < 2^-29 of it left), from an eighth on the first form (2^-19 of t).  With both for
+// all caps in bfloat16, 8 capped questions behind 4000 positions take 69.8 us in place of 60.5, three documents 15.1 in place of 14.4.
+template <bool FLOAT, int CT, int TILES>
+__device__ __forceinline__ void cap_scores(floatx4 (&s)[CT][TILES], float cap_pre, float scale_log2) {
+  auto direct = [](float x) {
+    const float grown = __builtin_amdgcn_exp2f(x * 2.8853900817779268f) + 1.f;
+    return 1.f - (FLOAT ? 2.f / grown : 2.f * __builtin_amdgcn_rcpf(grown));
+  };
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[ct][t][j] = f(s[ct][t][j] * cap_pre);
+  };
+  if (!FLOAT && scale_log2 <= 1024.f * 1.4426950408889634f) {                // (the same for the whole launch)
+    each(direct);
+    return;
+  }
+  each([&](float x) {
+    const float square = x * x, series = fmaf(x * square, fmaf(square, fmaf(square, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), x);
+    return fabsf(x) < 0.125f ? series : direct(x);
+  });
+}
+
 // Where an item that leaves its columns' results themselves has them go, and the keys 0 .. shared - 1 that it reads through another row.
 struct Direct {
   const int* pages;
@@ -170,18 +198,7 @@ __device__ __forceinline__ void prefix_item(const PrefixItem& item, const Direct
         }
       }
     settle(s);                                            // (branches follow, behind which the scores are read)
-    if (cap_pre > 0.f) {
-      // cap * tanh(s * scale / cap) = cap * (1 - 2 / (2^(2 log2(e) s scale / cap) + 1)); the cap is part of scale_log2
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float grown = __builtin_amdgcn_exp2f(s[ct][t][j] * (cap_pre * 2.8853900817779268f)) + 1.f;
-            s[ct][t][j] = 1.f - (FLOAT ? 2.f / grown : 2.f * __builtin_amdgcn_rcpf(grown));
-          }
-    }
+    if (cap_pre > 0.f) cap_scores<FLOAT>(s, cap_pre, scale_log2);          // (the cap is part of scale_log2)
     if (ragged) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
@@ -490,15 +507,7 @@ __device__ __forceinline__ void prefix_wide_item(const PrefixItem& item, int kvh
 #pragma unroll
         for (int w = 0; w < 4; ++w) values[dt][w] &= keep[w];
     }
-    if (cap_pre > 0.f) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            s[ct][t][j] = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[ct][t][j] * (cap_pre * 2.8853900817779268f)) + 1.f);
-    }
+    if (cap_pre > 0.f) cap_scores<false>(s, cap_pre, scale_log2);
     if (ragged) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
@@ -798,7 +807,8 @@ extern "C" int tlie_attention_prefix(const void* q, const void* cache, int dtype
     return kBadArgument;
   const bool is_direct = part_o == nullptr;
   const float scale_log2 = (softcap > 0.f ? softcap : scale) * 1.4426950408889634f, cap_pre = softcap > 0.f ? scale / softcap : 0.f;
-  if (!(scale_log2 < INFINITY) || !(cap_pre < INFINITY) || (softcap > 0.f && !(cap_pre > 0.f))) return kBadArgument;
+  // (below 2^-126 a number has fewer than 24 bits, and the scores would have no more)
+  if (!(scale_log2 < INFINITY) || !(cap_pre < INFINITY) || (softcap > 0.f && !(cap_pre >= 1.17549435e-38f))) return kBadArgument;
   const int page_shift = 31 - __builtin_clz(page_size);
   hipStream_t s = (hipStream_t)stream;
   int status = kBadArgument;
