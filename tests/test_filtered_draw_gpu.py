@@ -330,3 +330,23 @@ def test_rows_that_have_to_be_finite(rows, vocab):
         got, logprobs = draw(masked, finite=True)
         assert got[1] == -1 and math.isnan(logprobs[1]), place
         assert torch.equal(got[[0] + list(range(2, rows))], want[[0] + list(range(2, rows))])
+
+
+@pytest.mark.parametrize("gap", [4.0, 8.3, 9.7, 11.9, 13.7])
+@pytest.mark.parametrize("rows,vocab", [(3, 200003), (40, 33000)])
+def test_log_probabilities_of_mass_far_below_the_maximum(rows, vocab, gap):
+    """One high logit, and most of the weight (or as much as the vocabulary holds) at a gap below it.  A term of the sum is off by (2 + 1.2 gap)
+    2^-23 of it (the difference's and the product's roundings 2^-24 of the gap each, log2(e)'s own 2^-26; an exponential and a sum of four 2^-23
+    each), the sum by the mean of these by weight; the logarithm's error is the sum's relative one, and the result is rounded to 2^-24 of it."""
+    gen = torch.Generator().manual_seed(vocab)
+    logits = 3.0 - gap + 0.3 * torch.randn((rows, vocab), generator=gen).clamp(-3, 3)
+    logits[:, 17] = 3.0 + torch.rand((rows,), generator=gen)
+    uniform, temperature = torch.rand((rows,), generator=gen), torch.where(torch.arange(rows) % 3 == 0, 0.0, 1.0)
+    tokens, logprobs = ops.sample_filtered(logits.to(DEV), uniform.to(DEV), temperature.to(DEV), logprobs=True)
+    wide = logits.double()
+    below = wide.max(dim=1, keepdim=True).values - wide
+    weights = torch.exp(-below)
+    mean = (weights * below).sum(dim=1) / weights.sum(dim=1)
+    want = torch.log_softmax(wide, dim=1).gather(1, tokens.cpu().long().unsqueeze(1)).squeeze(1)
+    bound = (2.0 + 1.2 * mean) * 2.0 ** -23 + 2.0 ** -24 * want.abs()
+    assert float(((logprobs.double().cpu() - want).abs() - bound).max()) <= 0.0
