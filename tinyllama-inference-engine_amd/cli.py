@@ -18,7 +18,7 @@ holds `{"greedy_tokens": [...]}` and the (first prompt's) generated tokens must 
 Options (after the positionals): --dtype bfloat16|float32, --temperature T, --top-p P, --seed S
 (the reference's request options of the same names, app/server.cpp:601-613), --top-k K, --min-p P (both narrow the draw further);
 --answers N (so many to each prompt, which share its cache; the output then has `answers`, a list per prompt under `requests`), --logprobs
-(the tokens' log-probabilities beside them); the cache and the
+(the tokens' log-probabilities beside them, `logprobs` and `answer_logprobs`); the cache and the
 scheduler: --max-cache-tokens N (positions the page pool holds), --page-size P, --max-requests R
 (request slots), --max-tokens-per-step T (a step's token budget), --chunk-size C (the most tokens of
 one prompt in a step), --prompt-tokens-beside-decodes N (the most prompt tokens in a step that also
@@ -151,7 +151,8 @@ def command_generate(args) -> int:
         result["requests"] = [{"prompt_tokens": len(prompt), "generated_tokens": output,
                                **({"text": tokenizer.decode(output)} if tokenizer is not None else {}),
                                **({"logprobs": logprobs[index]} if logprobs is not None else {}),
-                               **({"answers": answers[index]} if args.answers > 1 else {})}
+                               **({"answers": answers[index]} if args.answers > 1 else {}),
+                               **({"answer_logprobs": logprob_answers[index]} if args.answers > 1 and logprobs is not None else {})}
                               for index, (prompt, output) in enumerate(zip(prompts, outputs))]
     print(json.dumps(result))
     return 0
