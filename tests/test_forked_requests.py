@@ -222,3 +222,45 @@ def test_a_plan_made_within_a_step_is_waited_for_by_the_next(monkeypatch):
     assert graph.prefix_plan(8, 2, 64, torch.bfloat16) == "plan"
     assert log == ["fill", "record"]
     assert graph.prefix_plan(8, 2, 64, torch.bfloat16) == "plan" and log == ["fill", "record"]
+
+
+@pytest.mark.parametrize("length", [16, 17, 21])
+def test_a_member_that_does_not_fit_yet_is_not_forked(monkeypatch, length):
+    """Blocked over many steps, for want of pages: no fork is made (each copies a page of every layer) until one that then runs.
+    Prompts whose shared positions end inside a page and at its end."""
+    cache = manager(pages=11, requests=8)
+    forks, real = [], cache.fork
+    monkeypatch.setattr(cache, "fork", lambda *call: (forks.append(call[1]), real(*call))[1])
+    scheduler = Scheduler(cache)
+    family = family_of(2, range(length), max_tokens=9)
+    other = Request(id="other", prompt=list(range(13)), params=SamplingParams(max_tokens=8))
+    for request in (family[0], other, family[1]):
+        scheduler.add(request)
+    blocked = 0
+    for _ in range(60):
+        if not scheduler.has_work():
+            break
+        before = len(forks)
+        plan = scheduler.schedule()
+        assert cache.reserve_all([(item.request.id, item.count) for item in plan])
+        for item in plan:
+            cache.commit(item.request.id, item.count)
+        cache.check()
+        planned = [item.request.id for item in plan]
+        assert all(name in planned for name in forks[before:])
+        blocked += family[1].state == "waiting" and family[0].computed >= length
+        scheduler.update(plan, [item.first + item.count for item in plan if item.samples])
+    assert not scheduler.has_work() and blocked > 2
+    assert forks.count(family[1].id) <= 1 + family[1].preemptions
+    assert [len(request.generated) for request in (*family, other)] == [9, 9, 8]
+
+
+@pytest.mark.parametrize("length,count", [(1, 1), (3, 1), (4, 1), (5, 3), (8, 9), (10, 1)])
+def test_the_pages_that_a_fork_takes(length, count):
+    cache = manager()
+    cache.admit("a")
+    grow(cache, "a", 10)
+    free, wanted = cache.free_pages(), cache.pages_to_fork(length, count)
+    cache.fork("a", "b", length)
+    cache.reserve("b", count)
+    assert cache.free_pages() == [have - need for have, need in zip(free, wanted)]

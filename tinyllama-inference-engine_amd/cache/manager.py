@@ -219,6 +219,10 @@ class CacheManager:
         blocks = self._blocks_for(entry.length + count)
         return [max(0, blocks - len(entry.pages[group])) for group in range(len(self.groups))]
 
+    def pages_to_fork(self, length: int, count: int) -> list[int]:
+        """Per group, how many new pages a fork of `length` positions takes by the time it has `count` more."""
+        return [self._blocks_for(length + count) - length // self.page_size for _ in self.groups]
+
     def free_pages(self) -> list[int]:
         return [group.allocator.num_free for group in self.groups]
 

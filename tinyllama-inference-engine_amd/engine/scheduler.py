@@ -264,14 +264,8 @@ class Scheduler:
         # 3. new requests, first come first served, while a slot, budget and pages allow
         while self.waiting and budget > 0 and len(plan) < self.max_seqs_per_step and self.cache.free_slots > 0:
             request = self.waiting[0]
-            if not self._enter(request, planned_pages):
-                break
-            count = 0
-            if not self.running or self.admit_partial or self._fits_whole(request):
-                count = self._portion(request, budget, planned_pages)
+            count = self._enter(request, budget, planned_pages)
             if count <= 0:
-                self.cache.release(request.id)
-                request.computed = 0
                 break
             self.waiting.popleft()
             request.state = "running"
@@ -281,25 +275,36 @@ class Scheduler:
             take(request, count)
         return plan
 
-    def _enter(self, request: Request, planned_pages: list[int]) -> bool:
-        """Gives a waiting request its slot, as a fork of a member of its family where that has the prompt's keys.  False: it waits, for a
-        member that is still computing them, or for a page."""
+    def _enter(self, request: Request, budget: int, planned_pages: list[int]) -> int:
+        """Gives a waiting request its slot, as a fork of a member of its family where that has the prompt's keys, and returns how many
+        tokens of it the step takes.  0: it waits, for a member that is still computing them, or for pages, and holds nothing; a fork, which
+        copies a page of every layer, is made only of a request that then runs."""
         base = len(request.prompt) - 1            # (the last token runs again: its logits are asked for)
+        alone = not self.running or self.admit_partial           # (what comes later may find no page)
         members = [member for member in request.family or () if member is not request and member.state == "running"]
-        if not members or base < self.cache.page_size or not self.cache.can_fork:
+        if members and base >= self.cache.page_size and self.cache.can_fork:
+            source = next((member for member in members if self.cache.length(member.id) >= base), None)
+            # (a page beyond those planned for is one for its next token)
+            if (source is None or any(free <= planned for free, planned in zip(self.cache.free_pages(), planned_pages))
+                    or not (alone or self._fits_whole(self.cache.pages_to_fork(base, request.total - base)))):
+                return 0
+            self.cache.fork(source.id, request.id, base)
+            request.computed = base
+        else:
             self.cache.admit(request.id)
-            return True
-        source = next((member for member in members if self.cache.length(member.id) >= base), None)
-        if source is None or any(free <= planned for free, planned in zip(self.cache.free_pages(), planned_pages)):
-            return False
-        self.cache.fork(source.id, request.id, base)
-        request.computed = base
-        return True
+            if not (alone or self._fits_whole(self.cache.pages_needed(request.id, request.remaining))):
+                self.cache.release(request.id)
+                return 0
+        count = self._portion(request, budget, planned_pages)
+        if count <= 0:
+            self.cache.release(request.id)
+            request.computed = 0
+        return count
 
-    def _fits_whole(self, request: Request) -> bool:
-        """Whether the pools have room for all of the (just admitted) request's tokens after what the
+    def _fits_whole(self, wanted: list[int]) -> bool:
+        """Whether the pools have room for the pages that all of a request's tokens take (wanted, per group) after what the
         running requests still need for theirs, with a page of growth for each of them and for it."""
-        wanted = self.cache.pages_needed(request.id, request.remaining)
+        wanted = list(wanted)
         for other in self.running:
             for group, pages in enumerate(self.cache.pages_needed(other.id, other.remaining)):
                 wanted[group] += pages
