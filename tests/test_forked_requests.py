@@ -264,3 +264,40 @@ def test_the_pages_that_a_fork_takes(length, count):
     cache.fork("a", "b", length)
     cache.reserve("b", count)
     assert cache.free_pages() == [have - need for have, need in zip(free, wanted)]
+
+
+def test_requests_behind_a_member_that_waits_for_its_familys_keys_go_on():
+    """A long prompt is computed in portions; its second answer waits for that, other prompts do not.  Its turn is the first when
+    the keys are there."""
+    cache = manager(pages=200, requests=8)
+    scheduler = Scheduler(cache, max_tokens_per_step=16, chunk_size=8)
+    family = family_of(3, range(80), max_tokens=4)
+    others = [Request(id=("other", index), prompt=list(range(6 + index)), params=SamplingParams(max_tokens=4)) for index in range(3)]
+    for request in (*family, *others):
+        scheduler.add(request)
+    seen = run(scheduler, cache)
+    begins = lambda name: next(index for index, step in enumerate(seen) if any(one == name for one, _, _ in step))
+    assert begins(("other", 0)) == 0 and begins(("other", 2)) < begins(family[1].id)
+    assert begins(family[1].id) == begins(family[2].id) == 1 + max(index for index, step in enumerate(seen) if (family[0].id, 72, 8) in step)
+
+
+def test_a_member_that_waits_for_pages_lets_nobody_ahead():
+    """First come, first served, once the keys are there: a request behind it that would fit does not take the pages it waits for."""
+    cache = manager(pages=12, requests=8)
+    scheduler = Scheduler(cache)
+    family = family_of(2, range(17), max_tokens=16)
+    small = Request(id="small", prompt=[1, 2], params=SamplingParams(max_tokens=3))
+    scheduler.add(family[0])
+    scheduler.add(family[1])
+    seen = []
+    while scheduler.has_work():
+        plan = scheduler.schedule()
+        assert cache.reserve_all([(item.request.id, item.count) for item in plan])
+        for item in plan:
+            cache.commit(item.request.id, item.count)
+        seen.append([item.request.id for item in plan])
+        scheduler.update(plan, [item.first + item.count for item in plan if item.samples])
+        if len(seen) == 1:                                # (the prompt's keys are there now; its second answer does not fit beside the first)
+            scheduler.add(small)
+    begins = lambda name: next(index for index, step in enumerate(seen) if name in step)
+    assert begins("small") >= begins(family[1].id) > 2

@@ -28,8 +28,8 @@ prompts, cut into portions.  Pages are taken as a request grows, so they can run
     portion fits.
 
 Requests of one family (`Request.family`: several answers to one prompt) share the prompt's pages where the cache can: a member is
-admitted as a fork of one that has the prompt's keys already, and waits while one is still computing them; all it brings then
-is the prompt's last token, whose logits its first token is drawn from.
+admitted as a fork of one that has the prompt's keys already, and waits while one is still computing them (requests behind it
+are then admitted before it); all it brings then is the prompt's last token, whose logits its first token is drawn from.
 
 The scheduler owns no device memory and calls no kernel: it plans with the cache manager's
 counts, and the engine loop runs what it plans.
@@ -261,13 +261,22 @@ class Scheduler:
             if count > 0:
                 take(request, count)
 
-        # 3. new requests, first come first served, while a slot, budget and pages allow
-        while self.waiting and budget > 0 and len(plan) < self.max_seqs_per_step and self.cache.free_slots > 0:
-            request = self.waiting[0]
+        # 3. new requests, first come first served, while a slot, budget and pages allow; past a member that waits for its
+        # family's keys those behind it may go first
+        place, computing = 0, set()
+        while place < len(self.waiting) and budget > 0 and len(plan) < self.max_seqs_per_step and self.cache.free_slots > 0:
+            request = self.waiting[place]
+            if id(request.family) in computing:
+                place += 1
+                continue
             count = self._enter(request, budget, planned_pages)
+            if count is None:
+                computing.add(id(request.family))
+                place += 1
+                continue
             if count <= 0:
                 break
-            self.waiting.popleft()
+            del self.waiting[place]
             request.state = "running"
             self._admitted += 1
             request.order = self._admitted
@@ -275,17 +284,19 @@ class Scheduler:
             take(request, count)
         return plan
 
-    def _enter(self, request: Request, budget: int, planned_pages: list[int]) -> int:
+    def _enter(self, request: Request, budget: int, planned_pages: list[int]) -> int | None:
         """Gives a waiting request its slot, as a fork of a member of its family where that has the prompt's keys, and returns how many
-        tokens of it the step takes.  0: it waits, for a member that is still computing them, or for pages, and holds nothing; a fork, which
-        copies a page of every layer, is made only of a request that then runs."""
+        tokens of it the step takes.  0: it waits for pages; None: for a member that is still computing the keys; it then holds nothing.  A fork,
+        which copies a page of every layer, is made only of a request that then runs."""
         base = len(request.prompt) - 1            # (the last token runs again: its logits are asked for)
         alone = not self.running or self.admit_partial           # (what comes later may find no page)
         members = [member for member in request.family or () if member is not request and member.state == "running"]
         if members and base >= self.cache.page_size and self.cache.can_fork:
             source = next((member for member in members if self.cache.length(member.id) >= base), None)
+            if source is None:
+                return None
             # (a page beyond those planned for is one for its next token)
-            if (source is None or any(free <= planned for free, planned in zip(self.cache.free_pages(), planned_pages))
+            if (any(free <= planned for free, planned in zip(self.cache.free_pages(), planned_pages))
                     or not (alone or self._fits_whole(self.cache.pages_to_fork(base, request.total - base)))):
                 return 0
             self.cache.fork(source.id, request.id, base)
