@@ -283,10 +283,11 @@ def test_requests_behind_a_member_that_waits_for_its_familys_keys_go_on():
 
 def test_a_member_that_waits_for_pages_lets_nobody_ahead():
     """First come, first served, once the keys are there: a request behind it that would fit does not take the pages it waits for."""
-    cache = manager(pages=12, requests=8)
+    cache = manager(pages=9, requests=8)
     scheduler = Scheduler(cache)
     family = family_of(2, range(17), max_tokens=16)
     small = Request(id="small", prompt=[1, 2], params=SamplingParams(max_tokens=3))
+    family[1].generated = [3] * 8                         # (preempted before: it brings these too, on three pages)
     scheduler.add(family[0])
     scheduler.add(family[1])
     seen = []
