@@ -302,3 +302,68 @@ def test_a_member_that_waits_for_pages_lets_nobody_ahead():
             scheduler.add(small)
     begins = lambda name: next(index for index, step in enumerate(seen) if name in step)
     assert begins("small") >= begins(family[1].id) > 2
+
+
+def runner_of(cache, kv_heads=8, dim=128):
+    from tlie_amd.engine.step import ModelRunner
+    mixer = SimpleNamespace(nkv=kv_heads, d=dim, takes_shared_prefix=True)
+    model = SimpleNamespace(device="cpu", spec=SimpleNamespace(vocab_size=100), blocks=[SimpleNamespace(mixer=mixer)])
+    return ModelRunner(model, cache, use_graphs=False)
+
+
+def test_steps_without_families_are_not_looked_through(monkeypatch):
+    """A step of an engine without forks asks no request for its pages; the last fork's end brings that back."""
+    from tlie_amd.engine.step import StepEntry
+    cache = manager(pages=200, requests=8, page_size=16)
+    runner = runner_of(cache)
+    asked, real = [], cache.held
+    monkeypatch.setattr(cache, "held", lambda request: (asked.append(request), real(request))[1])
+    for name in "abcd":
+        cache.admit(name)
+        grow(cache, name, 40)
+    entries = [StepEntry(name, [1], [0]) for name in "abcd"]
+    assert runner.shared_groups(entries) == [] and not asked and not cache.has_families
+    cache.fork("a", "e", 33)
+    assert cache.has_families
+    runner.shared_groups(entries)
+    assert asked == list("abcd")
+    cache.release("a")
+    assert cache.has_families
+    cache.release("e")
+    asked.clear()
+    assert runner.shared_groups(entries[1:]) == [] and not asked and not cache.has_families
+    cache.fork("b", "e", 15)                     # (less than a page: nothing is held together)
+    assert not cache.has_families
+
+
+def test_groups_are_runs_of_one_family(monkeypatch):
+    from tlie_amd.engine import step
+    monkeypatch.setattr(step, "ops_shared_prefix_pays", lambda *sizes: True)
+    rng = random.Random(1)
+    for _ in range(60):
+        cache = manager(pages=400, requests=40, page_size=16)
+        names, live = iter(range(1000)), []
+        for _ in range(4):
+            root = next(names)
+            cache.admit(root)
+            grow(cache, root, rng.randint(1, 90))
+            live.append(root)
+            for _ in range(rng.randint(0, 4)):
+                fork = next(names)
+                source = rng.choice(live)
+                cache.fork(source, fork, rng.randint(1, cache.length(source)))
+                live.append(fork)
+        for name in rng.sample(live, rng.randint(0, 3)):
+            cache.release(name)
+            live.remove(name)
+        assert cache.has_families == any(cache.held(name).family for name in live)
+        rng.shuffle(live)
+        live.sort(key=lambda name: cache.held(name).family if rng.random() < 0.8 else 0)
+        covered = [None] * len(live)
+        for group, (first, count, prefix) in enumerate(runner_of(cache).shared_groups([step.StepEntry(name, [1], [0]) for name in live])):
+            held = [cache.held(name) for name in live[first:first + count]]
+            assert count > 1 and prefix == min(info.shared for info in held) > 0 and len({info.family for info in held}) == 1 and held[0].family
+            covered[first:first + count] = [group] * count
+        for index in range(1, len(live)):
+            one, other = cache.held(live[index - 1]), cache.held(live[index])
+            assert (covered[index] is not None and covered[index] == covered[index - 1]) == (one.family == other.family != 0)

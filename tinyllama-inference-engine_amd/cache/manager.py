@@ -99,6 +99,7 @@ class CacheManager:
         self._free_slots = list(range(max_requests - 1, -1, -1))   # popped from the end: slot 0 first
         self._slot_in_use = bytearray(max_requests)
         self._admissions = 0
+        self._in_families = 0                              # live requests that hold pages with others (or did)
         self.state_areas: list[torch.Tensor] = []
 
         group_of_window: dict[int | None, int] = {}
@@ -185,8 +186,15 @@ class CacheManager:
         if whole:
             if not entry.family:
                 entry.family, entry.shared = entry.serial, whole * self.page_size
+                self._in_families += 1
+            self._in_families += 1
             forked.family, forked.shared = entry.family, min(whole * self.page_size, entry.shared)
         return slot
+
+    @property
+    def has_families(self) -> bool:
+        """Whether a live request is a fork, or has been forked."""
+        return self._in_families > 0
 
     def is_live(self, request: Hashable) -> bool:
         return request in self._requests
@@ -314,6 +322,7 @@ class CacheManager:
             raise invalid_argument(f"request slot {entry.slot} is freed twice")
         self._slot_in_use[entry.slot] = 0
         self._free_slots.append(entry.slot)
+        self._in_families -= entry.family != 0
         del self._requests[request]
 
     def page_list(self, request: Hashable, group: int) -> list[int]:

@@ -13,6 +13,8 @@ from __future__ import annotations
 import gc
 import weakref
 from dataclasses import dataclass, field
+from itertools import groupby
+from operator import attrgetter
 from typing import Hashable, Sequence
 
 import numpy as np
@@ -164,15 +166,14 @@ class ModelRunner:
     def shared_groups(self, entries: Sequence[StepEntry]) -> list[tuple[int, int, int]]:
         """The step's groups (first sequence, sequences, prefix) of neighbouring entries that hold the same pages, when reading those
         pages once for all of them pays; else none."""
-        if not self._prefix_sizes or len(entries) < 2 or not 16 <= self.cache.page_size <= 65536:
+        if not self.cache.has_families or not self._prefix_sizes or len(entries) < 2 or not 16 <= self.cache.page_size <= 65536:
             return []
-        groups, held = [], [self.cache.held(entry.request) for entry in entries]
-        first = 0
-        for index in range(1, len(held) + 1):
-            if index == len(held) or held[index].family != held[first].family or not held[first].family:
-                if index - first > 1:
-                    groups.append((first, index - first, min(info.shared for info in held[first:index])))
-                first = index
+        groups, held, first = [], [self.cache.held(entry.request) for entry in entries], 0
+        for family, members in groupby(held, attrgetter("family")):
+            shared = [info.shared for info in members]
+            if family and len(shared) > 1:
+                groups.append((first, len(shared), min(shared)))
+            first += len(shared)
         return groups if groups and any(ops_shared_prefix_pays(groups, *sizes) for sizes in self._prefix_sizes) else []
 
     def _length_bucket(self, longest: int) -> int:
