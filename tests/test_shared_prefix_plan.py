@@ -190,3 +190,54 @@ def test_a_recorded_plans_buffer_is_written_behind_its_last_transfer():
 def test_more_tokens_than_a_launch_takes_are_refused_and_not_allocated(start, lengths):
     with pytest.raises(EngineError):
         ops.shared_prefix_plan(start, lengths, [], 8, 4, 64, torch.bfloat16, "cpu")
+
+
+def recorded(tokens, start, lengths, groups, sizes):
+    plan = ops.RecordedPrefixPlan(tokens, 1 << max(int(length) for length in lengths).bit_length(), *sizes, "cpu")
+    plan.fill(start, lengths, groups)
+    return plan.plan
+
+
+@pytest.mark.parametrize("heads,kv_heads,count,prefix", [(32, 8, 24, 30000), (32, 8, 32, 20000), (32, 8, 32, 30000), (32, 8, 64, 20000), (32, 8, 64, 30000),
+                                                         (8, 1, 32, 12000), (32, 4, 64, 30000), (32, 32, 16, 30000)])
+def test_recorded_steps_are_cut_as_others_are(heads, kv_heads, count, prefix):
+    lengths = [prefix + 1 + 37 * i % 300 for i in range(count)]
+    start, sizes = range(count + 1), (heads, kv_heads, 128, torch.bfloat16)
+    items, part_first = ops.shared_prefix_items(start, lengths, [(0, count, prefix)], *sizes)
+    plan = recorded(1 << (count - 1).bit_length(), start, lengths, [(0, count, prefix)], sizes)
+    assert plan.items[:len(items)].tolist() == items.tolist() and not plan.items[len(items):].any()
+    assert plan.part_first[:count + 1].tolist() == part_first.tolist()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 4, 64), (32, 8, 128), (8, 8, 256), (40, 1, 64), (150, 1, 128), (12, 4, 48), (8, 1, 128), (32, 32, 128)])
+def test_recorded_steps_of_any_groups_are_cut_as_others_are(heads, kv_heads, dim, dtype):
+    """Groups of two sequences or more, others beside them, prefixes and own keys of any length."""
+    rng = random.Random(heads + dim)
+    for tokens in (1, 2, 4, 8, 16, 32, 64, 128, 256):
+        for _ in range(4):
+            count, groups, lengths = rng.randint(tokens // 2 + 1, tokens), [], []
+            while len(lengths) < count:
+                members = min(count - len(lengths), rng.choice([1, 2, 3, 8, count]))
+                prefix = int(2 ** rng.uniform(4, 15)) if members > 1 else 0
+                if members > 1:
+                    groups.append((len(lengths), members, prefix))
+                lengths += [prefix + int(2 ** rng.uniform(0, rng.choice([4, 9, 13]))) for _ in range(members)]
+            items, part_first = ops.shared_prefix_items(range(count + 1), lengths, groups, heads, kv_heads, dim, dtype)
+            plan = recorded(tokens, range(count + 1), lengths, groups, (heads, kv_heads, dim, dtype))
+            assert plan.items[:len(items)].tolist() == items.tolist() and not plan.items[len(items):].any()
+            assert plan.part_first[:count + 1].tolist() == part_first.tolist() and plan.parts >= part_first[-1]
+
+
+def test_a_recorded_plan_that_is_short_is_cut_as_finely_as_it_holds(monkeypatch):
+    """Not by halves: 33 parts of a prefix for room of 33 a token and one of its own each."""
+    count, prefix, sizes = 32, 30000, (32, 8, 128, torch.bfloat16)
+    lengths = [prefix + 1 + i for i in range(count)]
+    monkeypatch.setattr(ops.RecordedPrefixPlan, "room", staticmethod(lambda *sizes: (300, 34 * count)))
+    plan = recorded(count, range(count + 1), lengths, [(0, count, prefix)], sizes)
+    best = max(most for most in range(1, 65) if ops.shared_prefix_items(range(count + 1), lengths, [(0, count, prefix)], *sizes, 256, most)[1][-1] <= 34 * count)
+    items, part_first = ops.shared_prefix_items(range(count + 1), lengths, [(0, count, prefix)], *sizes, 256, best)
+    assert 24 < best < 64 and plan.items[:len(items)].tolist() == items.tolist() and plan.part_first[:count + 1].tolist() == part_first.tolist()
+    monkeypatch.setattr(ops.RecordedPrefixPlan, "room", staticmethod(lambda *sizes: (300, count)))
+    with pytest.raises(EngineError):
+        recorded(count, range(count + 1), lengths, [(0, count, prefix)], sizes)

@@ -2862,17 +2862,23 @@ class RecordedPrefixPlan:
     to `longest` positions: `fill` writes a step's work into it, on the current stream.  Items and parts beyond the step's have no tokens."""
 
     @staticmethod
-    def room(tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype) -> tuple[int, int]:
-        """(items, parts) that it holds.  With one part each, a token has ceil(G / step) items of its own and the groups ceil(columns / step) each;
-        room for parts beside."""
+    def room(tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, compute_units: int = 256) -> tuple[int, int]:
+        """(items, parts) that it holds.  With one part each, a token has ceil(G / step) items of its own and the groups ceil(columns / step)
+        each.  The plan cuts a step into some 15/8 workgroups a compute unit (csrc/attention_prefix.hip), so there are `spread` items a kv head beside
+        those, twice that where a group's last tile is cut as its wide ones are; and a group's tile has as many parts for each of its
+        tokens (with 24 a token, 32 sequences behind 30000 positions, 32 heads of 128 on 8, were cut into 16 parts for 47, and took 69.9 us for 43.9)."""
         group, step = num_heads // num_kv_heads, prefix_tile_columns(17, head_dim, dtype)
-        return tokens * -(-group // step) + -(-tokens * group // step) + tokens // 2 + 64, tokens * 24 + 256
+        spread = -(-15 * compute_units // (8 * num_kv_heads))
+        together = max(1, prefix_tile_columns(129, head_dim, dtype) // group)                  # tokens of a wide tile
+        return (tokens * -(-group // step) + -(-tokens * group // step) + tokens // 2 + max(64, 2 * spread),
+                min(PREFIX_PARTS * tokens, spread * min(tokens, 2 * together)) + 3 * tokens + spread)
 
     def __init__(self, tokens: int, longest: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device):
-        self.items, self.parts = self.room(tokens, num_heads, num_kv_heads, head_dim, dtype)
+        device = torch.device(device)
+        self._units = _compute_units(device) if device.type == "cuda" else 256
+        self.items, self.parts = self.room(tokens, num_heads, num_kv_heads, head_dim, dtype, self._units)
         self._device = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, device=device)
         self._host = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, pin_memory=self._device.is_cuda)
-        self._units = _compute_units(self._device.device) if self._device.is_cuda else 256
         self._sent = torch.cuda.Event() if self._device.is_cuda else None         # the last transfer has read the host's buffer
         self.plan = SharedPrefixPlan(self._device[:self.items * 8].view(self.items, 8), self._device[self.items * 8:], tokens, self.parts, tokens,
                                      longest, (num_heads, num_kv_heads, head_dim, dtype))
@@ -2880,7 +2886,7 @@ class RecordedPrefixPlan:
     def fill(self, seq_start, seq_len, groups) -> None:
         import numpy as np
         num_heads, num_kv_heads, head_dim, dtype = self.plan.sizes
-        host, begin, most = self._host.numpy(), self.items * 8, PREFIX_PARTS
+        host, begin = self._host.numpy(), self.items * 8
         tokens = int(seq_start[-1])
         if tokens > self.plan.tokens or len(seq_len) > self.plan.sequences:
             raise invalid_shape(f"a recorded plan for {self.plan.tokens} tokens does not hold {tokens} in {len(seq_len)} sequences")
@@ -2890,13 +2896,20 @@ class RecordedPrefixPlan:
         items, part_first = host[:begin].reshape(self.items, 8), host[begin:]
         if self._sent is not None:
             self._sent.synchronize()
-        while True:
+
+        def make(most):
             made = shared_prefix_items(seq_start, seq_len, groups, num_heads, num_kv_heads, head_dim, dtype, self._units, most, items, part_first)
-            if made is not None and int(part_first[tokens]) <= self.parts:
-                break
-            if most == 1:
+            return made if made is not None and int(part_first[tokens]) <= self.parts else None
+        made = make(PREFIX_PARTS)
+        if made is None:
+            # the most parts with which the step fits (a step's items and parts grow with the limit)
+            fits, past = 0, PREFIX_PARTS
+            while past - fits > 1:
+                middle = (fits + past) // 2
+                fits, past = (middle, past) if make(middle) is not None else (fits, middle)
+            if fits == 0:
                 raise invalid_shape("a recorded step's shared prefixes do not fit its plan")
-            most //= 2
+            made = make(fits)
         items[made[0].shape[0]:] = 0
         part_first[tokens + 1:] = part_first[tokens]
         self._device.copy_(self._host, non_blocking=True)
