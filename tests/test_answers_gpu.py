@@ -202,3 +202,46 @@ def test_logits_that_are_not_finite_are_errors_whatever_the_draw(filters):
         bad[1, 33] = value
         with pytest.raises(EngineError):
             sampler.sample(bad, params, [0, 0, 0])
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_steps_that_mix_a_family_with_portions_are_recorded(tmp_path, dtype, always_shared, counted):
+    """Answers that decode beside portions of other prompts, and portions of the family's own: by one recording per size, with changing
+    cuts, the same as launched one by one on its arrays; and, up to the other order of sums, as unrecorded and as the ordinary attention has it."""
+    folder = make_model(tmp_path / "m", CONFIG_B, 14, dtype)
+    prompt = random_tokens(40, 90, 512)
+    steps = [[("a", 1), ("b", 1), ("c", 1), ("x", 9)], [("x", 7), ("a", 1), ("b", 1)], [("a", 1), ("b", 1), ("c", 1), ("x", 9)],
+             [("b", 5), ("c", 3), ("x", 1), ("a", 1)], [("x", 2), ("y", 9), ("a", 1), ("c", 1)], [("a", 2), ("b", 2), ("c", 2), ("y", 1)]]
+    outputs = {}
+    for name, options in (("recorded", {}), ("laid out", dict(capture_graphs=False)), ("plain", dict(use_graphs=False)), ("ordinary", dict(use_graphs=False))):
+        engine = Engine(folder, dtype=dtype, max_tokens=4096, max_requests=8, **options)
+        if name == "ordinary":
+            engine.runner.shared_groups = lambda entries: []
+        for request in "axy":
+            engine.admit(request)
+        engine.step([StepEntry("a", prompt, [])])
+        for request in "bc":
+            engine.cache.fork("a", request, 85)
+            engine.step([StepEntry(request, prompt[85:], [])])
+        counted.clear()
+        others = len(engine.runner._portion_graphs)           # (of the prompts)
+        logits, at = [], 0
+        for step in steps:
+            entries = []
+            for request, count in step:
+                entries.append(StepEntry(request, [(31 * at + 7 * place) % 512 for place in range(count)], [count - 1]))
+                at += count
+            logits.append(engine.step(entries))
+        if name == "recorded":
+            assert len(engine.runner._shared_portion_graphs) == 1 and len(engine.runner._portion_graphs) == others
+            assert len(counted) == 2 * 3                      # each layer twice, to run and to record; the other steps are replays
+        else:
+            assert len(counted) == (0 if name == "ordinary" else 3 * len(steps))
+        engine.cache.check()
+        outputs[name] = torch.cat(logits).double().cpu()
+    assert torch.equal(outputs["recorded"], outputs["laid out"])
+    scale = outputs["ordinary"].abs().amax(dim=-1, keepdim=True)
+    # two results of different cuts, each within the bound of the truth (float: as above, over 3 layers)
+    tolerance = 4 * CUT_TOLERANCE[dtype] if dtype == "float32" else CUT_TOLERANCE[dtype]
+    for name in ("recorded", "plain"):
+        assert float(((outputs[name] - outputs["ordinary"]).abs() / scale).max()) <= tolerance

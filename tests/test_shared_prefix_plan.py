@@ -241,3 +241,33 @@ def test_a_recorded_plan_that_is_short_is_cut_as_finely_as_it_holds(monkeypatch)
     monkeypatch.setattr(ops.RecordedPrefixPlan, "room", staticmethod(lambda *sizes: (300, count)))
     with pytest.raises(EngineError):
         recorded(count, range(count + 1), lengths, [(0, count, prefix)], sizes)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 4, 64), (32, 8, 128), (8, 8, 256), (40, 1, 64), (12, 4, 48), (24, 8, 80), (64, 8, 64)])
+def test_recorded_steps_of_portions_are_cut_as_others_are(heads, kv_heads, dim, dtype):
+    """Families that decode, or bring portions, beside others' portions; sequences beyond the step's bring nothing."""
+    rng = random.Random(heads + dim)
+    for tokens in (16, 64, 256, 512):
+        for sequences in (8, min(64, tokens)):
+            for _ in range(4):
+                left, counts, lengths, groups = tokens, [], [], []
+                while left > 0 and len(counts) < sequences:
+                    members = min(sequences - len(counts), rng.choice([1, 2, 5, sequences]), left)
+                    prefix = int(2 ** rng.uniform(4, 15)) if members > 1 else 0
+                    if members > 1:
+                        groups.append((len(counts), members, prefix))
+                    for _ in range(members):
+                        counts.append(1 if rng.random() < 0.6 else rng.randint(1, max(1, left // 2)))
+                        counts[-1] = min(counts[-1], left)
+                        left -= counts[-1]
+                        lengths.append(prefix + counts[-1] + int(2 ** rng.uniform(0, rng.choice([4, 9, 13]))))
+                start = np.concatenate([[0], np.cumsum(counts)])
+                items, part_first = ops.shared_prefix_items(start, lengths, groups, heads, kv_heads, dim, dtype)
+                padded = np.concatenate([start, np.full(sequences - len(counts), start[-1])]), lengths + [1] * (sequences - len(counts))
+                plan = ops.RecordedPrefixPlan(tokens, 1 << max(lengths).bit_length(), heads, kv_heads, dim, dtype, "cpu", sequences)
+                plan.fill(*padded, groups)
+                plan = plan.plan
+                assert plan.sequences == sequences and plan.items[:len(items)].tolist() == items.tolist() and not plan.items[len(items):].any()
+                assert plan.part_first[:start[-1] + 1].tolist() == part_first.tolist() and (plan.part_first[start[-1]:] == part_first[-1]).all()
+                assert plan.parts >= part_first[-1]

@@ -129,10 +129,11 @@ class ModelRunner:
         self.capture = capture
         mixers = [block.mixer for block in getattr(model, "blocks", ())]
         self._prefix_sizes = {(mixer.nkv, mixer.d) for mixer in mixers if getattr(mixer, "takes_shared_prefix", False)}
-        self._shared_graphs: dict[tuple[int, int], "SharedDecodeGraph"] = {}   # of steps whose sequences share prefixes
         self.device_tokens: torch.Tensor | None = None     # int32, where sampling leaves a step's tokens (set by the engine)
         self._graphs: dict[tuple[int, int], "DecodeGraph"] = {}      # by (most sequences, longest sequence)
         self._portion_graphs: dict[tuple[int, int, int], "PortionGraph"] = {}   # by (most tokens, most sequences, longest sequence)
+        self._shared_graphs: dict[tuple[int, int], "SharedDecodeGraph"] = {}   # the same, of steps whose sequences share prefixes
+        self._shared_portion_graphs: dict[tuple[int, int, int], "SharedPortionGraph"] = {}
 
     # ---- checks and context ------------------------------------------------------------------
     def _validate(self, entries: Sequence[StepEntry]) -> None:
@@ -254,12 +255,15 @@ class ModelRunner:
                 logits = self._graphs[key].run(entries, marks[1] if marks else None)
                 if keep:
                     logits = logits.clone()
-            elif trace is None and not shared and (sizes := self.records(entries)) is not None:
+            elif trace is None and (sizes := self.records(entries)) is not None:
                 longest = max(self.cache.length(request) + count for request, count in wanted)
                 key = (*sizes, self._length_bucket(longest))
-                if key not in self._portion_graphs:
-                    self._portion_graphs[key] = PortionGraph(self, *key)
-                logits = self._portion_graphs[key].run(entries, marks[1] if marks else None)
+                graphs, kind = (self._shared_portion_graphs, SharedPortionGraph) if shared else (self._portion_graphs, PortionGraph)
+                if key not in graphs:
+                    graphs[key] = kind(self, *key)
+                if shared:
+                    graphs[key].shared = shared
+                logits = graphs[key].run(entries, marks[1] if marks else None)
                 if keep:
                     logits = logits.clone()
             else:
@@ -283,7 +287,7 @@ class ModelRunner:
             # their committed positions lie on), so that a later step finds the lists it expects
             for request, _ in wanted:
                 self.cache.unreserve(request)
-            for recording in (*self._graphs.values(), *self._shared_graphs.values(), *self._portion_graphs.values()):
+            for recording in (*self._graphs.values(), *self._shared_graphs.values(), *self._portion_graphs.values(), *self._shared_portion_graphs.values()):
                 recording.forget()                      # (a page list that shrank and grew again is not the list a row remembers)
             raise
         for request, count in wanted:
@@ -481,35 +485,6 @@ class DecodeGraph:
         """Work lists that depend on how the step is cut (a decode step has none)."""
 
 
-class SharedDecodeGraph(DecodeGraph):
-    """A recorded decode step whose sequences share prefixes (`shared`: the step's groups): the plan of the attention that reads them
-    once has a fixed size too, and is filled again before every replay."""
-
-    def __init__(self, runner: "ModelRunner", bucket: int, longest: int):
-        super().__init__(runner, bucket, longest)
-        self.shared: list = []
-        self._plans: dict = {}            # by sizes
-        self.ctx.shared, self.ctx.prefix_owner = [(0, 0, 0)], self     # (not empty; what it holds is the plans')
-
-    def prefix_plan(self, num_heads: int, num_kv_heads: int, head_dim: int, dtype):
-        key = (num_heads, num_kv_heads, head_dim, dtype)
-        if key not in self._plans:
-            if torch.cuda.is_current_stream_capturing():
-                raise invalid_argument("a plan first asked for inside a recording")
-            self._plans[key] = ops_RecordedPrefixPlan(self.bucket, self.longest, *key, self.device_flat.device)
-            self._fill_plan(self._plans[key])
-            self.copied.record()                             # (the next step's plan waits for this transfer too)
-        return self._plans[key].plan
-
-    def _fill_plan(self, plan) -> None:
-        live = self._rows_filled
-        plan.fill(self.host["seq_start"][:live + 1], self.host["seq_len"][:live], self.shared)
-
-    def _send_lists(self) -> None:
-        for plan in self._plans.values():
-            self._fill_plan(plan)
-
-
 class PortionGraph(DecodeGraph):
     """A recorded step of up to `tokens` tokens in up to `seqs` sequences, cut anywhere: portions
     of prompts beside single tokens, with at most `seqs` wanted rows.  Tokens beyond the step's
@@ -583,6 +558,54 @@ class PortionGraph(DecodeGraph):
                                             for entry, start, n in zip(entries, first, counts)])
             slots[total:] = -1
         return len(want)
+
+
+class _SharedPlans:
+    """What recordings of steps whose sequences share prefixes (`shared`: the step's groups) have beside others: the plan of the attention that
+    reads those once has a fixed size too, and is filled again before every replay."""
+
+    def __init__(self, runner: "ModelRunner", *sizes: int):
+        super().__init__(runner, *sizes)
+        self.shared: list = []
+        self._plans: dict = {}            # by sizes
+        self.ctx.shared, self.ctx.prefix_owner = [(0, 0, 0)], self     # (not empty; what it holds is the plans')
+
+    def _make_plan(self, *sizes):
+        return ops_RecordedPrefixPlan(self.bucket, self.longest, *sizes, self.device_flat.device)
+
+    def prefix_plan(self, num_heads: int, num_kv_heads: int, head_dim: int, dtype):
+        key = (num_heads, num_kv_heads, head_dim, dtype)
+        if key not in self._plans:
+            if torch.cuda.is_current_stream_capturing():
+                raise invalid_argument("a plan first asked for inside a recording")
+            self._plans[key] = self._make_plan(*key)
+            self._fill_plan(self._plans[key])
+            self.copied.record()                             # (the next step's plan waits for this transfer too)
+        return self._plans[key].plan
+
+    def _fill_plan(self, plan) -> None:
+        live = self._rows_filled
+        plan.fill(self.host["seq_start"][:live + 1], self.host["seq_len"][:live], self.shared)
+
+    def _send_lists(self) -> None:
+        super()._send_lists()
+        for plan in self._plans.values():
+            self._fill_plan(plan)
+
+
+class SharedDecodeGraph(_SharedPlans, DecodeGraph):
+    """A recorded decode step whose sequences share prefixes."""
+
+
+class SharedPortionGraph(_SharedPlans, PortionGraph):
+    """A recorded step of portions beside single tokens some of whose sequences share prefixes.  Sequences beyond the step's bring no tokens to
+    its plan."""
+
+    def _make_plan(self, *sizes):
+        return ops_RecordedPrefixPlan(self.bucket, self.longest, *sizes, self.device_flat.device, self.seqs)
+
+    def _fill_plan(self, plan) -> None:
+        plan.fill(self.host["seq_start"], self.host["seq_len"], self.shared)
 
 
 def _compute_units(device) -> int:

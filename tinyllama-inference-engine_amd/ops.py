@@ -2858,30 +2858,34 @@ def shared_prefix_pays(groups, num_kv_heads: int, head_dim: int) -> bool:
 
 
 class RecordedPrefixPlan:
-    """A `SharedPrefixPlan` at fixed addresses and of fixed size, for a recorded step of up to `tokens` single tokens in as many sequences of up
-    to `longest` positions: `fill` writes a step's work into it, on the current stream.  Items and parts beyond the step's have no tokens."""
+    """A `SharedPrefixPlan` at fixed addresses and of fixed size, for a recorded step of up to `tokens` tokens in up to `sequences` sequences
+    (None: single tokens, as many as those) of up to `longest` positions: `fill` writes a step's work into it, on the current stream.  Items and
+    parts beyond the step's have no tokens."""
 
     @staticmethod
-    def room(tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, compute_units: int = 256) -> tuple[int, int]:
-        """(items, parts) that it holds.  With one part each, a token has ceil(G / step) items of its own and the groups ceil(columns / step)
-        each.  The plan cuts a step into some 15/8 workgroups a compute unit (csrc/attention_prefix.hip), so there are `spread` items a kv head beside
+    def room(tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, compute_units: int = 256,
+             sequences: int | None = None) -> tuple[int, int]:
+        """(items, parts) that it holds.  With one part each, a sequence, and a group of two sequences or more, has ceil(columns / step)
+        items.  The plan cuts a step into some 15/8 workgroups a compute unit (csrc/attention_prefix.hip), so there are `spread` items a kv head beside
         those, twice that where a group's last tile is cut as its wide ones are; and a group's tile has as many parts for each of its
         tokens (with 24 a token, 32 sequences behind 30000 positions, 32 heads of 128 on 8, were cut into 16 parts for 47, and took 69.9 us for 43.9)."""
         group, step = num_heads // num_kv_heads, prefix_tile_columns(17, head_dim, dtype)
         spread = -(-15 * compute_units // (8 * num_kv_heads))
         together = max(1, prefix_tile_columns(129, head_dim, dtype) // group)                  # tokens of a wide tile
-        return (tokens * -(-group // step) + -(-tokens * group // step) + tokens // 2 + max(64, 2 * spread),
+        sequences = tokens if sequences is None else sequences
+        return (2 * -(-tokens * group // step) + sequences + sequences // 2 + max(64, 2 * spread),
                 min(PREFIX_PARTS * tokens, spread * min(tokens, 2 * together)) + 3 * tokens + spread)
 
-    def __init__(self, tokens: int, longest: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device):
+    def __init__(self, tokens: int, longest: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, device,
+                 sequences: int | None = None):
         device = torch.device(device)
         self._units = _compute_units(device) if device.type == "cuda" else 256
-        self.items, self.parts = self.room(tokens, num_heads, num_kv_heads, head_dim, dtype, self._units)
+        self.items, self.parts = self.room(tokens, num_heads, num_kv_heads, head_dim, dtype, self._units, sequences)
         self._device = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, device=device)
         self._host = torch.zeros((self.items * 8 + tokens + 1,), dtype=torch.int32, pin_memory=self._device.is_cuda)
         self._sent = torch.cuda.Event() if self._device.is_cuda else None         # the last transfer has read the host's buffer
-        self.plan = SharedPrefixPlan(self._device[:self.items * 8].view(self.items, 8), self._device[self.items * 8:], tokens, self.parts, tokens,
-                                     longest, (num_heads, num_kv_heads, head_dim, dtype))
+        self.plan = SharedPrefixPlan(self._device[:self.items * 8].view(self.items, 8), self._device[self.items * 8:], tokens, self.parts,
+                                     tokens if sequences is None else sequences, longest, (num_heads, num_kv_heads, head_dim, dtype))
 
     def fill(self, seq_start, seq_len, groups) -> None:
         import numpy as np
@@ -2889,7 +2893,7 @@ class RecordedPrefixPlan:
         host, begin = self._host.numpy(), self.items * 8
         tokens = int(seq_start[-1])
         if tokens > self.plan.tokens or len(seq_len) > self.plan.sequences:
-            raise invalid_shape(f"a recorded plan for {self.plan.tokens} tokens does not hold {tokens} in {len(seq_len)} sequences")
+            raise invalid_shape(f"a recorded plan for {self.plan.tokens} tokens in {self.plan.sequences} sequences does not hold {tokens} in {len(seq_len)}")
         longest = int(np.max(seq_len, initial=0))
         if longest > self.plan.longest:
             raise invalid_shape(f"a recorded plan for {self.plan.longest} positions does not hold a sequence of {longest}")
