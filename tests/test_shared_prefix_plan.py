@@ -271,3 +271,25 @@ def test_recorded_steps_of_portions_are_cut_as_others_are(heads, kv_heads, dim, 
                 assert plan.sequences == sequences and plan.items[:len(items)].tolist() == items.tolist() and not plan.items[len(items):].any()
                 assert plan.part_first[:start[-1] + 1].tolist() == part_first.tolist() and (plan.part_first[start[-1]:] == part_first[-1]).all()
                 assert plan.parts >= part_first[-1]
+
+
+@pytest.mark.parametrize("heads,groups,count,prefix,portion,dtype,pays", [
+    ((4, 64), 1, 64, 500, 0, torch.bfloat16, False), ((4, 64), 1, 64, 1000, 0, torch.bfloat16, True), ((4, 64), 8, 8, 1000, 0, torch.bfloat16, True),
+    ((4, 64), 8, 8, 500, 0, torch.bfloat16, False), ((4, 64), 1, 32, 2000, 0, torch.bfloat16, True), ((4, 64), 1, 8, 2000, 0, torch.bfloat16, False),
+    ((8, 128), 1, 64, 250, 0, torch.bfloat16, False), ((8, 128), 1, 64, 500, 0, torch.bfloat16, True), ((8, 128), 16, 4, 250, 0, torch.bfloat16, False),
+    ((8, 128), 1, 16, 500, 0, torch.bfloat16, True), ((8, 128), 1, 8, 1000, 0, torch.bfloat16, True), ((8, 128), 1, 2, 8000, 0, torch.bfloat16, True),
+    ((32, 64), 1, 64, 250, 0, torch.bfloat16, False), ((8, 80), 1, 64, 500, 0, torch.bfloat16, False), ((8, 80), 1, 64, 1000, 0, torch.bfloat16, True),
+    ((8, 64), 1, 64, 250, 0, torch.float32, True), ((8, 64), 1, 64, 500, 0, torch.float32, True), ((8, 128), 1, 64, 250, 0, torch.float32, True),
+    ((4, 64), 1, 4, 300, 0, torch.float32, False),
+    ((4, 64), 1, 32, 2000, 2000, torch.bfloat16, False), ((4, 64), 1, 64, 2000, 636, torch.bfloat16, True), ((4, 64), 1, 32, 2000, 1000, torch.bfloat16, False),
+    ((4, 64), 1, 16, 6000, 2000, torch.bfloat16, True), ((8, 128), 1, 32, 2000, 2000, torch.bfloat16, True), ((8, 128), 1, 32, 1500, 2000, torch.bfloat16, False),
+    ((4, 64), 1, 64, 400, 256, torch.bfloat16, True), ((4, 64), 1, 32, 2000, 2000, torch.float32, True)])
+def test_steps_take_the_faster_attention(heads, groups, count, prefix, portion, dtype, pays):
+    """Measured on both sides of each line, families that decode, alone or beside another prompt's portion."""
+    of = [(group * count, count, prefix) for group in range(groups)]
+    assert ops.shared_prefix_pays(of, *heads, dtype, groups * count + portion if portion else 0) is pays
+
+
+def test_many_short_groups_count_as_their_sum():
+    groups = [(4 * i, 4, 1200) for i in range(8)]
+    assert ops.shared_prefix_pays(groups, 8, 128) and not ops.shared_prefix_pays(groups[:1], 8, 128)

@@ -175,7 +175,12 @@ class ModelRunner:
             if family and len(shared) > 1:
                 groups.append((first, len(shared), min(shared)))
             first += len(shared)
-        return groups if groups and any(ops_shared_prefix_pays(groups, *sizes) for sizes in self._prefix_sizes) else []
+        if not groups:
+            return []
+        tokens = sum(len(entry.tokens) for entry in entries)
+        if tokens == len(entries):
+            tokens = 0                                      # (single tokens, no portion)
+        return groups if any(ops_shared_prefix_pays(groups, *sizes, self.cache.dtype, tokens) for sizes in self._prefix_sizes) else []
 
     def _length_bucket(self, longest: int) -> int:
         """The sequence length a recording is made for: the next power of two from 256 on, up to

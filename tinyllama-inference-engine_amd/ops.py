@@ -2850,11 +2850,31 @@ def shared_prefix_plan(seq_start, seq_len, groups, num_heads: int, num_kv_heads:
     return SharedPrefixPlan(both[:count * 8].view(count, 8), both[count * 8:], tokens, parts, len(seq_len), longest, sizes)
 
 
-def shared_prefix_pays(groups, num_kv_heads: int, head_dim: int) -> bool:
-    """Whether a decode step of these groups is faster through `attention_shared_prefix` than through `attention_mfma`: from four million
-    elements of keys on that are not read again (32 heads of 64 on 4, 64 sequences behind 1024 positions 13.6 us against 12.5, behind 2048 15.9 against 18.8;
-    of 128 on 8, 2 behind 1024 10.4 and 10.2, 8 behind 1024 10.0 against 13.8, 64 behind 2048 19.7 against 56.9; on 32, 4 behind 256 10.6 and 10.3)."""
-    return sum((count - 1) * prefix for _, count, prefix in groups) * num_kv_heads * head_dim >= 4_000_000
+def shared_prefix_pays(groups, num_kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, tokens: int = 0) -> bool:
+    """Whether a step of these groups is faster through `attention_shared_prefix` than through the attention that reads every sequence's keys
+    for itself.  tokens: 0 for a step of single tokens, else how many a step with portions brings.  All of it replayed, this kernel's time first.
+
+    From four million elements of keys on that are not read again (32 heads of 128 on 8, 2 sequences behind 1024 positions 10.4 us and 10.2,
+    behind 2000 10.9 and 12.1, 8 behind 1000 9.9 and 13.5; 32 of 64 on 4, 8 behind 2000 10.2 and 9.6).  That is all in 32 bits, where the other kernel is
+    slower (32 heads of 128 on 8, 64 behind 250 27 us and 71; 8 of 64 on 8 14.4 and 15.9).
+
+    Single tokens in bfloat16: and prefixes of 48 thousand / head_dim positions on average.  Behind shorter ones the other kernel finds the keys
+    in the caches, and this one has a second kernel and each sequence's own keys as items beside (64 sequences in one group, 32 heads of 64 on 4, behind
+    500 12.0 us and 9.4, behind 1000 13.3 and 12.3, behind 2000 15.6 and 17.5, in 8 groups behind 1000 12.6 and 16.4; of 128 on 8 behind 250 17.7 and 15.0,
+    behind 500 20.3 and 23.3; 24 of 80 on 8 behind 500 14.8 and 13.3, behind 1000 16.1 and 18.1).  Sequences in no group do not count (8 behind 4000, 32
+    heads of 64 on 4, and 48 of 500: 14.1 us and 29.8).
+
+    With portions in bfloat16: a step of more than 700 tokens pays for them what it saves behind a prefix shorter than 2.5 times that many, with
+    heads of more than 64 dims than 0.9 times (32 heads of 64 on 4, 32 decoding behind 2000 beside 700 tokens 33.0 us and 38.6, beside 1000 44.3 and
+    38.6, beside 2000 72.9 and 47.8, 16 behind 6000 beside 2000 73.0 and 100; of 128 on 8, 32 behind 2000 beside 2000 102 and 107, 32 portions of 60 behind
+    1500 99.5 and 83.8, of 30 56.6 and 60.0)."""
+    if sum((count - 1) * prefix for _, count, prefix in groups) * num_kv_heads * head_dim < 4_000_000:
+        return False
+    if dtype == torch.float32:
+        return True
+    if tokens == 0:
+        return sum(count * prefix for _, count, prefix in groups) * head_dim >= 48_000 * sum(count for _, count, _ in groups)
+    return tokens <= 700 or max(prefix for _, _, prefix in groups) >= tokens * (2.5 if head_dim <= 64 else 0.9)
 
 
 class RecordedPrefixPlan:
