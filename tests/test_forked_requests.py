@@ -367,3 +367,24 @@ def test_groups_are_runs_of_one_family(monkeypatch):
         for index in range(1, len(live)):
             one, other = cache.held(live[index - 1]), cache.held(live[index])
             assert (covered[index] is not None and covered[index] == covered[index - 1]) == (one.family == other.family != 0)
+
+
+def test_what_the_rows_of_a_step_ask():
+    """The same as row by row, and without looking at each when nobody asks."""
+    from tlie_amd.sampling.sampler import what_rows_ask
+    rng = random.Random(4)
+    kinds = [dict(), dict(temperature=0.7), dict(temperature=0.7, top_k=5), dict(top_k=5), dict(temperature=1.0, min_p=0.1), dict(min_p=0.1), dict(logprobs=True),
+             dict(temperature=0.5, top_k=3, min_p=0.2, logprobs=True)]
+    for _ in range(300):
+        params = [SamplingParams(**rng.choice(kinds[:rng.randint(1, len(kinds))])) for _ in range(rng.randint(1, 6))]
+        filtered = [one.temperature > 0 and (one.top_k > 0 or one.min_p > 0) for one in params]
+        assert what_rows_ask(params) == (any(one.logprobs for one in params), filtered if any(filtered) else None)
+    bare = [SimpleNamespace(temperature=0.5, top_p=1.0, seed=1)]
+    assert what_rows_ask(bare) == (False, None)
+    assert what_rows_ask(bare + [SamplingParams(temperature=0.5, top_k=2, logprobs=True)]) == (True, [False, True])
+
+    class Asked(SamplingParams):
+        @property
+        def filtered(self):
+            raise AssertionError("looked at row by row")
+    assert what_rows_ask([Asked(temperature=0.9) for _ in range(3)]) == (False, None)
