@@ -209,7 +209,8 @@ struct Seen {
     bad = bad || !(v.x < INFINITY) || !(v.y < INFINITY) || !(v.z < INFINITY) || !(v.w < INFINITY);
     const float here = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
     float low = fminf(fminf(v.x, v.y), fminf(v.z, v.w));
-    if (low == -INFINITY) {                                       // (a token that cannot be drawn, or none: of the others)
+    // a token that cannot be drawn, or none: of the others.  (A branch of the wave: taken lane by lane, 256 rows of 128256 tokens take 89.0 us for 88.4)
+    if (__builtin_amdgcn_ballot_w64(low == -INFINITY) != 0) {
       const float none = INFINITY;
       low = fminf(fminf(v.x > -INFINITY ? v.x : none, v.y > -INFINITY ? v.y : none), fminf(v.z > -INFINITY ? v.z : none, v.w > -INFINITY ? v.w : none));
       auto cannot = [&](int i, float x) { return x == -INFINITY && i >= begin && i < end; };
