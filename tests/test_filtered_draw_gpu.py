@@ -350,3 +350,16 @@ def test_log_probabilities_of_mass_far_below_the_maximum(rows, vocab, gap):
     want = torch.log_softmax(wide, dim=1).gather(1, tokens.cpu().long().unsqueeze(1)).squeeze(1)
     bound = (2.0 + 1.2 * mean) * 2.0 ** -23 + 2.0 ** -24 * want.abs()
     assert float(((logprobs.double().cpu() - want).abs() - bound).max()) <= 0.0
+
+
+@pytest.mark.parametrize("t", [1e-3, 1.0, 1e10, 1e18, 1e20, 1e37, math.inf])
+@pytest.mark.parametrize("rows,vocab", [(9, 900), (9, 4000), (2, 60000)])
+def test_min_p_of_one_at_any_temperature(rows, vocab, t):
+    """Kept is what weighs as much as the largest in 64 bits: equal logits, and at a temperature beyond 10^17 times the logits all of them."""
+    logits, _, gen = rows_of(vocab + 5, rows, vocab)
+    logits[:, [3, 600]] = 25.0
+    ones = torch.ones(rows)
+    for u in (0.0, 0.3, 0.77, 0.999):
+        check(logits, u * ones, temperature=t * ones, min_p=ones)
+        check(logits, u * ones, temperature=t * ones, min_p=ones, top_p=0.7 * ones, top_k=torch.full((rows,), 300).int())
+        check(logits, u * ones, temperature=t * ones, min_p=(1 - 2.0 ** -24) * ones)

@@ -474,7 +474,8 @@ __device__ RowState find_classes(ClassShared<THREADS>& s, const RowScale& scale,
   }
   if (ask.floor > 0.f) {
     // the class of the gap at which the weight is min_p, and its neighbours, for the rounding of the gap
-    const float gap = fmaxf(-logf(fminf(ask.floor, 1.f)) * ask.t, 0.f);
+    // (2^-52 at the least: so near the first token every weight is rounded to the largest's, which at a high temperature may be all of them)
+    const float gap = fmaxf(-logf(fminf(ask.floor, 1.f)), 2.220446e-16f) * ask.t;
     const int c = static_cast<int>(fminf(gap * scale.class_scale, static_cast<float>(kClasses - 1)));
     want(c - 1, c + 1);
     state.kept_floor = max(one, mass_upto(c - 2));
