@@ -363,3 +363,37 @@ def test_min_p_of_one_at_any_temperature(rows, vocab, t):
         check(logits, u * ones, temperature=t * ones, min_p=ones)
         check(logits, u * ones, temperature=t * ones, min_p=ones, top_p=0.7 * ones, top_k=torch.full((rows,), 300).int())
         check(logits, u * ones, temperature=t * ones, min_p=(1 - 2.0 ** -24) * ones)
+
+
+@pytest.mark.parametrize("t", [1.0, 1e18, 1e24, math.inf])
+def test_min_p_above_one_at_any_temperature(t):
+    logits, uniform, _ = rows_of(77, 24, 3000)
+    got = check(logits, uniform, temperature=torch.full((24,), t), min_p=torch.full((24,), 1.5))
+    assert torch.equal(got.cpu().long(), logits.argmax(dim=1))
+
+
+@pytest.mark.parametrize("t", [2.0 ** 42, 2.0 ** 46, 2.0 ** 50, 2.0 ** 54])
+@pytest.mark.parametrize("rows,vocab", [(9, 700), (9, 3000), (2, 60000)])
+def test_min_p_of_one_where_some_weights_are_the_largests_in_64_bits(rows, vocab, t):
+    """Gaps of x T 2^-54: exp(-x 2^-54) = 1 - x 2^-54 (the square is below 2^-100) lies x / 2 of a step of 2^-53 below 1, and is 1 when rounded for
+    x < 1 and less for x > 1.  So what is kept, with equal weights, is known without an exponential (numpy's gives less than 1 from
+    x = 0.9 on), and the token is the first of which more than u of them stand no later."""
+    gen = torch.Generator().manual_seed(vocab)
+    steps = torch.randint(1, 40, (rows, vocab), generator=gen).double() + 0.25
+    steps[:, 11] = 0.0
+    fewer = steps * 0.3
+    fewer[:, 12] = 1.2
+    for x, k in ((steps, 0), (steps, 5), (fewer, 0), (fewer, 17)):
+        logits = (-x * (t * 2.0 ** -54)).float()                  # (x of few bits, or rounded to 2^-24 of it: none near 1 but 0.975 and 1.275)
+        order = np.lexsort((np.broadcast_to(np.arange(vocab), (rows, vocab)), -logits.numpy()), axis=1)
+        for u in (0.0, 0.3, 0.77, 0.999):
+            number = float(np.float32(u))
+            want = []
+            for row in range(rows):
+                kept = int((x[row] < 1.0).sum())
+                kept = min(kept, k) if k else kept
+                want.append(order[row, min(kept - 1, int(number * kept))])
+            ones = torch.ones(rows, device=DEV)
+            got = ops.sample_filtered(logits.to(DEV), number * ones, t * ones, min_p=ones,
+                                      top_k=torch.full((rows,), k, dtype=torch.int32, device=DEV))
+            np.testing.assert_array_equal(got.cpu().numpy(), np.array(want))

@@ -472,14 +472,17 @@ __device__ RowState find_classes(ClassShared<THREADS>& s, const RowScale& scale,
     want(c_lo, c_hi);
     kept_lo = mass_upto(c_lo - 1), kept_hi = min(kept_hi, mass_upto(c_hi));
   }
-  if (ask.floor > 0.f) {
-    // the class of the gap at which the weight is min_p, and its neighbours, for the rounding of the gap
-    // (2^-52 at the least: so near the first token every weight is rounded to the largest's, which at a high temperature may be all of them)
-    const float gap = fmaxf(-logf(fminf(ask.floor, 1.f)), 2.220446e-16f) * ask.t;
-    const int c = static_cast<int>(fminf(gap * scale.class_scale, static_cast<float>(kClasses - 1)));
-    want(c - 1, c + 1);
-    state.kept_floor = max(one, mass_upto(c - 2));
-    kept_lo = min(kept_lo, state.kept_floor), kept_hi = min(kept_hi, mass_upto(c + 1));
+  if (ask.floor > 1.f) {
+    kept_lo = kept_hi = one;                                      // (no weight reaches it)
+  } else if (ask.floor > 0.f) {
+    // The class of the gap at which the weight is min_p, and its neighbours, for the rounding of the gap; of 1, up to the gap of 2^-52 T: nearer weights
+    // may be rounded to the largest's, which at a very high temperature can be every token's.
+    auto class_at = [&](float gap) { return static_cast<int>(fminf(gap * scale.class_scale, static_cast<float>(kClasses - 1))); };
+    const float gap = fmaxf(-logf(ask.floor), 0.f);
+    const int first = gap > 0.f ? class_at(gap * ask.t) : 0, last = class_at(fmaxf(gap, 2.220446e-16f) * ask.t);
+    want(first - 1, last + 1);
+    state.kept_floor = max(one, mass_upto(first - 2));
+    kept_lo = min(kept_lo, state.kept_floor), kept_hi = min(kept_hi, mass_upto(last + 1));
   }
   kept_lo = max(kept_lo, one), kept_hi = max(kept_hi, one);       // (the first token is always kept)
   const uint64_t goal = goal_of(ask.u, kept_lo);
